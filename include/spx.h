@@ -364,6 +364,122 @@ SPX_API int spx_hot_append(const void* k, const void* v, int64_t k_stride_b, int
                            void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * Per-head RMS norms of queries and keys with the position rotation in the same pass
+ * (models whose attention normalises each head before the rotation).  For each token row
+ * (b, t) and head, in float32, rounded once to dtype at the store:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight           (weight: head_dim values, q and k their own)
+ *   out[i] = y[i] c_i - y[i + h] s_i,  out[i + h] = y[i + h] c_i + y[i] s_i,  h = head_dim / 2
+ * with c, s the first half of the tables' row at the token's position (clamped to the
+ * table).  Queries are always rotated, keys only with rotate_keys (this library's cache
+ * holds keys before the rotation).  Inputs are rows of heads x head_dim values, so views
+ * of a packed q|k|v projection can be passed; outputs are head-major.
+ * ------------------------------------------------------------------------------- */
+typedef struct spx_qk_norm_args {
+  int32_t batch, tokens;       /* >= 0; nothing is launched when either is 0 */
+  int32_t num_q_heads;         /* >= 1 */
+  int32_t num_kv_heads;        /* >= 0; 0: queries only */
+  int32_t head_dim;            /* even, 2..1024 */
+  int32_t dtype;               /* spx_dtype of inputs, weights and outputs */
+  int32_t rope_len;            /* rows of the tables */
+  int32_t rotate_keys;
+  float eps;
+  int32_t reserved;            /* 0 */
+  const void* q;               /* element (b, t, h, d) at b*q_stride_b + t*q_stride_t + h*head_dim + d */
+  const void* k;               /* likewise with the k strides; may be NULL when num_kv_heads is 0 */
+  int64_t q_stride_b, q_stride_t, k_stride_b, k_stride_t;
+  const void* q_weight;        /* [head_dim] */
+  const void* k_weight;        /* [head_dim] */
+  const float* cos_table;      /* f32 [rope_len][head_dim] */
+  const float* sin_table;
+  const int64_t* pos;          /* position of (b, t) at b*pos_stride_b + t*pos_stride_t; NULL: pos_start + t */
+  int64_t pos_stride_b, pos_stride_t, pos_start;
+  void* q_out;                 /* [batch][num_q_heads][tokens][head_dim] */
+  void* k_out;                 /* element (b, h, t, d) at b*k_out_stride_b + h*k_out_stride_h + t*head_dim + d */
+  int64_t k_out_stride_b, k_out_stride_h;
+} spx_qk_norm_args;
+
+SPX_API int spx_qk_norm_rope(const spx_qk_norm_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside one shared projection.  Slot a of a pool
+ * holds, for each of `parts` column ranges of the projection (q | k | v, or one part),
+ * A [rank][in] and B [width][rank]; row r of the batch uses one slot or none:
+ *   out[r] = y[r] + scale[a][p] * B[a][p] (A[a][p] x[r]),   out[r] = y[r] without a slot.
+ * The inner product A x is held in float32, split into two values of dtype for the
+ * second product (so its rounding does not show in the result), and the sum is rounded
+ * once.  Rows are taken through `order`, grouped in tiles of one slot.
+ * ------------------------------------------------------------------------------- */
+#define SPX_LORA_MAX_PARTS 4
+#define SPX_LORA_MAX_RANK 128
+typedef struct spx_lora_args {
+  int32_t num_tiles;           /* tiles of up to tile_rows rows of one slot */
+  int32_t tile_rows;           /* 16 or 32 */
+  int32_t num_rows;            /* entries of order */
+  int32_t in_features;         /* multiple of 8 */
+  int32_t parts;               /* 1..SPX_LORA_MAX_PARTS */
+  int32_t part_width[SPX_LORA_MAX_PARTS];  /* columns of each part, multiples of 8; they are adjacent in y and out */
+  int32_t max_rank;            /* stored rank: multiple of 16, <= SPX_LORA_MAX_RANK */
+  int32_t slots;
+  int32_t dtype;               /* SPX_F16 or SPX_BF16: x, y, A, B, out */
+  const void* x;               /* row r at x + r*x_stride; 16-byte aligned rows */
+  const void* y;
+  void* out;                   /* may be y itself (same stride) */
+  int64_t x_stride, y_stride, out_stride;
+  const void* a;               /* [slots][parts][max_rank][in_features] */
+  const void* b;               /* [slots][sum of part_width][max_rank], zero past the slot's rank */
+  const int32_t* ranks;        /* [slots][parts]: rank in use, 0 = nothing loaded */
+  const float* scales;         /* [slots][parts] */
+  const int32_t* tiles;        /* [num_tiles][4]: slot (-1 none), first entry of order, rows, 0 */
+  const int32_t* order;        /* [num_rows]: row of x, y and out */
+  float* workspace;            /* f32 [num_rows][parts*max_rank]: the inner products */
+  size_t workspace_bytes;
+} spx_lora_args;
+
+SPX_API size_t spx_lora_workspace_size(const spx_lora_args* args);
+SPX_API int spx_lora_add(const spx_lora_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Rules on a decode step's logits, and the greedy choice under them, in one pass.  Row b
+ * of logits [batch][vocab], each operation rounded in float32:
+ *   seen (prompt or output):  l = l > 0 ? l / repetition : l * repetition
+ *   l = l - frequency * count;  l = l - presence when count > 0;  l = l + bias[token]
+ *   l = -inf where the allow bit is clear
+ * out (optional) is l rounded to dtype; token (optional) is the index of the largest l
+ * before that rounding: the lowest index among equals, a NaN counts as largest, 0 when
+ * every token is at -inf.  record: the chosen token is then added to the output history.
+ * Bit t % 32 of word t / 32 stands for token t in every bitmap; W = ceil(vocab / 32).
+ * ------------------------------------------------------------------------------- */
+typedef struct spx_logits_args {
+  int32_t batch, vocab;
+  int32_t dtype;               /* of logits and out */
+  int32_t record;
+  const void* logits;
+  int64_t logits_stride;       /* elements between rows */
+  void* out;                   /* may be logits itself */
+  int64_t out_stride;
+  int64_t* token;              /* [batch] */
+  const float* repetition;     /* [batch], > 0; NULL: none */
+  const float* frequency;      /* [batch]; NULL: none */
+  const float* presence;       /* [batch]; NULL: none */
+  const uint32_t* prompt_bits; /* [batch][W] */
+  uint32_t* output_bits;       /* [batch][W] */
+  int32_t* counts;             /* [batch][vocab]: times each token was put out */
+  const uint32_t* bias_bits;   /* [batch][W]: tokens with a bias; NULL: none */
+  const int32_t* bias_rows;    /* [batch + 1]: range of each row in bias_tokens */
+  const int32_t* bias_tokens;  /* ascending within a row */
+  const float* bias_values;
+  const uint32_t* allow;       /* row b at allow + b*allow_stride; NULL: every token allowed */
+  int64_t allow_stride;        /* words between rows, 0: one row for all */
+} spx_logits_args;
+
+SPX_API int spx_logits_rules(const spx_logits_args* args, void* stream);
+
+/* Tokens [batch][count] (int64, rows `stride` apart) added to the history: to the bitmap,
+ * and to counts when it is not NULL.  Values outside [0, vocab) are skipped (padding). */
+SPX_API int spx_logits_observe(const int64_t* tokens, int64_t stride, int batch, int count, int vocab, uint32_t* bits,
+                               int32_t* counts, void* stream);
+
+/* ---------------------------------------------------------------------------------
  * Utilities.
  * ------------------------------------------------------------------------------- */
 SPX_API int spx_abi_version(void);

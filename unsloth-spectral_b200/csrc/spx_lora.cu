@@ -1,0 +1,429 @@
+// Low-rank adapters of many requests beside one shared projection (spx_lora_add,
+// include/spx.h):  out[r] = y[r] + scale * B[a] (A[a] x[r]),  a = the slot of row r.
+// Two kernels over tiles of rows of one slot:
+//   shrink  t = A x      (K = in_features is long, the result has `rank` columns: the warps
+//                         and the CTAs of a cluster split K, the partial sums meet in
+//                         shared and distributed shared memory in a fixed order)
+//   expand  out = y + scale * B t   (each warp owns 64 output columns and keeps their B
+//                         fragments in registers over the tile's rows)
+// Both are streams with little arithmetic (2 * rank flops a value of x and of y), so the
+// operands go from global memory straight into mma fragments.  The sum over k may take its
+// terms in any order, so lane c of a quad takes k = 8c..8c+7 of 32 as the k of two
+// m16n8k16 steps (16-byte loads, whole sectors); the same choice over the output columns
+// gives 16-byte accesses of y and out.
+// t is kept in float32; for the second product it is split into a high and a low value of
+// the row type (two MMAs), which keeps about 16 (bf16) or 22 (f16) bits of it.
+#include <cooperative_groups.h>
+
+#include "spx_common.cuh"
+
+namespace spx {
+namespace lora {
+
+namespace cg = cooperative_groups;
+
+constexpr int SW = 8;    // warps of a shrink CTA
+constexpr int EW = 4;    // warps of an expand CTA
+
+struct Params {
+  const void *x, *y, *a, *b;
+  void* out;
+  int64_t xs, ys, os;
+  const int32_t* ranks;
+  const float* scales;
+  const int4* tiles;
+  const int32_t* order;
+  float* t;
+  int K, parts, R, SR, OUT;
+  int width[SPX_LORA_MAX_PARTS];
+};
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                   uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack2(__half lo, __half hi) {
+  return (uint32_t)__half_as_ushort(lo) | ((uint32_t)__half_as_ushort(hi) << 16);
+}
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16 lo, __nv_bfloat16 hi) {
+  return (uint32_t)__bfloat16_as_ushort(lo) | ((uint32_t)__bfloat16_as_ushort(hi) << 16);
+}
+
+// ------------------------------------------------------------------------- shrink ----
+// Tile of 16 * MT rows x 8 * NT of the parts * max_rank columns; the CTAs of a cluster and
+// their warps take the 32-wide steps of k in turn.
+template <typename T, int MT, int NT>
+__global__ void __launch_bounds__(SW * 32) shrink_kernel(const Params p) {
+  extern __shared__ float sums[];   // [SW][MT * 16][NT * 8]
+  cg::cluster_group cl = cg::this_cluster();
+  const int cs = (int)cl.num_blocks(), cr = (int)cl.block_rank();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int4 tile = p.tiles[blockIdx.x / cs];
+  if (tile.x < 0) return;   // rows without an adapter: the whole cluster leaves
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int col0 = blockIdx.y * (NT * 8);
+  const T* xr[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = m * 16 + h * 8 + g;
+      xr[m][h] = r < tile.z ? static_cast<const T*>(p.x) + (int64_t)p.order[tile.y + r] * p.xs + 8 * c : nullptr;
+    }
+  uint32_t act = 0;   // column groups of eight that hold a rank in use
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int col = col0 + n * 8;
+    if (col < p.SR && col % p.R < p.ranks[tile.x * p.parts + col / p.R]) act |= 1u << n;
+  }
+  const T* ar = static_cast<const T*>(p.a) + ((int64_t)tile.x * p.SR + col0 + g) * p.K + 8 * c;
+  float acc[MT][NT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
+  const int steps = (p.K + 31) / 32;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  if (act) {
+#pragma unroll 2
+    for (int s = cr * SW + warp; s < steps; s += cs * SW) {
+      const bool in = s * 32 + 8 * c < p.K;
+      uint4 xa[MT][2], bw[NT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          xa[m][h] = in && xr[m][h] ? *reinterpret_cast<const uint4*>(xr[m][h] + s * 32) : zero;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        bw[n] = in && ((act >> n) & 1u) ? *reinterpret_cast<const uint4*>(ar + (int64_t)n * 8 * p.K + s * 32) : zero;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma<T>(acc[m][n], xa[m][0].x, xa[m][1].x, xa[m][0].y, xa[m][1].y, bw[n].x, bw[n].y);
+          mma<T>(acc[m][n], xa[m][0].z, xa[m][1].z, xa[m][0].w, xa[m][1].w, bw[n].z, bw[n].w);
+        }
+    }
+  }
+  constexpr int N = NT * 8, E = MT * 16 * N;
+  float* mine = sums + warp * E;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      *reinterpret_cast<float2*>(mine + (m * 16 + g) * N + n * 8 + 2 * c) = make_float2(acc[m][n][0], acc[m][n][1]);
+      *reinterpret_cast<float2*>(mine + (m * 16 + g + 8) * N + n * 8 + 2 * c) = make_float2(acc[m][n][2], acc[m][n][3]);
+    }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += SW * 32) {   // each thread its own elements: in place
+    float v = sums[e];
+#pragma unroll
+    for (int w = 1; w < SW; ++w) v += sums[w * E + e];
+    sums[e] = v;
+  }
+  cl.sync();
+  for (int e = cr * SW * 32 + threadIdx.x; e < E; e += cs * SW * 32) {
+    const int r = e / N, col = col0 + e % N;
+    float v = 0.f;
+    for (int k = 0; k < cs; ++k) v += cl.map_shared_rank(sums, k)[e];
+    if (r < tile.z && col < p.SR) {
+      // past the rank: exact zeros, also where x holds an infinity
+      if (col % p.R >= p.ranks[tile.x * p.parts + col / p.R]) v = 0.f;
+      p.t[(int64_t)(tile.y + r) * p.SR + col] = v;
+    }
+  }
+  cl.sync();   // no CTA leaves while its shared memory may be read
+}
+
+// ------------------------------------------------------------------------- expand ----
+// KS = max_rank / 16 steps of k; a warp owns NC * 8 columns of one part.
+template <typename T, int KS, int NC>
+__global__ void __launch_bounds__(EW * 32) expand_kernel(const Params p) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  int grp = blockIdx.y * EW + (threadIdx.x >> 5), part = 0, first = 0;
+  while (part < p.parts) {   // the part that this group of columns lies in
+    const int n = (p.width[part] + NC * 8 - 1) / (NC * 8);
+    if (grp < n) break;
+    grp -= n;
+    first += p.width[part];
+    ++part;
+  }
+  if (part == p.parts) return;
+  const int col0 = grp * NC * 8, left = p.width[part] - col0;   // columns of this part from col0 on
+  const int4 tile = p.tiles[blockIdx.x];
+  const int rank = tile.x < 0 ? 0 : p.ranks[tile.x * p.parts + part];
+  const float scale = tile.x < 0 ? 0.f : p.scales[tile.x * p.parts + part];
+  // B fragments: k of the lane in step ks is ks * 16 + 4c..4c+3; column of n-tile 4q + j,
+  // n = g, is 32q + 8 (g / 2) + 2j + g % 2, so that a lane's results are 8 adjacent columns
+  uint2 bw[NC][KS];
+  if (rank > 0) {
+    const T* bb = static_cast<const T*>(p.b) + ((int64_t)tile.x * p.OUT + first + col0) * p.R + 4 * c;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int col = (n / 4) * 32 + 8 * (g >> 1) + 2 * (n % 4) + (g & 1);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        bw[n][ks] = col < left && ks * 16 < rank ? *reinterpret_cast<const uint2*>(bb + (int64_t)col * p.R + ks * 16)
+                                                 : make_uint2(0u, 0u);
+    }
+  }
+  // t of the shrink kernel; also before the first store, so that this grid never ends
+  // before the one that still reads x and writes the workspace
+  bool waited = false;
+  for (int m = 0; m * 16 < tile.z; ++m) {
+    int64_t row[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = m * 16 + h * 8 + g;
+      row[h] = r < tile.z ? p.order[tile.y + r] : -1;
+    }
+    uint4 yv[NC / 4][2];
+#pragma unroll
+    for (int q = 0; q < NC / 4; ++q)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (row[h] >= 0 && q * 32 + 8 * c < left)
+          yv[q][h] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.y) + row[h] * p.ys + first + col0 +
+                                                     q * 32 + 8 * c);
+    float acc[NC][4];
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+    float un[2] = {1.f, 1.f};
+    if (!waited) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      waited = true;
+    }
+    if (rank > 0) {
+      float4 tv[KS][2];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          tv[ks][h] = row[h] >= 0 && ks * 16 < rank
+                          ? *reinterpret_cast<const float4*>(p.t + (int64_t)(tile.y + m * 16 + h * 8 + g) * p.SR +
+                                                             part * p.R + ks * 16 + 4 * c)
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
+      if (sizeof(T) == 2 && !__is_same(T, __nv_bfloat16)) {
+        // f16: the row is scaled by a power of two so that its largest value is near 2^8
+        // (no overflow of the high parts, no underflow of the low parts), and back below
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+            mx = fmaxf(fmaxf(fmaxf(fabsf(tv[ks][h].x), fabsf(tv[ks][h].y)), fmaxf(fabsf(tv[ks][h].z), fabsf(tv[ks][h].w))), mx);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          int ex = (int)((__float_as_uint(mx) >> 23) & 0xff) - 127 - 8;
+          ex = max(-118, min(118, ex));
+          const float dn = __uint_as_float((uint32_t)(127 - ex) << 23);
+          un[h] = __uint_as_float((uint32_t)(127 + ex) << 23);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+            tv[ks][h].x *= dn, tv[ks][h].y *= dn, tv[ks][h].z *= dn, tv[ks][h].w *= dn;
+        }
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (ks * 16 >= rank) break;
+        uint32_t hi[4], lo[4];   // a0..a3: row g k-pair 0, row g + 8 k-pair 0, row g k-pair 1, row g + 8 k-pair 1
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4 v = tv[ks][e & 1];
+          const float f0 = e < 2 ? v.x : v.z, f1 = e < 2 ? v.y : v.w;
+          const T h0 = from_f<T>(f0), h1 = from_f<T>(f1);
+          // an infinity has no low part
+          const float l0 = fabsf(to_f(h0)) < INFINITY ? f0 - to_f(h0) : 0.f;
+          const float l1 = fabsf(to_f(h1)) < INFINITY ? f1 - to_f(h1) : 0.f;
+          hi[e] = pack2(h0, h1);
+          lo[e] = pack2(from_f<T>(l0), from_f<T>(l1));
+        }
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+          mma<T>(acc[n], lo[0], lo[1], lo[2], lo[3], bw[n][ks].x, bw[n][ks].y);
+          mma<T>(acc[n], hi[0], hi[1], hi[2], hi[3], bw[n][ks].x, bw[n][ks].y);
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float sc = scale * un[h];
+#pragma unroll
+      for (int q = 0; q < NC / 4; ++q) {
+        if (row[h] < 0 || q * 32 + 8 * c >= left) continue;
+        uint4 o = yv[q][h];
+        if (rank > 0) {
+          T* oe = reinterpret_cast<T*>(&o);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              oe[2 * j + e] = from_f<T>(fmaf(sc, acc[4 * q + j][2 * h + e], to_f(oe[2 * j + e])));
+        }
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row[h] * p.os + first + col0 + q * 32 + 8 * c) = o;
+      }
+    }
+  }
+}
+
+template <typename T, int MT, int NT>
+int launch_shrink(const Params& p, int tiles, int groups, int cs, cudaStream_t st) {
+  const size_t smem = (size_t)SW * MT * 16 * NT * 8 * sizeof(float);
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(shrink_kernel<T, MT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)smem);
+    if (e != cudaSuccess) {
+      set_error("lora shrink_kernel: %s", cudaGetErrorString(e));
+      return SPX_ERR_CUDA;
+    }
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(tiles * cs), (unsigned)groups);
+  cfg.blockDim = dim3(SW * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cs, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, shrink_kernel<T, MT, NT>, p);
+  if (e != cudaSuccess) {
+    set_error("lora shrink_kernel: %s", cudaGetErrorString(e));
+    return SPX_ERR_CUDA;
+  }
+  return launch_status("lora shrink_kernel");
+}
+
+template <typename T, int KS, int NC>
+int launch_expand(const Params& p, int tiles, cudaStream_t st) {
+  int groups = 0;
+  for (int s = 0; s < p.parts; ++s) groups += (p.width[s] + NC * 8 - 1) / (NC * 8);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)tiles, (unsigned)((groups + EW - 1) / EW));
+  cfg.blockDim = dim3(EW * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, expand_kernel<T, KS, NC>, p);
+  if (e != cudaSuccess) {
+    set_error("lora expand_kernel: %s", cudaGetErrorString(e));
+    return SPX_ERR_CUDA;
+  }
+  return launch_status("lora expand_kernel");
+}
+
+template <typename T>
+int launch(const Params& p, int tiles, int tile_rows, cudaStream_t st) {
+  const int groups = (p.SR + 63) / 64;                            // of up to 64 columns
+  const int nt = ((p.SR / 8 + groups - 1) / groups + 1) / 2 * 2;  // 2, 4, 6 or 8
+  // CTAs that share a tile's k: until the grid fills the SMs, with at least two steps of 32
+  // for each warp, 8 at most (the portable cluster size).
+  int cs = 1;
+  while (cs < 8 && (int64_t)tiles * groups * cs < 148 && p.K >= 32 * SW * 2 * cs) cs *= 2;
+  int rc;
+  if (tile_rows == 16) {
+    rc = nt == 2   ? launch_shrink<T, 1, 2>(p, tiles, groups, cs, st)
+         : nt == 4 ? launch_shrink<T, 1, 4>(p, tiles, groups, cs, st)
+         : nt == 6 ? launch_shrink<T, 1, 6>(p, tiles, groups, cs, st)
+                   : launch_shrink<T, 1, 8>(p, tiles, groups, cs, st);
+  } else {
+    rc = nt == 2   ? launch_shrink<T, 2, 2>(p, tiles, groups, cs, st)
+         : nt == 4 ? launch_shrink<T, 2, 4>(p, tiles, groups, cs, st)
+         : nt == 6 ? launch_shrink<T, 2, 6>(p, tiles, groups, cs, st)
+                   : launch_shrink<T, 2, 8>(p, tiles, groups, cs, st);
+  }
+  if (rc != SPX_OK) return rc;
+  switch (p.R / 16) {
+    case 1: return launch_expand<T, 1, 8>(p, tiles, st);
+    case 2: return launch_expand<T, 2, 8>(p, tiles, st);
+    case 3: return launch_expand<T, 3, 8>(p, tiles, st);
+    case 4: return launch_expand<T, 4, 8>(p, tiles, st);
+    case 5:
+    case 6: return launch_expand<T, 6, 4>(p, tiles, st);
+    default: return launch_expand<T, 8, 4>(p, tiles, st);
+  }
+}
+
+static int validate(const spx_lora_args* a) {
+  SPX_REQUIRE(a, SPX_ERR_NULL, "spx_lora_add: args are required");
+  SPX_REQUIRE(a->dtype == SPX_F16 || a->dtype == SPX_BF16, SPX_ERR_UNSUPPORTED,
+              "spx_lora_add: dtype must be F16 or BF16");
+  SPX_REQUIRE(a->num_tiles >= 0 && a->num_rows >= 0 && (a->tile_rows == 16 || a->tile_rows == 32) &&
+                  a->num_tiles <= (1 << 27),
+              SPX_ERR_SHAPE, "spx_lora_add: bad tiling: %d tiles of %d rows", a->num_tiles, a->tile_rows);
+  SPX_REQUIRE(a->in_features >= 8 && a->in_features % 8 == 0 && a->in_features <= (1 << 24), SPX_ERR_SHAPE,
+              "spx_lora_add: in_features %d must be a multiple of 8", a->in_features);
+  SPX_REQUIRE(a->parts >= 1 && a->parts <= SPX_LORA_MAX_PARTS && a->slots >= 1 && a->max_rank >= 16 &&
+                  a->max_rank % 16 == 0 && a->max_rank <= SPX_LORA_MAX_RANK,
+              SPX_ERR_SHAPE, "spx_lora_add: bad pool: %d parts, %d slots, max_rank %d", a->parts, a->slots, a->max_rank);
+  int64_t out = 0;
+  for (int s = 0; s < a->parts; ++s) {
+    SPX_REQUIRE(a->part_width[s] >= 8 && a->part_width[s] % 8 == 0 && a->part_width[s] <= (1 << 22), SPX_ERR_SHAPE,
+                "spx_lora_add: width %d of part %d must be a multiple of 8", a->part_width[s], s);
+    out += a->part_width[s];
+  }
+  if (a->num_tiles == 0) return SPX_OK;
+  SPX_REQUIRE(a->x && a->y && a->out && a->a && a->b && a->ranks && a->scales && a->tiles && a->order, SPX_ERR_NULL,
+              "spx_lora_add: every pointer is required");
+  SPX_REQUIRE(a->x_stride >= a->in_features && a->y_stride >= out && a->out_stride >= out, SPX_ERR_SHAPE,
+              "spx_lora_add: a row stride is shorter than a row");
+  SPX_REQUIRE(aligned16(a->x) && aligned16(a->y) && aligned16(a->out) && aligned16(a->a) && aligned16(a->b) &&
+                  aligned16(a->tiles) && aligned16(a->workspace) &&
+                  (a->x_stride | a->y_stride | a->out_stride) % 8 == 0,
+              SPX_ERR_ALIGN, "spx_lora_add: rows of x, y and out, A, B, tiles and workspace must start on 16 bytes");
+  return SPX_OK;
+}
+
+}  // namespace lora
+}  // namespace spx
+
+using namespace spx;
+
+size_t spx_lora_workspace_size(const spx_lora_args* a) {
+  if (!a || lora::validate(a) != SPX_OK) return 0;
+  return (size_t)a->num_rows * a->parts * a->max_rank * sizeof(float);
+}
+
+int spx_lora_add(const spx_lora_args* a, void* stream) {
+  const int rc = lora::validate(a);
+  if (rc != SPX_OK || a->num_tiles == 0) return rc;
+  const size_t need = (size_t)a->num_rows * a->parts * a->max_rank * sizeof(float);
+  SPX_REQUIRE(a->workspace && a->workspace_bytes >= need, SPX_ERR_WORKSPACE,
+              "spx_lora_add: workspace of %zu bytes needed, %zu given", need, a->workspace ? a->workspace_bytes : 0);
+  lora::Params p{};
+  p.x = a->x, p.y = a->y, p.a = a->a, p.b = a->b, p.out = a->out;
+  p.xs = a->x_stride, p.ys = a->y_stride, p.os = a->out_stride;
+  p.ranks = a->ranks, p.scales = a->scales;
+  p.tiles = static_cast<const int4*>(static_cast<const void*>(a->tiles));
+  p.order = a->order, p.t = a->workspace;
+  p.K = a->in_features, p.parts = a->parts, p.R = a->max_rank, p.SR = a->parts * a->max_rank;
+  for (int s = 0; s < a->parts; ++s) p.width[s] = a->part_width[s], p.OUT += a->part_width[s];
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return a->dtype == SPX_BF16 ? lora::launch<__nv_bfloat16>(p, a->num_tiles, a->tile_rows, st)
+                              : lora::launch<__half>(p, a->num_tiles, a->tile_rows, st);
+}

@@ -1,0 +1,235 @@
+// Per-head RMS norms of queries and keys with the position rotation in the same pass
+// (spx_qk_norm_rope, include/spx.h).  For a head vector x of D values, h = D / 2:
+//   y = x * rsqrt(sum(x^2) / D + eps) * w,   out = (y1 c - y2 s, y2 c + y1 s)
+// Everything between the load and the store is float32 (one rounding, at the store: the
+// norm's output never exists in the row type, so nothing is lost between it and the
+// rotation).  Bound by memory: each value is read once and written once; the tables' rows
+// come from L2 and are held in registers over the heads of a token.
+#include "spx_common.cuh"
+
+namespace spx {
+namespace qkn {
+
+constexpr int WARPS = 8;
+
+struct Params {
+  const void *q, *k, *qw, *kw;
+  void *qo, *ko;
+  const float *cosT, *sinT;
+  const int64_t* pos;
+  int64_t qsb, qst, ksb, kst, psb, pst, pos0, kob, koh;
+  int64_t rows;
+  int T, Hq, H, D, len, rotk;
+  float eps;
+  int wpr;   // warps that share the heads of one token row
+};
+
+__device__ __forceinline__ int64_t position(const Params& p, int64_t b, int64_t t) {
+  const int64_t v = p.pos ? p.pos[b * p.psb + t * p.pst] : p.pos0 + t;
+  return v < 0 ? 0 : (v >= p.len ? p.len - 1 : v);
+}
+
+// Eight consecutive values of the row type, as loaded.
+template <typename T>
+struct Raw {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ float get(int e) const { return to_f(reinterpret_cast<const T*>(v)[e]); }
+  __device__ __forceinline__ void set(int e, float f) { reinterpret_cast<T*>(v)[e] = from_f<T>(f); }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
+  }
+};
+
+// G lanes hold one head vector: lane l its values 8l..8l+7 of both halves, so that the two
+// values of a rotation meet in one lane and only the sum of squares crosses lanes.
+template <typename T, int G, int U>
+__device__ __forceinline__ void heads(const T* src, T* dst, int64_t dst_h, const T* w, int j, int n, int step, int l,
+                                      bool on, int h, const float (&c)[8], const float (&s)[8], float eps) {
+  if (j >= n) return;   // uniform over the G lanes; the shuffles below name them alone
+  const unsigned mask = G == 32 ? 0xffffffffu : ((1u << (G & 31)) - 1u) << ((threadIdx.x & 31) / G * G);
+  float w1[8], w2[8];
+  {
+    Raw<T> a, b;
+    if (on) a.load(w + 8 * l), b.load(w + h + 8 * l);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w1[e] = on ? a.get(e) : 0.f, w2[e] = on ? b.get(e) : 0.f;
+  }
+  const float inv_d = 1.f / (float)(2 * h);
+  for (; j < n; j += U * step) {
+    Raw<T> a[U], b[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (on && j + u * step < n) {
+        const T* p = src + (int64_t)(j + u * step) * (2 * h) + 8 * l;
+        a[u].load(p), b[u].load(p + h);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int ju = j + u * step;
+      if (ju >= n) break;
+      float ss = 0.f;
+      if (on) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x1 = a[u].get(e), x2 = b[u].get(e);
+          ss = fmaf(x1, x1, ss);
+          ss = fmaf(x2, x2, ss);
+        }
+      }
+#pragma unroll
+      for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+      const float inv = rsqrtf(fmaf(ss, inv_d, eps));
+      if (on) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y1 = a[u].get(e) * inv * w1[e], y2 = b[u].get(e) * inv * w2[e];
+          a[u].set(e, y1 * c[e] - y2 * s[e]);
+          b[u].set(e, y2 * c[e] + y1 * s[e]);
+        }
+        T* o = dst + (int64_t)ju * dst_h + 8 * l;
+        a[u].store(o), b[u].store(o + h);
+      }
+    }
+  }
+}
+
+template <typename T, int G, int U>
+__global__ void __launch_bounds__(WARPS * 32) vec_kernel(const Params p) {
+  constexpr int NG = 32 / G;
+  const int lane = threadIdx.x & 31, l = lane % G, h = p.D / 2;
+  const int64_t wid = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  const int64_t row = wid / p.wpr;
+  if (row >= p.rows) return;
+  const int64_t b = row / p.T, t = row - b * p.T;
+  const int g = (int)(wid - row * p.wpr) * NG + lane / G, step = p.wpr * NG;
+  const bool on = 8 * l < h;
+  float c[8], s[8];
+  const int64_t at = position(p, b, t) * p.D + 8 * l;
+  Raw<float> cr, sr;
+  if (on) cr.load(p.cosT + at), sr.load(p.sinT + at);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c[e] = on ? cr.get(e) : 1.f, s[e] = on ? sr.get(e) : 0.f;
+  const int64_t plane = (int64_t)p.T * p.D;
+  heads<T, G, U>(static_cast<const T*>(p.q) + b * p.qsb + t * p.qst, static_cast<T*>(p.qo) + b * p.Hq * plane + t * p.D,
+                 plane, static_cast<const T*>(p.qw), g, p.Hq, step, l, on, h, c, s, p.eps);
+  if (!p.rotk) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = 1.f, s[e] = 0.f;
+  }
+  // the group after the last one of the queries takes the first key head
+  const int first = (g - p.Hq % step + step) % step;
+  heads<T, G, U>(static_cast<const T*>(p.k) + b * p.ksb + t * p.kst, static_cast<T*>(p.ko) + b * p.kob + t * p.D, p.koh,
+                 static_cast<const T*>(p.kw), first, p.H, step, l, on, h, c, s, p.eps);
+}
+
+// Any even head dim, any alignment: one warp per head vector, read twice (the second time
+// from L1).
+template <typename T>
+__global__ void __launch_bounds__(WARPS * 32) any_kernel(const Params p) {
+  const int lane = threadIdx.x & 31, h = p.D / 2, n = p.Hq + p.H;
+  const int64_t wid = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  const int64_t row = wid / n;
+  if (row >= p.rows) return;
+  const int64_t b = row / p.T, t = row - b * p.T;
+  const int j = (int)(wid - row * n);
+  const bool isq = j < p.Hq;
+  const T* x = isq ? static_cast<const T*>(p.q) + b * p.qsb + t * p.qst + (int64_t)j * p.D
+                   : static_cast<const T*>(p.k) + b * p.ksb + t * p.kst + (int64_t)(j - p.Hq) * p.D;
+  T* o = isq ? static_cast<T*>(p.qo) + ((b * p.Hq + j) * p.T + t) * p.D
+             : static_cast<T*>(p.ko) + b * p.kob + (j - p.Hq) * p.koh + t * p.D;
+  const T* w = static_cast<const T*>(isq ? p.qw : p.kw);
+  float ss = 0.f;
+  for (int i = lane; i < p.D; i += 32) {
+    const float v = to_f(x[i]);
+    ss = fmaf(v, v, ss);
+  }
+  ss = warp_sum(ss);
+  const float inv = rsqrtf(ss / (float)p.D + p.eps);
+  const int64_t at = position(p, b, t) * p.D;
+  const bool turn = isq || p.rotk;
+  for (int i = lane; i < h; i += 32) {
+    const float y1 = to_f(x[i]) * inv * to_f(w[i]), y2 = to_f(x[i + h]) * inv * to_f(w[i + h]);
+    const float c = turn ? p.cosT[at + i] : 1.f, s = turn ? p.sinT[at + i] : 0.f;
+    o[i] = from_f<T>(y1 * c - y2 * s);
+    o[i + h] = from_f<T>(y2 * c + y1 * s);
+  }
+}
+
+template <typename T>
+int launch(const Params& p, bool vec, cudaStream_t st) {
+  const int h = p.D / 2;
+  int64_t warps;
+  if (!vec) {
+    warps = p.rows * (p.Hq + p.H);
+    SPX_REQUIRE((warps + WARPS - 1) / WARPS <= 0x7fffffff, SPX_ERR_SHAPE, "spx_qk_norm_rope: too many rows");
+    any_kernel<T><<<(unsigned)((warps + WARPS - 1) / WARPS), WARPS * 32, 0, st>>>(p);
+    return launch_status("qk_norm any_kernel");
+  }
+  int G = 1;
+  while (8 * G < h) G *= 2;
+  Params q = p;
+  // Few rows: the heads of a row are spread over several warps, until the grid has about
+  // 16 warps for each SM or every group of lanes has one head.
+  const int ng = 32 / G, most = (p.Hq + p.H + ng - 1) / ng;
+  const int64_t want = (148 * 16 + p.rows - 1) / p.rows;
+  q.wpr = (int)(want < most ? want : most);
+  warps = p.rows * q.wpr;
+  SPX_REQUIRE((warps + WARPS - 1) / WARPS <= 0x7fffffff, SPX_ERR_SHAPE, "spx_qk_norm_rope: too many rows");
+  const unsigned grid = (unsigned)((warps + WARPS - 1) / WARPS);
+  constexpr int U = sizeof(T) == 4 ? 2 : 4;
+  switch (G) {
+    case 1: vec_kernel<T, 1, U><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 2: vec_kernel<T, 2, U><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 4: vec_kernel<T, 4, U><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 8: vec_kernel<T, 8, U><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 16: vec_kernel<T, 16, U><<<grid, WARPS * 32, 0, st>>>(q); break;
+    default: vec_kernel<T, 32, U><<<grid, WARPS * 32, 0, st>>>(q); break;
+  }
+  return launch_status("qk_norm vec_kernel");
+}
+
+}  // namespace qkn
+}  // namespace spx
+
+using namespace spx;
+
+int spx_qk_norm_rope(const spx_qk_norm_args* a, void* stream) {
+  SPX_REQUIRE(a, SPX_ERR_NULL, "spx_qk_norm_rope: args are required");
+  SPX_REQUIRE(dtype_ok(a->dtype), SPX_ERR_UNSUPPORTED, "spx_qk_norm_rope: bad dtype %d", a->dtype);
+  SPX_REQUIRE(a->batch >= 0 && a->tokens >= 0 && a->num_q_heads >= 1 && a->num_q_heads <= 65535 &&
+                  a->num_kv_heads >= 0 && a->num_kv_heads <= 65535 && a->head_dim >= 2 && a->head_dim % 2 == 0 &&
+                  a->head_dim <= 1024 && a->rope_len >= 1 && a->eps >= 0.f,
+              SPX_ERR_SHAPE, "spx_qk_norm_rope: bad shape batch %d tokens %d heads %d/%d head_dim %d rope_len %d",
+              a->batch, a->tokens, a->num_q_heads, a->num_kv_heads, a->head_dim, a->rope_len);
+  const bool keys = a->num_kv_heads > 0;
+  SPX_REQUIRE(a->q && a->q_weight && a->cos_table && a->sin_table && a->q_out, SPX_ERR_NULL,
+              "spx_qk_norm_rope: q, q_weight, tables and q_out are required");
+  SPX_REQUIRE(!keys || (a->k && a->k_weight && a->k_out), SPX_ERR_NULL,
+              "spx_qk_norm_rope: k, k_weight and k_out are required with key heads");
+  SPX_REQUIRE(a->q_stride_b >= 0 && a->q_stride_t >= 0 && a->k_stride_b >= 0 && a->k_stride_t >= 0 &&
+                  a->k_out_stride_b >= 0 && a->k_out_stride_h >= 0,
+              SPX_ERR_SHAPE, "spx_qk_norm_rope: negative stride");
+  if (a->batch == 0 || a->tokens == 0) return SPX_OK;
+  qkn::Params p{};
+  p.q = a->q, p.k = a->k, p.qw = a->q_weight, p.kw = a->k_weight, p.qo = a->q_out, p.ko = a->k_out;
+  p.cosT = a->cos_table, p.sinT = a->sin_table, p.pos = a->pos;
+  p.qsb = a->q_stride_b, p.qst = a->q_stride_t, p.ksb = a->k_stride_b, p.kst = a->k_stride_t;
+  p.psb = a->pos_stride_b, p.pst = a->pos_stride_t, p.pos0 = a->pos_start;
+  p.kob = a->k_out_stride_b, p.koh = a->k_out_stride_h;
+  p.rows = (int64_t)a->batch * a->tokens;
+  p.T = a->tokens, p.Hq = a->num_q_heads, p.H = a->num_kv_heads, p.D = a->head_dim, p.len = a->rope_len;
+  p.rotk = a->rotate_keys, p.eps = a->eps, p.wpr = 1;
+  // 16-byte loads: both halves of a head start on 16 bytes and hold whole groups of eight
+  const int per = 16 / dtype_size(a->dtype);
+  const int64_t strides = a->q_stride_b | a->q_stride_t | (keys ? a->k_stride_b | a->k_stride_t | a->k_out_stride_b |
+                                                                      a->k_out_stride_h : 0);
+  const bool vec = a->head_dim % 16 == 0 && a->head_dim <= 512 && strides % per == 0 && aligned16(a->q) &&
+                   aligned16(a->q_weight) && aligned16(a->q_out) && aligned16(a->cos_table) && aligned16(a->sin_table) &&
+                   (!keys || (aligned16(a->k) && aligned16(a->k_weight) && aligned16(a->k_out)));
+  return SPX_DISPATCH_DTYPE(a->dtype, T, [&] { return qkn::launch<T>(p, vec, reinterpret_cast<cudaStream_t>(stream)); });
+}

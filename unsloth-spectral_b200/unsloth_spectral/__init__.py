@@ -6,6 +6,9 @@ Drop-in for the reference package's decode path: same public names
 ``validate_spectral_attention``, ``patch_unsloth_attention``, ``get_cache_stats``,
 ``TRITON_AVAILABLE`` / ``TRITON_VERSION`` and, when the library loads,
 ``spectral_attention_decode`` and ``TritonSpectralConfig``.
+Operators of the serving step beside them: ``qk_norm_rope`` (per-head query/key norms and
+rotation), ``LoraPool`` / ``LoraBatch`` (adapters of many requests), ``LogitsRules``
+(penalties, biases, allowed tokens, greedy choice).
 Set ``UNSLOTH_SPECTRAL_QUIET=1`` to silence the import banner.
 """
 import os
@@ -13,9 +16,12 @@ import os
 __version__ = "0.1.0+b200"
 
 from .spectral_cache import SpectralBlock, SpectralCache  # noqa: E402
-from .spectral_attention import spectral_attention_forward, validate_spectral_attention  # noqa: E402
+from .spectral_attention import (qk_norm_rope, spectral_attention_forward,  # noqa: E402
+                                 validate_spectral_attention)
 from .integration import get_cache_stats, patch_unsloth_attention  # noqa: E402
 from .kernels import TRITON_AVAILABLE, TRITON_VERSION  # noqa: E402
+from .adapters import LoraBatch, LoraPool  # noqa: E402
+from .logits import LogitsRules  # noqa: E402
 from .rsvd import batched_randomized_svd  # noqa: E402
 
 __all__ = [
@@ -26,6 +32,10 @@ __all__ = [
     "patch_unsloth_attention",
     "get_cache_stats",
     "batched_randomized_svd",
+    "qk_norm_rope",
+    "LoraPool",
+    "LoraBatch",
+    "LogitsRules",
     "TRITON_AVAILABLE",
     "TRITON_VERSION",
 ]

@@ -93,6 +93,37 @@ class PrefillArgs(C.Structure):
         (n, C.c_int64) for n in ("mask_stride_b", "mask_stride_h", "mask_stride_q")] + [("out", C.c_void_p)]
 
 
+class QkNormArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in (
+        "batch", "tokens", "num_q_heads", "num_kv_heads", "head_dim", "dtype", "rope_len", "rotate_keys")] + [
+        ("eps", C.c_float), ("reserved", C.c_int32), ("q", C.c_void_p), ("k", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("q_stride_b", "q_stride_t", "k_stride_b", "k_stride_t")] + [
+        (n, C.c_void_p) for n in ("q_weight", "k_weight", "cos_table", "sin_table", "pos")] + [
+        (n, C.c_int64) for n in ("pos_stride_b", "pos_stride_t", "pos_start")] + [
+        ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("k_out_stride_b", C.c_int64), ("k_out_stride_h", C.c_int64)]
+
+
+LORA_MAX_PARTS, LORA_MAX_RANK = 4, 128
+
+
+class LoraArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("num_tiles", "tile_rows", "num_rows", "in_features", "parts")] + [
+        ("part_width", C.c_int32 * LORA_MAX_PARTS)] + [
+        (n, C.c_int32) for n in ("max_rank", "slots", "dtype")] + [
+        (n, C.c_void_p) for n in ("x", "y", "out")] + [
+        (n, C.c_int64) for n in ("x_stride", "y_stride", "out_stride")] + [
+        (n, C.c_void_p) for n in ("a", "b", "ranks", "scales", "tiles", "order", "workspace")] + [
+        ("workspace_bytes", C.c_size_t)]
+
+
+class LogitsArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "vocab", "dtype", "record")] + [
+        ("logits", C.c_void_p), ("logits_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64)] + [
+        (n, C.c_void_p) for n in (
+            "token", "repetition", "frequency", "presence", "prompt_bits", "output_bits", "counts", "bias_bits",
+            "bias_rows", "bias_tokens", "bias_values", "allow")] + [("allow_stride", C.c_int64)]
+
+
 EXPORTS = {
     "spx_decode_workspace_size": (C.c_size_t, [C.POINTER(DecodeArgs)]),
     "spx_decode_attn": (C.c_int, [C.POINTER(DecodeArgs), C.c_void_p]),
@@ -112,6 +143,12 @@ EXPORTS = {
     "spx_block_scores": (C.c_int, [C.POINTER(BlockScoreArgs), C.c_void_p]),
     "spx_block_values": (C.c_int, [C.POINTER(BlockValueArgs), C.c_void_p]),
     "spx_prefill_attn": (C.c_int, [C.POINTER(PrefillArgs), C.c_void_p]),
+    "spx_qk_norm_rope": (C.c_int, [C.POINTER(QkNormArgs), C.c_void_p]),
+    "spx_lora_workspace_size": (C.c_size_t, [C.POINTER(LoraArgs)]),
+    "spx_lora_add": (C.c_int, [C.POINTER(LoraArgs), C.c_void_p]),
+    "spx_logits_rules": (C.c_int, [C.POINTER(LogitsArgs), C.c_void_p]),
+    "spx_logits_observe": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
+                                     C.c_void_p]),
     "spx_abi_version": (C.c_int, []),
     "spx_status_string": (C.c_char_p, [C.c_int]),
     "spx_last_error": (C.c_char_p, []),
@@ -194,6 +231,15 @@ def ptr(t) -> int:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device: torch.device, fn, *args):
+    """``fn(*args)`` with ``device`` current (a launch goes to the current device, whatever
+    device its pointers and stream belong to)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
 _workspaces = {}

@@ -162,6 +162,71 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optiona
     return out if residual is None else (out, h)
 
 
+def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, position_ids, eps: float, rotate_keys: bool):
+    """``spx_qk_norm_rope``; arguments and results as ``spectral_attention.qk_norm_rope``."""
+    dev, dt = q.device, q.dtype
+    code = N.dtype_code(dt)
+    if q.dim() != 3 or q_weight.dim() != 1:
+        raise ValueError(f"q must be [B, T, H * D] and q_weight [D], got {tuple(q.shape)} and {tuple(q_weight.shape)}")
+    B, T, n = q.shape
+    D = q_weight.shape[0]
+    if D == 0 or D % 2 or n == 0 or n % D:
+        raise ValueError(f"{n} query columns are no whole heads of {D} (an even number)")
+    if eps < 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    H = 0
+    given = [q_weight]
+    if k is not None:
+        if k_weight is None:
+            raise ValueError("k needs k_weight")
+        if k.dim() != 3 or k.shape[:2] != q.shape[:2] or k_weight.shape != q_weight.shape or k.shape[2] % D:
+            raise ValueError(f"k {tuple(k.shape)} / k_weight {tuple(k_weight.shape)} do not fit q {tuple(q.shape)} "
+                             f"with heads of {D}")
+        H = k.shape[2] // D
+        given += [k, k_weight]
+    for t in given:
+        if t.dtype != dt or t.device != dev:
+            raise ValueError(f"q, k and their weights must share dtype and device: {dt} on {dev}, "
+                             f"got {t.dtype} on {t.device}")
+    lib = N.lib_for(dev)
+    cos, sin = rope_table_f32(cos, dev), rope_table_f32(sin, dev)
+    if cos.shape != sin.shape or cos.shape[1] != D or cos.shape[0] == 0:
+        raise ValueError(f"cos/sin must be [len, {D}] tables, got {tuple(cos.shape)} and {tuple(sin.shape)}")
+    pos, psb, pst, start = None, 0, 0, 0
+    if isinstance(position_ids, torch.Tensor):
+        pos = position_ids
+        if pos.dim() == 1:
+            pos = pos[None]
+        if pos.dim() != 2 or pos.dtype != torch.int64 or pos.device != dev or pos.shape[1] != T \
+                or pos.shape[0] not in (1, B):
+            raise ValueError(f"position_ids must be int64 [{T}], [1, {T}] or [{B}, {T}] on {dev}, got "
+                             f"{position_ids.dtype} {tuple(position_ids.shape)} on {position_ids.device}")
+        psb = pos.stride(0) if pos.shape[0] > 1 else 0
+        pst = pos.stride(1)
+    else:
+        start = int(position_ids)
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    q_weight = q_weight.contiguous()
+    qo = torch.empty(B, n // D, T, D, dtype=dt, device=dev)
+    ko = None
+    a = N.QkNormArgs(batch=B, tokens=T, num_q_heads=n // D, num_kv_heads=H, head_dim=D, dtype=code,
+                     rope_len=cos.shape[0], rotate_keys=int(bool(rotate_keys)), eps=eps, q=q.data_ptr(),
+                     q_stride_b=q.stride(0), q_stride_t=q.stride(1), q_weight=q_weight.data_ptr(),
+                     cos_table=cos.data_ptr(), sin_table=sin.data_ptr(), pos=N.ptr(pos), pos_stride_b=psb,
+                     pos_stride_t=pst, pos_start=start, q_out=qo.data_ptr())
+    if k is not None:
+        if k.stride(2) != 1:
+            k = k.contiguous()
+        k_weight = k_weight.contiguous()
+        ko = torch.empty(B, H, T, D, dtype=dt, device=dev)
+        a.k, a.k_stride_b, a.k_stride_t = k.data_ptr(), k.stride(0), k.stride(1)
+        a.k_weight, a.k_out, a.k_out_stride_b, a.k_out_stride_h = k_weight.data_ptr(), ko.data_ptr(), H * T * D, T * D
+    if B and T:
+        N.check(lib, N.on_device(dev, lib.spx_qk_norm_rope, a, N.stream_handle(dev)), "spx_qk_norm_rope")
+    return qo, ko
+
+
 def quantize_int8(x: torch.Tensor):
     """Per-leading-index INT8 quantisation; returns (codes int8, scale f32 [N],
     minmax f32 [N, 2], dequantised f32) -- bit-exact with the reference's

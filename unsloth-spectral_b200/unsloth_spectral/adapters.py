@@ -1,0 +1,188 @@
+"""Low-rank adapters of many requests beside one shared projection.
+
+A ``LoraPool`` holds the adapters of one projection (several fine-tunes of one base
+weight) in slots on the device; a ``LoraBatch`` says which slot each sequence of a batch
+uses; ``pool.add(y, x, batch)`` adds each sequence's low-rank product to the shared
+projection's output ``y = x W^T``::
+
+    out[r] = y[r] + scale * B (A x[r])        A [rank, in], B [out, rank] of the row's slot
+
+One call serves every adapter of the batch (two launches of ``libspx``), for prompts and
+for single tokens.  A projection whose output is several weights side by side (a packed
+q|k|v projection) has several ``parts``, each with its own A and B.  float16 and bfloat16;
+no gradients.
+"""
+from __future__ import annotations
+
+import math
+from typing import Dict, Sequence, Tuple, Union
+
+import torch
+
+from . import _native as N
+
+
+class LoraBatch:
+    """The adapter slot of each sequence of a batch (-1: none), as host integers.  The rows
+    are grouped by slot once, on first use for a number of tokens per sequence, and kept on
+    ``device``; build the batch before capturing a CUDA graph that uses it (``prepare``)."""
+
+    def __init__(self, slots: Sequence[int], device="cuda"):
+        self.slots: Tuple[int, ...] = tuple(int(s) for s in slots)
+        if any(s < -1 for s in self.slots):
+            raise ValueError(f"a slot is -1 (none) or a pool's slot number, got {min(self.slots)}")
+        self.highest = max(self.slots, default=-1)
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self._plans: Dict[int, tuple] = {}
+
+    def __len__(self) -> int:
+        return len(self.slots)
+
+    def prepare(self, tokens: int = 1) -> "LoraBatch":
+        """Group the rows of ``tokens`` tokens per sequence now."""
+        self._plan(tokens)
+        return self
+
+    @staticmethod
+    def tiles_of(slots: Sequence[int], tokens: int):
+        """Host lists ``(tile_rows, tiles, order)``: rows sorted by slot, cut into tiles of
+        one slot.  16 rows are one MMA tile; groups beyond that use 32, which reads the
+        adapter's weights half as often."""
+        groups: Dict[int, list] = {}
+        for i, s in enumerate(slots):
+            groups.setdefault(s, []).append(i)
+        most = max((len(g) for g in groups.values()), default=0) * tokens
+        rows = 16 if most <= 16 else 32
+        order = torch.empty(len(slots) * tokens, dtype=torch.int32)
+        tiles, at = [], 0
+        for s in sorted(groups):
+            seqs = torch.tensor(groups[s], dtype=torch.int32)
+            n = len(groups[s]) * tokens
+            order[at:at + n] = (seqs[:, None] * tokens + torch.arange(tokens, dtype=torch.int32)[None]).reshape(-1)
+            tiles += [(s, at + i, min(rows, n - i), 0) for i in range(0, n, rows)]
+            at += n
+        return rows, tiles, order
+
+    def _plan(self, tokens: int):
+        p = self._plans.get(tokens)
+        if p is None:
+            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"call LoraBatch.prepare({tokens}) before capturing a graph that uses the batch")
+            rows, tiles, order = self.tiles_of(self.slots, tokens)
+            t = torch.tensor(tiles, dtype=torch.int32).reshape(-1, 4)
+            p = (rows, t.to(self.device), order.to(self.device))
+            self._plans[tokens] = p
+        return p
+
+
+class LoraPool:
+    """Adapters of one projection ``in_features -> out_features`` (an int, or the widths of
+    its parts).  ``max_rank`` (up to 128) bounds the rank of an adapter; widths and
+    ``in_features`` are multiples of 8."""
+
+    def __init__(self, in_features: int, out_features: Union[int, Sequence[int]], max_rank: int = 16, slots: int = 8,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        widths = (out_features,) if isinstance(out_features, int) else tuple(int(w) for w in out_features)
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"adapters are float16 or bfloat16, got {dtype}")
+        if not 1 <= len(widths) <= N.LORA_MAX_PARTS:
+            raise ValueError(f"1 to {N.LORA_MAX_PARTS} parts, got {len(widths)}")
+        if in_features < 8 or in_features % 8 or any(w < 8 or w % 8 for w in widths):
+            raise ValueError(f"in_features {in_features} and widths {widths} must be multiples of 8")
+        if not 1 <= max_rank <= N.LORA_MAX_RANK or slots < 1:
+            raise ValueError(f"max_rank 1..{N.LORA_MAX_RANK} and at least one slot, got {max_rank} and {slots}")
+        self.in_features, self.widths, self.out_features = in_features, widths, sum(widths)
+        self.max_rank, self.slots, self.dtype = max_rank, slots, dtype
+        self._rank = (max_rank + 15) // 16 * 16    # stored rank
+        parts = len(widths)
+        self.a = torch.zeros(slots, parts, self._rank, in_features, dtype=dtype, device=device)
+        self.b = torch.zeros(slots, self.out_features, self._rank, dtype=dtype, device=device)
+        self.ranks = torch.zeros(slots, parts, dtype=torch.int32, device=device)
+        self.scales = torch.zeros(slots, parts, dtype=torch.float32, device=device)
+        self.device = self.a.device
+        self._fixed = dict(in_features=in_features, parts=parts,
+                           part_width=(N.C.c_int32 * N.LORA_MAX_PARTS)(*widths), max_rank=self._rank, slots=slots,
+                           dtype=N.dtype_code(dtype), a=self.a.data_ptr(), b=self.b.data_ptr(),
+                           ranks=self.ranks.data_ptr(), scales=self.scales.data_ptr())
+
+    def _slot(self, slot: int, part: int):
+        if not 0 <= slot < self.slots or not 0 <= part < len(self.widths):
+            raise IndexError(f"slot {slot}, part {part} of a pool of {self.slots} slots, {len(self.widths)} parts")
+
+    def load(self, slot: int, A: torch.Tensor, B: torch.Tensor, scale: float = 1.0, part: int = 0):
+        """Put an adapter's ``A [rank, in_features]``, ``B [width, rank]`` and scale
+        (alpha / rank) into a slot; its other parts keep what they hold (nothing at first:
+        the shared projection alone)."""
+        self._slot(slot, part)
+        w = self.widths[part]
+        r = A.shape[0]
+        if A.shape != (r, self.in_features) or B.shape != (w, r) or not 1 <= r <= self.max_rank:
+            raise ValueError(f"A must be [rank, {self.in_features}] and B [{w}, rank] with rank 1..{self.max_rank}, "
+                             f"got {tuple(A.shape)} and {tuple(B.shape)}")
+        if not math.isfinite(scale):
+            raise ValueError(f"scale must be finite, got {scale}")
+        at = sum(self.widths[:part])
+        with torch.no_grad():
+            self.a[slot, part].zero_()
+            self.a[slot, part, :r].copy_(A)
+            self.b[slot, at:at + w].zero_()
+            self.b[slot, at:at + w, :r].copy_(B)
+            self.ranks[slot, part] = r
+            self.scales[slot, part] = float(scale)
+
+    def unload(self, slot: int):
+        """Empty a slot: its sequences get the shared projection alone."""
+        self._slot(slot, 0)
+        self.ranks[slot].zero_()
+
+    def add(self, y: torch.Tensor, x: torch.Tensor, batch: LoraBatch, out=None) -> torch.Tensor:
+        """``y + scale * B (A x)`` of each sequence's slot.  ``x [B, T, in]`` (or ``[B, in]``:
+        one token each) and ``y [B, T, out]`` in the pool's dtype, rows on 16 bytes and evenly
+        spaced; ``out`` may be ``y`` itself (in place), else a new tensor is returned."""
+        dev, dt = self.device, self.dtype
+        if x.dim() not in (2, 3) or x.shape[-1] != self.in_features or y.shape[:-1] != x.shape[:-1] \
+                or y.shape[-1] != self.out_features or x.shape[0] != len(batch):
+            raise ValueError(f"x [B, T, {self.in_features}] and y [B, T, {self.out_features}] of {len(batch)} sequences "
+                             f"expected, got {tuple(x.shape)} and {tuple(y.shape)}")
+        if batch.highest >= self.slots:
+            raise IndexError(f"the batch names slot {batch.highest}, the pool has {self.slots}")
+        if out is None:
+            out = torch.empty(y.shape, dtype=dt, device=dev)
+        elif out.shape != y.shape:
+            raise ValueError(f"out {tuple(out.shape)} must have the shape of y {tuple(y.shape)}")
+        for t in (x, y, out):
+            if t.dtype != dt or t.device != dev:
+                raise ValueError(f"x, y and out must be {dt} on {dev}, got {t.dtype} on {t.device}")
+        if batch.device != dev:
+            raise ValueError(f"the batch is on {batch.device}, the pool on {dev}")
+        lib = N.lib_for(dev)
+        tokens = x.shape[1] if x.dim() == 3 else 1
+        if x.numel() == 0:
+            return out
+        rows, tiles, order = batch._plan(tokens)
+        n = order.shape[0]
+        # the inner products, a buffer of each call's own: two streams or two captured graphs
+        # never share one (the caching allocator hands it out in stream order)
+        ws = torch.empty(n * len(self.widths) * self._rank, dtype=torch.float32, device=dev)
+        a = N.LoraArgs(num_tiles=tiles.shape[0], tile_rows=rows, num_rows=n, x=x.data_ptr(), y=y.data_ptr(),
+                       out=out.data_ptr(), x_stride=_row_stride(x), y_stride=_row_stride(y),
+                       out_stride=_row_stride(out), tiles=tiles.data_ptr(), order=order.data_ptr(),
+                       workspace=ws.data_ptr(), workspace_bytes=4 * ws.numel(), **self._fixed)
+        N.check(lib, N.on_device(dev, lib.spx_lora_add, a, N.stream_handle(dev)), "spx_lora_add")
+        return out
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """The distance between the rows of ``t [.., n]``, which must be even."""
+    if t.stride(-1) != 1:
+        raise ValueError(f"the last dimension must be contiguous, got strides {t.stride()}")
+    if t.dim() == 2:
+        return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    B, T, n = t.shape
+    if T == 1:
+        return t.stride(0) if B > 1 else max(t.stride(0), n)
+    if B > 1 and t.stride(0) != T * t.stride(1):
+        raise ValueError(f"rows must be evenly spaced, got strides {t.stride()} of {tuple(t.shape)}")
+    return t.stride(1)

@@ -42,6 +42,23 @@ def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.T
     return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1)
 
 
+def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.Tensor,
+                 k_weight: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, position_ids=0, *,
+                 eps: float = 1e-6, rotate_keys: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """RMS norms of the query and key heads with the rotation in the same pass, for models
+    whose attention normalises each head (``q_norm`` / ``k_norm``).
+
+    ``q`` ``[B, T, H_q * D]`` and ``k`` ``[B, T, H * D]`` (or None) are projection rows, e.g.
+    views of a packed q|k|v projection; ``q_weight`` / ``k_weight`` ``[D]`` in their dtype;
+    ``cos`` / ``sin`` ``[len, D]`` tables (first half used for both halves, as ``apply_rope``);
+    ``position_ids`` int64 ``[T]``, ``[1, T]`` or ``[B, T]`` on the device, or the first
+    position as an int; positions are clamped to the tables.  Returns
+    ``q`` ``[B, H_q, T, D]`` normalised and rotated, and ``k`` ``[B, H, T, D]`` normalised and,
+    with ``rotate_keys``, rotated (``SpectralCache`` holds keys before the rotation).
+    float32 / float16 / bfloat16; float32 inside, rounded once.  No gradients."""
+    return _ops.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, position_ids, eps, rotate_keys)
+
+
 def _as_device_cache(cache, device) -> SpectralCache:
     """Copy a reference-style cache (``cold_blocks`` list + hot tensors) into device tiers."""
     blocks = list(getattr(cache, "cold_blocks", []) or [])
