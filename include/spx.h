@@ -461,23 +461,23 @@ typedef struct spx_logits_args {
   const float* repetition;     /* [batch], > 0; NULL: none */
   const float* frequency;      /* [batch]; NULL: none */
   const float* presence;       /* [batch]; NULL: none */
-  const uint32_t* prompt_bits; /* [batch][W] */
-  uint32_t* output_bits;       /* [batch][W] */
+  uint32_t* seen_bits;         /* [batch][W]: tokens of the prompt or put out */
+  uint32_t* touched_bits;      /* [batch][W]: seen or biased (may be seen_bits when nothing is biased) */
   int32_t* counts;             /* [batch][vocab]: times each token was put out */
   const uint32_t* bias_bits;   /* [batch][W]: tokens with a bias; NULL: none */
-  const int32_t* bias_rows;    /* [batch + 1]: range of each row in bias_tokens */
-  const int32_t* bias_tokens;  /* ascending within a row */
-  const float* bias_values;
+  const int32_t* bias_first;   /* [batch][W]: index in bias_values of a word's first bias */
+  const float* bias_values;    /* by row, then ascending by token */
   const uint32_t* allow;       /* row b at allow + b*allow_stride; NULL: every token allowed */
   int64_t allow_stride;        /* words between rows, 0: one row for all */
 } spx_logits_args;
 
 SPX_API int spx_logits_rules(const spx_logits_args* args, void* stream);
 
-/* Tokens [batch][count] (int64, rows `stride` apart) added to the history: to the bitmap,
- * and to counts when it is not NULL.  Values outside [0, vocab) are skipped (padding). */
-SPX_API int spx_logits_observe(const int64_t* tokens, int64_t stride, int batch, int count, int vocab, uint32_t* bits,
-                               int32_t* counts, void* stream);
+/* Tokens [batch][count] (int64, rows `stride` apart) added to the history: to both bitmaps,
+ * and to counts when it is not NULL (tokens put out; NULL for a prompt's).  Values outside
+ * [0, vocab) are skipped (padding). */
+SPX_API int spx_logits_observe(const int64_t* tokens, int64_t stride, int batch, int count, int vocab,
+                               uint32_t* seen_bits, uint32_t* touched_bits, int32_t* counts, void* stream);
 
 /* ---------------------------------------------------------------------------------
  * Utilities.

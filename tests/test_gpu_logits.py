@@ -170,6 +170,6 @@ def test_strides_streams_and_graphs():
         steps.append(t.clone())
     other = LogitsRules(B, V, presence_penalty=0.5)
     assert torch.equal(torch.stack(steps), torch.stack([other.pick(x, record=True) for _ in range(4)]))
-    assert torch.equal(rules.counts, other.counts) and torch.equal(rules.output_bits, other.output_bits)
+    assert torch.equal(rules.counts, other.counts) and torch.equal(rules.seen_bits, other.seen_bits)
     one = torch.randn(1, 1, device="cuda")
     assert LogitsRules(1, 1).pick(one).tolist() == [0]

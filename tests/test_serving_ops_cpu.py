@@ -37,6 +37,19 @@ def test_struct_layouts_match_header():
     assert (got["parts"], got["rank"]) == (N.LORA_MAX_PARTS, N.LORA_MAX_RANK)
 
 
+@pytest.mark.parametrize("pack,struct", [(N.QK_NORM_PACK, N.QkNormArgs), (N.LORA_PACK, N.LoraArgs),
+                                         (N.LOGITS_PACK, N.LogitsArgs)])
+def test_packed_args_are_the_struct(pack, struct):
+    """The struct formats put every value at its field's place: distinct values read back."""
+    assert pack.size == C.sizeof(struct)
+    fields = [(f, t, i) for f, t in struct._fields_ for i in range(getattr(t, "_length_", 1))]
+    vals = [k + 1 for k in range(len(fields))]
+    got = struct.from_buffer_copy(pack.pack(*vals))
+    for (f, t, i), v in zip(fields, vals):
+        x = getattr(got, f)
+        assert (x[i] if hasattr(t, "_length_") else x) == v, f
+
+
 def _qk(**kw):
     a = N.QkNormArgs(batch=1, tokens=1, num_q_heads=4, num_kv_heads=2, head_dim=64, dtype=N.SPX_BF16, rope_len=8, eps=1e-6,
                      q=256, k=256, q_weight=256, k_weight=256, cos_table=256, sin_table=256, q_out=256, k_out=256)
@@ -83,15 +96,15 @@ def test_lora_c_refusals(status, kw):
 
 def _logits(**kw):
     a = N.LogitsArgs(batch=2, vocab=100, dtype=N.SPX_F32, logits=256, logits_stride=100, token=256, repetition=256,
-                     prompt_bits=256, output_bits=256, counts=256)
+                     seen_bits=256, touched_bits=256, counts=256)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
 
 
 @pytest.mark.parametrize("status,kw", [
-    (0, dict(batch=0)), (1, dict(logits=None)), (1, dict(token=None)), (1, dict(prompt_bits=None)),
-    (1, dict(counts=None)), (1, dict(bias_bits=256)), (1, dict(repetition=None, record=1, output_bits=None)),
+    (0, dict(batch=0)), (1, dict(logits=None)), (1, dict(token=None)), (1, dict(seen_bits=None)), (1, dict(touched_bits=None)),
+    (1, dict(counts=None)), (1, dict(bias_bits=256)), (1, dict(repetition=None, record=1, seen_bits=None)),
     (2, dict(vocab=0)), (2, dict(batch=-1)), (2, dict(logits_stride=99)), (2, dict(out=256, out_stride=99)),
     (2, dict(allow=256, allow_stride=3)), (3, dict(dtype=9))])
 def test_logits_c_refusals(status, kw):
@@ -100,12 +113,13 @@ def test_logits_c_refusals(status, kw):
 
 def test_observe_c_refusals():
     lib = N.load()
-    assert lib.spx_logits_observe(None, 1, 2, 3, 100, 256, 256, None) == 1
-    assert lib.spx_logits_observe(256, 1, 2, 3, 100, None, 256, None) == 1
-    assert lib.spx_logits_observe(256, 1, 2, -3, 100, 256, 256, None) == 2
-    assert lib.spx_logits_observe(256, -1, 2, 3, 100, 256, 256, None) == 2
-    assert lib.spx_logits_observe(256, 1, 2, 3, 0, 256, 256, None) == 2
-    assert lib.spx_logits_observe(None, 1, 2, 0, 100, 256, None, None) == 0
+    assert lib.spx_logits_observe(None, 1, 2, 3, 100, 256, 256, 256, None) == 1
+    assert lib.spx_logits_observe(256, 1, 2, 3, 100, None, 256, 256, None) == 1
+    assert lib.spx_logits_observe(256, 1, 2, 3, 100, 256, None, 256, None) == 1
+    assert lib.spx_logits_observe(256, 1, 2, -3, 100, 256, 256, 256, None) == 2
+    assert lib.spx_logits_observe(256, -1, 2, 3, 100, 256, 256, 256, None) == 2
+    assert lib.spx_logits_observe(256, 1, 2, 3, 0, 256, 256, 256, None) == 2
+    assert lib.spx_logits_observe(None, 1, 2, 0, 100, 256, 256, None, None) == 0
 
 
 def test_qk_norm_python_refusals():
@@ -184,7 +198,7 @@ def test_logits_python_refusals():
             LogitsRules(**{**dict(batch=2, vocab=50, device="cpu"), **bad})
     r = LogitsRules(2, 50, device="cpu", logit_bias=[{31: 1.0, 0: 2.0, 49: 3.0}, None])
     assert r._bias[0].tolist() == [[1 - (1 << 31), 1 << 17], [0, 0]]
-    assert r._bias[1].tolist() == [0, 3, 3] and r._bias[2].tolist() == [0, 31, 49]
+    assert r._bias[1].tolist() == [[0, 2], [3, 3]] and r._bias[2].tolist() == [2.0, 1.0, 3.0]
     x = torch.zeros(2, 50)
     for call in (lambda: r.pick(x[:1]), lambda: r.pick(x.t()), lambda: r.apply(x, out=x.half()),
                  lambda: r.pick(x, allow=torch.zeros(2, 1, dtype=torch.int32)),

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -120,9 +121,16 @@ class LogitsArgs(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("batch", "vocab", "dtype", "record")] + [
         ("logits", C.c_void_p), ("logits_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64)] + [
         (n, C.c_void_p) for n in (
-            "token", "repetition", "frequency", "presence", "prompt_bits", "output_bits", "counts", "bias_bits",
-            "bias_rows", "bias_tokens", "bias_values", "allow")] + [("allow_stride", C.c_int64)]
+            "token", "repetition", "frequency", "presence", "seen_bits", "touched_bits", "counts", "bias_bits",
+            "bias_first", "bias_values", "allow")] + [("allow_stride", C.c_int64)]
 
+
+# The three structs above as `struct` formats, field by field: the entry points that a decode
+# step calls for every layer take them packed (bytes), which costs about 1 us a call where
+# filling a ctypes.Structure costs 6 to 8.
+QK_NORM_PACK = struct.Struct("@8ifi2P4q5P3q2P2q0q")
+LORA_PACK = struct.Struct("@5i4i3i3P3q7PN0q")
+LOGITS_PACK = struct.Struct("@4iPqPq11Pq0q")
 
 EXPORTS = {
     "spx_decode_workspace_size": (C.c_size_t, [C.POINTER(DecodeArgs)]),
@@ -148,7 +156,7 @@ EXPORTS = {
     "spx_lora_add": (C.c_int, [C.POINTER(LoraArgs), C.c_void_p]),
     "spx_logits_rules": (C.c_int, [C.POINTER(LogitsArgs), C.c_void_p]),
     "spx_logits_observe": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
-                                     C.c_void_p]),
+                                     C.c_void_p, C.c_void_p]),
     "spx_abi_version": (C.c_int, []),
     "spx_status_string": (C.c_char_p, [C.c_int]),
     "spx_last_error": (C.c_char_p, []),
@@ -233,9 +241,32 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_packed = {}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def launch_packed(what: str, index: int, args: bytes):
+    """Call the entry point ``what`` with its packed args struct on the current stream of CUDA
+    device ``index``, with that device current (a launch goes to the current device,
+    whatever device its pointers and stream belong to); raises unless it returns SPX_OK."""
+    fn = _packed.get(what)
+    if fn is None:
+        fn = load()[what]                     # a binding of its own: bytes for the struct pointer
+        fn.restype, fn.argtypes = C.c_int, [C.c_char_p, C.c_void_p]
+        _packed[what] = fn
+    if index not in _device_ok or _device_ok[index] != SPX_OK:
+        lib_for(torch.device("cuda", index))
+    if index == torch.cuda.current_device():
+        rc = fn(args, _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(args, torch.cuda.current_stream(index).cuda_stream)
+    if rc != SPX_OK:
+        check(_lib, rc, what)
+
+
 def on_device(device: torch.device, fn, *args):
-    """``fn(*args)`` with ``device`` current (a launch goes to the current device, whatever
-    device its pointers and stream belong to)."""
+    """``fn(*args)`` with ``device`` current."""
     if device.index is None or device.index == torch.cuda.current_device():
         return fn(*args)
     with torch.cuda.device(device):

@@ -163,8 +163,9 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optiona
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, position_ids, eps: float, rotate_keys: bool):
-    """``spx_qk_norm_rope``; arguments and results as ``spectral_attention.qk_norm_rope``."""
-    dev, dt = q.device, q.dtype
+    """``spx_qk_norm_rope``; arguments and results as ``spectral_attention.qk_norm_rope``.
+    Runs for every layer of a decode step, so it looks at each tensor as little as it can."""
+    dt, dev = q.dtype, q.get_device()
     code = N.dtype_code(dt)
     if q.dim() != 3 or q_weight.dim() != 1:
         raise ValueError(f"q must be [B, T, H * D] and q_weight [D], got {tuple(q.shape)} and {tuple(q_weight.shape)}")
@@ -172,58 +173,64 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, position_ids, eps: float, r
     D = q_weight.shape[0]
     if D == 0 or D % 2 or n == 0 or n % D:
         raise ValueError(f"{n} query columns are no whole heads of {D} (an even number)")
-    if eps < 0:
+    if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
+    fits = q_weight.dtype == dt and q_weight.get_device() == dev
     H = 0
-    given = [q_weight]
     if k is not None:
         if k_weight is None:
             raise ValueError("k needs k_weight")
-        if k.dim() != 3 or k.shape[:2] != q.shape[:2] or k_weight.shape != q_weight.shape or k.shape[2] % D:
+        if k.dim() != 3 or k.shape[0] != B or k.shape[1] != T or k_weight.shape != q_weight.shape or k.shape[2] % D:
             raise ValueError(f"k {tuple(k.shape)} / k_weight {tuple(k_weight.shape)} do not fit q {tuple(q.shape)} "
                              f"with heads of {D}")
         H = k.shape[2] // D
-        given += [k, k_weight]
-    for t in given:
-        if t.dtype != dt or t.device != dev:
-            raise ValueError(f"q, k and their weights must share dtype and device: {dt} on {dev}, "
-                             f"got {t.dtype} on {t.device}")
-    lib = N.lib_for(dev)
-    cos, sin = rope_table_f32(cos, dev), rope_table_f32(sin, dev)
-    if cos.shape != sin.shape or cos.shape[1] != D or cos.shape[0] == 0:
+        fits = (fits and k.dtype == dt and k_weight.dtype == dt and k.get_device() == dev
+                and k_weight.get_device() == dev)
+    if not fits:
+        raise ValueError(f"q, k and their weights must share dtype and device: q has {dt} on {q.device}")
+    if dev < 0:
+        N.lib_for(q.device)
+    if cos.dtype != torch.float32 or cos.dim() != 2 or not cos.is_contiguous() or cos.get_device() != dev:
+        cos = rope_table_f32(cos, q.device)
+    if sin.dtype != torch.float32 or sin.dim() != 2 or not sin.is_contiguous() or sin.get_device() != dev:
+        sin = rope_table_f32(sin, q.device)
+    length = cos.shape[0]
+    if cos.shape != sin.shape or cos.shape[1] != D or length == 0:
         raise ValueError(f"cos/sin must be [len, {D}] tables, got {tuple(cos.shape)} and {tuple(sin.shape)}")
-    pos, psb, pst, start = None, 0, 0, 0
+    pos_ptr = psb = pst = start = 0
     if isinstance(position_ids, torch.Tensor):
-        pos = position_ids
-        if pos.dim() == 1:
-            pos = pos[None]
-        if pos.dim() != 2 or pos.dtype != torch.int64 or pos.device != dev or pos.shape[1] != T \
-                or pos.shape[0] not in (1, B):
-            raise ValueError(f"position_ids must be int64 [{T}], [1, {T}] or [{B}, {T}] on {dev}, got "
+        shape, stride = position_ids.shape, position_ids.stride()
+        if len(shape) == 1:
+            shape, stride = (1, *shape), (0, *stride)
+        if len(shape) != 2 or position_ids.dtype != torch.int64 or position_ids.get_device() != dev \
+                or shape[1] != T or (shape[0] != 1 and shape[0] != B):
+            raise ValueError(f"position_ids must be int64 [{T}], [1, {T}] or [{B}, {T}] on {q.device}, got "
                              f"{position_ids.dtype} {tuple(position_ids.shape)} on {position_ids.device}")
-        psb = pos.stride(0) if pos.shape[0] > 1 else 0
-        pst = pos.stride(1)
+        pos_ptr = position_ids.data_ptr()
+        psb, pst = stride if shape[0] > 1 else (0, stride[1])
     else:
         start = int(position_ids)
-    if q.stride(2) != 1:
+    qs = q.stride()
+    if qs[2] != 1:
         q = q.contiguous()
+        qs = q.stride()
     q_weight = q_weight.contiguous()
-    qo = torch.empty(B, n // D, T, D, dtype=dt, device=dev)
-    ko = None
-    a = N.QkNormArgs(batch=B, tokens=T, num_q_heads=n // D, num_kv_heads=H, head_dim=D, dtype=code,
-                     rope_len=cos.shape[0], rotate_keys=int(bool(rotate_keys)), eps=eps, q=q.data_ptr(),
-                     q_stride_b=q.stride(0), q_stride_t=q.stride(1), q_weight=q_weight.data_ptr(),
-                     cos_table=cos.data_ptr(), sin_table=sin.data_ptr(), pos=N.ptr(pos), pos_stride_b=psb,
-                     pos_stride_t=pst, pos_start=start, q_out=qo.data_ptr())
-    if k is not None:
-        if k.stride(2) != 1:
+    qo = q.new_empty((B, n // D, T, D))
+    if k is None:
+        ko, kp, kwp, kop, ks = None, 0, 0, 0, (0, 0)
+    else:
+        ks = k.stride()
+        if ks[2] != 1:
             k = k.contiguous()
+            ks = k.stride()
         k_weight = k_weight.contiguous()
-        ko = torch.empty(B, H, T, D, dtype=dt, device=dev)
-        a.k, a.k_stride_b, a.k_stride_t = k.data_ptr(), k.stride(0), k.stride(1)
-        a.k_weight, a.k_out, a.k_out_stride_b, a.k_out_stride_h = k_weight.data_ptr(), ko.data_ptr(), H * T * D, T * D
+        ko = k.new_empty((B, H, T, D))
+        kp, kwp, kop = k.data_ptr(), k_weight.data_ptr(), ko.data_ptr()
     if B and T:
-        N.check(lib, N.on_device(dev, lib.spx_qk_norm_rope, a, N.stream_handle(dev)), "spx_qk_norm_rope")
+        N.launch_packed("spx_qk_norm_rope", dev, N.QK_NORM_PACK.pack(
+            B, T, n // D, H, D, code, length, 1 if rotate_keys else 0, eps, 0, q.data_ptr(), kp, qs[0], qs[1], ks[0], ks[1],
+            q_weight.data_ptr(), kwp, cos.data_ptr(), sin.data_ptr(), pos_ptr, psb, pst, start, qo.data_ptr(), kop,
+            H * T * D, T * D))
     return qo, ko
 
 

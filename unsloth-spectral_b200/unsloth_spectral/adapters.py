@@ -72,7 +72,7 @@ class LoraBatch:
                 raise RuntimeError(f"call LoraBatch.prepare({tokens}) before capturing a graph that uses the batch")
             rows, tiles, order = self.tiles_of(self.slots, tokens)
             t = torch.tensor(tiles, dtype=torch.int32).reshape(-1, 4)
-            p = (rows, t.to(self.device), order.to(self.device))
+            p = (rows, len(tiles), len(order), t.to(self.device), order.to(self.device))
             self._plans[tokens] = p
         return p
 
@@ -102,10 +102,11 @@ class LoraPool:
         self.ranks = torch.zeros(slots, parts, dtype=torch.int32, device=device)
         self.scales = torch.zeros(slots, parts, dtype=torch.float32, device=device)
         self.device = self.a.device
-        self._fixed = dict(in_features=in_features, parts=parts,
-                           part_width=(N.C.c_int32 * N.LORA_MAX_PARTS)(*widths), max_rank=self._rank, slots=slots,
-                           dtype=N.dtype_code(dtype), a=self.a.data_ptr(), b=self.b.data_ptr(),
-                           ranks=self.ranks.data_ptr(), scales=self.scales.data_ptr())
+        self._index = self.a.get_device()
+        # what of spx_lora_args does not change from call to call
+        self._pool_args = (in_features, parts, *widths, *(0,) * (N.LORA_MAX_PARTS - parts), self._rank, slots,
+                           N.dtype_code(dtype))
+        self._pool_ptrs = (self.a.data_ptr(), self.b.data_ptr(), self.ranks.data_ptr(), self.scales.data_ptr())
 
     def _slot(self, slot: int, part: int):
         if not 0 <= slot < self.slots or not 0 <= part < len(self.widths):
@@ -141,48 +142,47 @@ class LoraPool:
         """``y + scale * B (A x)`` of each sequence's slot.  ``x [B, T, in]`` (or ``[B, in]``:
         one token each) and ``y [B, T, out]`` in the pool's dtype, rows on 16 bytes and evenly
         spaced; ``out`` may be ``y`` itself (in place), else a new tensor is returned."""
-        dev, dt = self.device, self.dtype
-        if x.dim() not in (2, 3) or x.shape[-1] != self.in_features or y.shape[:-1] != x.shape[:-1] \
-                or y.shape[-1] != self.out_features or x.shape[0] != len(batch):
+        dev, dt = self._index, self.dtype
+        xs, ys = x.shape, y.shape
+        tokens = xs[1] if len(xs) == 3 else 1
+        if len(xs) not in (2, 3) or len(ys) != len(xs) or xs[-1] != self.in_features or ys[-1] != self.out_features \
+                or ys[:-1] != xs[:-1] or xs[0] != len(batch.slots):
             raise ValueError(f"x [B, T, {self.in_features}] and y [B, T, {self.out_features}] of {len(batch)} sequences "
-                             f"expected, got {tuple(x.shape)} and {tuple(y.shape)}")
+                             f"expected, got {tuple(xs)} and {tuple(ys)}")
         if batch.highest >= self.slots:
             raise IndexError(f"the batch names slot {batch.highest}, the pool has {self.slots}")
         if out is None:
-            out = torch.empty(y.shape, dtype=dt, device=dev)
-        elif out.shape != y.shape:
-            raise ValueError(f"out {tuple(out.shape)} must have the shape of y {tuple(y.shape)}")
-        for t in (x, y, out):
-            if t.dtype != dt or t.device != dev:
-                raise ValueError(f"x, y and out must be {dt} on {dev}, got {t.dtype} on {t.device}")
-        if batch.device != dev:
-            raise ValueError(f"the batch is on {batch.device}, the pool on {dev}")
-        lib = N.lib_for(dev)
-        tokens = x.shape[1] if x.dim() == 3 else 1
-        if x.numel() == 0:
+            out = x.new_empty(ys)
+        elif out.shape != ys:
+            raise ValueError(f"out {tuple(out.shape)} must have the shape of y {tuple(ys)}")
+        if not (x.dtype == dt and y.dtype == dt and out.dtype == dt and x.get_device() == dev and y.get_device() == dev
+                and out.get_device() == dev):
+            raise ValueError(f"x, y and out must be {dt} on {self.device}")
+        if batch.device != self.device:
+            raise ValueError(f"the batch is on {batch.device}, the pool on {self.device}")
+        if dev < 0:
+            N.lib_for(self.device)
+        if tokens == 0 or not batch.slots:
             return out
-        rows, tiles, order = batch._plan(tokens)
-        n = order.shape[0]
+        rows, n_tiles, n, tiles, order = batch._plan(tokens)
         # the inner products, a buffer of each call's own: two streams or two captured graphs
         # never share one (the caching allocator hands it out in stream order)
-        ws = torch.empty(n * len(self.widths) * self._rank, dtype=torch.float32, device=dev)
-        a = N.LoraArgs(num_tiles=tiles.shape[0], tile_rows=rows, num_rows=n, x=x.data_ptr(), y=y.data_ptr(),
-                       out=out.data_ptr(), x_stride=_row_stride(x), y_stride=_row_stride(y),
-                       out_stride=_row_stride(out), tiles=tiles.data_ptr(), order=order.data_ptr(),
-                       workspace=ws.data_ptr(), workspace_bytes=4 * ws.numel(), **self._fixed)
-        N.check(lib, N.on_device(dev, lib.spx_lora_add, a, N.stream_handle(dev)), "spx_lora_add")
+        size = n * len(self.widths) * self._rank
+        ws = self.scales.new_empty(size)
+        N.launch_packed("spx_lora_add", dev, N.LORA_PACK.pack(
+            n_tiles, rows, n, *self._pool_args, x.data_ptr(), y.data_ptr(), out.data_ptr(), _row_stride(x),
+            _row_stride(y), _row_stride(out), *self._pool_ptrs, tiles.data_ptr(), order.data_ptr(), ws.data_ptr(),
+            4 * size))
         return out
 
 
 def _row_stride(t: torch.Tensor) -> int:
     """The distance between the rows of ``t [.., n]``, which must be even."""
-    if t.stride(-1) != 1:
-        raise ValueError(f"the last dimension must be contiguous, got strides {t.stride()}")
-    if t.dim() == 2:
-        return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
-    B, T, n = t.shape
-    if T == 1:
-        return t.stride(0) if B > 1 else max(t.stride(0), n)
-    if B > 1 and t.stride(0) != T * t.stride(1):
-        raise ValueError(f"rows must be evenly spaced, got strides {t.stride()} of {tuple(t.shape)}")
-    return t.stride(1)
+    shape, stride = t.shape, t.stride()
+    if stride[-1] != 1:
+        raise ValueError(f"the last dimension must be contiguous, got strides {stride}")
+    if len(shape) == 2 or shape[1] == 1:
+        return stride[0] if shape[0] > 1 else max(stride[0], shape[-1])
+    if shape[0] > 1 and stride[0] != shape[1] * stride[1]:
+        raise ValueError(f"rows must be evenly spaced, got strides {stride} of {tuple(shape)}")
+    return stride[1]

@@ -45,15 +45,14 @@ class LogitsRules:
         if batch < 1 or batch > 65535 or not 1 <= vocab <= 1 << 30:
             raise ValueError(f"batch 1..65535 and vocab 1..2^30 expected, got {batch} and {vocab}")
         self.batch, self.vocab = batch, vocab
-        words = allow_words(vocab)
+        words = self._words = allow_words(vocab)
         rep = _setting("repetition_penalty", repetition_penalty, batch)
         if any(v <= 0 for v in rep):
             raise ValueError("repetition_penalty must be positive")
         freq = _setting("frequency_penalty", frequency_penalty, batch)
         pres = _setting("presence_penalty", presence_penalty, batch)
-        at, toks, vals = _biases(logit_bias, batch, vocab)
-        self.prompt_bits = torch.zeros(batch, words, dtype=torch.int32, device=device)
-        self.output_bits = torch.zeros(batch, words, dtype=torch.int32, device=device)
+        rows, toks, vals = _biases(logit_bias, batch, vocab)
+        self.seen_bits = torch.zeros(batch, words, dtype=torch.int32, device=device)
         self.counts = torch.zeros(batch, vocab, dtype=torch.int32, device=device)
         dev = self.device = self.counts.device
         put = lambda v, neutral: torch.tensor(v, dtype=torch.float32, device=dev) if any(  # noqa: E731
@@ -61,35 +60,40 @@ class LogitsRules:
         self._rep, self._freq, self._pres = put(rep, 1.0), put(freq, 0.0), put(pres, 0.0)
         self._bias = None
         if toks:
-            t = torch.tensor(toks, dtype=torch.int32)
-            rows = torch.repeat_interleave(torch.arange(batch), torch.tensor(at).diff())
+            t = torch.tensor(toks, dtype=torch.int64)
+            word = torch.tensor(rows, dtype=torch.int64) * words + t // 32
             bits = torch.zeros(batch * words, dtype=torch.int64)
             # one bit of a word for each distinct token: a sum sets them
-            bits.scatter_add_(0, rows * words + t.long() // 32, torch.ones_like(rows) << (t.long() % 32))
-            bits = torch.where(bits >= 1 << 31, bits - (1 << 32), bits).to(torch.int32).view(batch, words)
-            self._bias = (bits.to(dev), torch.tensor(at, dtype=torch.int32, device=dev), t.to(dev),
+            bits.scatter_add_(0, word, torch.ones_like(t) << (t % 32))
+            bits = torch.where(bits >= 1 << 31, bits - (1 << 32), bits).to(torch.int32)
+            n = torch.bincount(word, minlength=batch * words)
+            first = (n.cumsum(0) - n).to(torch.int32)
+            self._bias = (bits.view(batch, words).to(dev), first.view(batch, words).to(dev),
                           torch.tensor(vals, dtype=torch.float32, device=dev))
-        b = self._bias or (None,) * 4
-        self._fixed = dict(batch=batch, vocab=vocab, repetition=N.ptr(self._rep), frequency=N.ptr(self._freq),
-                           presence=N.ptr(self._pres), prompt_bits=N.ptr(self.prompt_bits),
-                           output_bits=N.ptr(self.output_bits), counts=N.ptr(self.counts), bias_bits=N.ptr(b[0]),
-                           bias_rows=N.ptr(b[1]), bias_tokens=N.ptr(b[2]), bias_values=N.ptr(b[3]))
+        b = self._bias or (None,) * 3
+        # the tokens that a rule touches: seen ones and, where there are any, biased ones
+        self._touched = self.seen_bits if b[0] is None else b[0].clone()
+        self._index = self.counts.get_device()
+        # what of spx_logits_args does not change from call to call
+        self._state_ptrs = (N.ptr(self._rep), N.ptr(self._freq), N.ptr(self._pres), N.ptr(self.seen_bits),
+                            N.ptr(self._touched), N.ptr(self.counts), *(N.ptr(t) for t in b))
 
     def reset(self):
         """Forget the history (a new generation with the same settings)."""
-        self.prompt_bits.zero_()
-        self.output_bits.zero_()
+        self.seen_bits.zero_()
         self.counts.zero_()
+        if self._bias is not None:
+            self._touched.copy_(self._bias[0])
 
     def observe_prompt(self, tokens: torch.Tensor):
         """Add the prompt's tokens ``[batch, n]`` (int64; negative ones are padding)."""
-        self._observe(tokens, self.prompt_bits, None)
+        self._observe(tokens, None)
 
     def observe(self, tokens: torch.Tensor):
         """Add tokens put out, ``[batch]`` or ``[batch, n]`` (int64; negative ones are padding)."""
-        self._observe(tokens, self.output_bits, self.counts)
+        self._observe(tokens, self.counts)
 
-    def _observe(self, tokens, bits, counts):
+    def _observe(self, tokens, counts):
         t = tokens[:, None] if tokens.dim() == 1 else tokens
         if t.dim() != 2 or t.shape[0] != self.batch or t.dtype != torch.int64 or t.device != self.device:
             raise ValueError(f"tokens must be int64 [{self.batch}, n] on {self.device}, got {tokens.dtype} "
@@ -98,7 +102,8 @@ class LogitsRules:
         if t.shape[1] > 1 and t.stride(1) != 1 or t.stride(0) < 0:
             t = t.contiguous()
         N.check(lib, N.on_device(self.device, lib.spx_logits_observe, N.ptr(t), t.stride(0), self.batch, t.shape[1],
-                                 self.vocab, N.ptr(bits), N.ptr(counts), N.stream_handle(self.device)),
+                                 self.vocab, N.ptr(self.seen_bits), N.ptr(self._touched), N.ptr(counts),
+                                 N.stream_handle(self.device)),
                 "spx_logits_observe")
 
     def apply(self, logits: torch.Tensor, allow: Optional[torch.Tensor] = None,
@@ -107,7 +112,7 @@ class LogitsRules:
         bfloat16; the processed ones are rounded to that dtype, into ``out`` when given
         (``out`` may be ``logits``).  The history is left as it is."""
         if out is None:
-            out = torch.empty(self.batch, self.vocab, dtype=logits.dtype, device=self.device)
+            out = logits.new_empty((self.batch, self.vocab))
         return out, self._run(logits, allow, out, False)
 
     def pick(self, logits: torch.Tensor, allow: Optional[torch.Tensor] = None, record: bool = False) -> torch.Tensor:
@@ -115,31 +120,34 @@ class LogitsRules:
         return self._run(logits, allow, None, record)
 
     def _run(self, logits, allow, out, record):
-        shape = (self.batch, self.vocab)
-        code = N.dtype_code(logits.dtype)
-        for name, t in (("logits", logits), ("out", out)):
-            if t is None:
-                continue
-            if t.shape != shape or t.device != self.device or t.dtype != logits.dtype \
-                    or (t.stride(1) != 1 and self.vocab > 1):
-                raise ValueError(f"{name} must be [{self.batch}, {self.vocab}] {logits.dtype} rows on {self.device}, got "
-                                 f"{t.dtype} {tuple(t.shape)} (strides {t.stride()}) on {t.device}")
-        stride = 0
+        shape, dev, dt = (self.batch, self.vocab), self._index, logits.dtype
+        code = N.dtype_code(dt)
+        stride = logits.stride()
+        if logits.shape != shape or logits.get_device() != dev or stride[1] != 1 and self.vocab > 1:
+            raise ValueError(f"logits must be [{self.batch}, {self.vocab}] rows on {self.device}, got "
+                             f"{tuple(logits.shape)} (strides {stride}) on {logits.device}")
+        out_ptr = out_stride = 0
+        if out is not None:
+            out_ptr, out_stride = out.data_ptr(), out.stride(0)
+            if out.shape != shape or out.get_device() != dev or out.dtype != dt or out.stride(1) != 1 and self.vocab > 1:
+                raise ValueError(f"out must be [{self.batch}, {self.vocab}] {dt} rows on {self.device}, got {out.dtype} "
+                                 f"{tuple(out.shape)} (strides {out.stride()}) on {out.device}")
+        allow_ptr = allow_stride = 0
         if allow is not None:
-            if allow.dim() == 1:
-                allow = allow[None]
-            if allow.dim() != 2 or allow.shape[0] not in (1, self.batch) or allow.dtype != torch.int32 \
-                    or allow.shape[1] < allow_words(self.vocab) or allow.stride(1) != 1 or allow.device != self.device:
-                raise ValueError(f"allow must be int32 [{self.batch} or 1, {allow_words(self.vocab)}] on {self.device}, got "
+            ashape, astride = allow.shape, allow.stride()
+            if len(ashape) == 1:
+                ashape, astride = (1, *ashape), (0, *astride)
+            if len(ashape) != 2 or ashape[0] not in (1, self.batch) or allow.dtype != torch.int32 \
+                    or ashape[1] < self._words or astride[1] != 1 or allow.get_device() != dev:
+                raise ValueError(f"allow must be int32 [{self.batch} or 1, {self._words}] on {self.device}, got "
                                  f"{allow.dtype} {tuple(allow.shape)} on {allow.device}")
-            stride = allow.stride(0) if allow.shape[0] > 1 else 0
-        lib = N.lib_for(self.device)
-        token = torch.empty(self.batch, dtype=torch.int64, device=self.device)
-        a = N.LogitsArgs(dtype=code, record=int(record), logits=logits.data_ptr(), logits_stride=logits.stride(0),
-                         out=N.ptr(out), out_stride=0 if out is None else out.stride(0), token=token.data_ptr(),
-                         allow=N.ptr(allow), allow_stride=stride, **self._fixed)
-        N.check(lib, N.on_device(self.device, lib.spx_logits_rules, a, N.stream_handle(self.device)),
-                "spx_logits_rules")
+            allow_ptr, allow_stride = allow.data_ptr(), astride[0] if ashape[0] > 1 else 0
+        if dev < 0:
+            N.lib_for(self.device)
+        token = logits.new_empty(self.batch, dtype=torch.int64)
+        N.launch_packed("spx_logits_rules", dev, N.LOGITS_PACK.pack(
+            self.batch, self.vocab, code, 1 if record else 0, logits.data_ptr(), stride[0], out_ptr, out_stride,
+            token.data_ptr(), *self._state_ptrs, allow_ptr, allow_stride))
         return token
 
 
@@ -151,17 +159,17 @@ def _setting(name: str, v: Setting, batch: int):
 
 
 def _biases(bias, batch: int, vocab: int):
-    """(row offsets [batch + 1], tokens ascending within a row, values) as host lists."""
-    rows = [bias] * batch if bias is None or isinstance(bias, dict) else list(bias)
-    if len(rows) != batch:
-        raise ValueError(f"logit_bias must be one dict or {batch} of them, got {len(rows)}")
-    at, toks, vals = [0], [], []
-    for d in rows:
+    """(rows, tokens, values) of the biases as host lists, by row and then by token."""
+    each = [bias] * batch if bias is None or isinstance(bias, dict) else list(bias)
+    if len(each) != batch:
+        raise ValueError(f"logit_bias must be one dict or {batch} of them, got {len(each)}")
+    rows, toks, vals = [], [], []
+    for b, d in enumerate(each):
         for t in sorted(d or {}):
             v = float(d[t])
             if not isinstance(t, int) or not 0 <= t < vocab or math.isnan(v) or v == math.inf:
                 raise ValueError(f"logit_bias {{{t!r}: {d[t]!r}}}: a token 0..{vocab - 1} and a number (or -inf) expected")
+            rows.append(b)
             toks.append(t)
             vals.append(v)
-        at.append(len(toks))
-    return at, toks, vals
+    return rows, toks, vals
