@@ -413,7 +413,8 @@ SPX_API int spx_qk_norm_rope(const spx_qk_norm_args* args, void* stream);
 #define SPX_LORA_MAX_RANK 128
 typedef struct spx_lora_args {
   int32_t num_tiles;           /* tiles of up to tile_rows rows of one slot */
-  int32_t tile_rows;           /* 16 or 32 */
+  int32_t tile_rows;           /* 16 or 32; or 128: the rows of a tile are then adjacent
+                                  (order[first + i] = order[first] + i) */
   int32_t num_rows;            /* entries of order */
   int32_t in_features;         /* multiple of 8 */
   int32_t parts;               /* 1..SPX_LORA_MAX_PARTS */
@@ -431,7 +432,9 @@ typedef struct spx_lora_args {
   const float* scales;         /* [slots][parts] */
   const int32_t* tiles;        /* [num_tiles][4]: slot (-1 none), first entry of order, rows, 0 */
   const int32_t* order;        /* [num_rows]: row of x, y and out */
-  float* workspace;            /* f32 [num_rows][parts*max_rank]: the inner products */
+  float* workspace;            /* >= spx_lora_workspace_size(args) bytes: the inner products,
+                                  f32 [num_rows][parts*max_rank], then an int32 that is set to 1
+                                  when a kernel's wait expired (out is not valid then) */
   size_t workspace_bytes;
 } spx_lora_args;
 

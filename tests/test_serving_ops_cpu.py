@@ -77,7 +77,7 @@ def _lora(**kw):
     a = N.LoraArgs(num_tiles=2, tile_rows=16, num_rows=20, in_features=64, parts=2,
                    part_width=(C.c_int32 * 4)(64, 32, 0, 0), max_rank=16, slots=2, dtype=N.SPX_F16, x=256, y=256, out=256,
                    x_stride=64, y_stride=96, out_stride=96, a=256, b=256, ranks=256, scales=256, tiles=256, order=256,
-                   workspace=256, workspace_bytes=20 * 32 * 4)
+                   workspace=256, workspace_bytes=20 * 32 * 4 + 16)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -87,11 +87,11 @@ def _lora(**kw):
     (0, dict(num_tiles=0, x=None)), (1, dict(x=None)), (1, dict(tiles=None)), (2, dict(in_features=60)),
     (2, dict(parts=0)), (2, dict(parts=5)), (2, dict(parts=3)), (2, dict(max_rank=24)), (2, dict(max_rank=144)),
     (2, dict(tile_rows=8)), (2, dict(x_stride=56)), (2, dict(y_stride=88)), (3, dict(dtype=N.SPX_F32)), (4, dict(x=264)),
-    (4, dict(out_stride=100)), (5, dict(workspace=None)), (5, dict(workspace_bytes=20 * 32 * 4 - 1))])
+    (4, dict(out_stride=100)), (5, dict(workspace=None)), (5, dict(workspace_bytes=20 * 32 * 4 + 15))])
 def test_lora_c_refusals(status, kw):
     lib = N.load()
     assert lib.spx_lora_add(_lora(**kw), None) == status
-    assert lib.spx_lora_workspace_size(_lora()) == 20 * 32 * 4
+    assert lib.spx_lora_workspace_size(_lora()) == 20 * 32 * 4 + 16
 
 
 def _logits(**kw):
@@ -141,12 +141,14 @@ def test_qk_norm_python_refusals():
 
 
 def test_lora_batch_groups_rows_by_slot():
-    for slots, tokens in (([2, -1, 2, 0], 1), ([0] * 17, 1), ([1, 0, 1], 33), ([], 4), ([5], 0), ([-1], 2)):
+    for slots, tokens in (([2, -1, 2, 0], 1), ([0] * 17, 1), ([1, 0, 1], 33), ([1, -1, 1], 300), ([0, 0], 64), ([], 4), ([5], 0), ([-1], 2)):
         rows, tiles, order = LoraBatch.tiles_of(slots, tokens)
         assert sorted(order.tolist()) == list(range(len(slots) * tokens))
         seen = []
         for slot, first, n, _ in tiles:
-            assert 1 <= n <= rows and rows in (16, 32)
+            assert 1 <= n <= rows and rows in (16, 32, 128)
+            if rows == 128:
+                assert order[first:first + n].tolist() == list(range(int(order[first]), int(order[first]) + n))
             assert all(slots[r // tokens] == slot for r in order[first:first + n].tolist())
             seen += list(range(first, first + n))
         assert seen == list(range(len(slots) * tokens))

@@ -15,7 +15,7 @@
 // the row type (two MMAs), which keeps about 16 (bf16) or 22 (f16) bits of it.
 #include <cooperative_groups.h>
 
-#include "spx_common.cuh"
+#include "spx_lora.cuh"
 
 namespace spx {
 namespace lora {
@@ -24,46 +24,6 @@ namespace cg = cooperative_groups;
 
 constexpr int SW = 8;    // warps of a shrink CTA
 constexpr int EW = 4;    // warps of an expand CTA
-
-struct Params {
-  const void *x, *y, *a, *b;
-  void* out;
-  int64_t xs, ys, os;
-  const int32_t* ranks;
-  const float* scales;
-  const int4* tiles;
-  const int32_t* order;
-  float* t;
-  int K, parts, R, SR, OUT;
-  int width[SPX_LORA_MAX_PARTS];
-};
-
-template <typename T>
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1);
-template <>
-__device__ __forceinline__ void mma<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                            uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                   uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t pack2(__half lo, __half hi) {
-  return (uint32_t)__half_as_ushort(lo) | ((uint32_t)__half_as_ushort(hi) << 16);
-}
-__device__ __forceinline__ uint32_t pack2(__nv_bfloat16 lo, __nv_bfloat16 hi) {
-  return (uint32_t)__bfloat16_as_ushort(lo) | ((uint32_t)__bfloat16_as_ushort(hi) << 16);
-}
 
 // ------------------------------------------------------------------------- shrink ----
 // Tile of 16 * MT rows x 8 * NT of the parts * max_rank columns; the CTAs of a cluster and
@@ -155,23 +115,44 @@ __global__ void __launch_bounds__(SW * 32) shrink_kernel(const Params p) {
 }
 
 // ------------------------------------------------------------------------- expand ----
-// KS = max_rank / 16 steps of k; a warp owns NC * 8 columns of one part.
+// KS = max_rank / 16 steps of k; a warp owns NC * 8 columns, a CTA EW such groups of one
+// part.  The tile's t is split into its high and low halves once for the CTA, into shared
+// memory in the order of the MMA's fragments (split by every warp for itself and fetched from
+// L2 in the loop it cost 1 to 4 us a call).
 template <typename T, int KS, int NC>
-__global__ void __launch_bounds__(EW * 32) expand_kernel(const Params p) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  int grp = blockIdx.y * EW + (threadIdx.x >> 5), part = 0, first = 0;
-  while (part < p.parts) {   // the part that this group of columns lies in
-    const int n = (p.width[part] + NC * 8 - 1) / (NC * 8);
-    if (grp < n) break;
-    grp -= n;
+__global__ void __launch_bounds__(EW * 32) expand_kernel(const Params p, const int cblocks) {
+  extern __shared__ uint4 frag[];   // [steps of 16 rows][KS][hi, lo][32 lanes], then the row scales (f16)
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  // column blocks of a tile after one another, so that whole rows of y and out are in flight
+  const int blk = blockIdx.x / cblocks;
+  int cb = blockIdx.x - blk * cblocks, part = 0, first = 0;
+  for (;; ++part) {   // the part that this block of columns lies in
+    const int n = (p.width[part] + EW * NC * 8 - 1) / (EW * NC * 8);
+    if (cb < n) break;
+    cb -= n;
     first += p.width[part];
-    ++part;
   }
-  if (part == p.parts) return;
-  const int col0 = grp * NC * 8, left = p.width[part] - col0;   // columns of this part from col0 on
-  const int4 tile = p.tiles[blockIdx.x];
-  const int rank = tile.x < 0 ? 0 : p.ranks[tile.x * p.parts + part];
+  const int col0 = (cb * EW + warp) * NC * 8, left = p.width[part] - col0;   // columns of this part from col0 on
+  const int4 tile = p.tiles[blk];
+  const int rank = tile.x < 0 ? 0 : p.ranks[tile.x * p.parts + part], msteps = (tile.z + 15) / 16;
   const float scale = tile.x < 0 ? 0.f : p.scales[tile.x * p.parts + part];
+  float* row_scale = reinterpret_cast<float*>(frag + msteps * KS * 64);
+  // rows g and g + 8 of a 16-row step
+  int64_t row[2];
+  uint4 yv[NC / 4][2];
+  const auto load = [&](int m, int64_t (&rw)[2], uint4 (&v)[NC / 4][2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = m * 16 + h * 8 + g;
+      rw[h] = r < tile.z ? p.order[tile.y + r] : -1;
+#pragma unroll
+      for (int q = 0; q < NC / 4; ++q)
+        if (rw[h] >= 0 && q * 32 + 8 * c < left)
+          v[q][h] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.y) + rw[h] * p.ys + first + col0 + q * 32 +
+                                                    8 * c);
+    }
+  };
+  load(0, row, yv);
   // B fragments: k of the lane in step ks is ks * 16 + 4c..4c+3; column of n-tile 4q + j,
   // n = g, is 32q + 8 (g / 2) + 2j + g % 2, so that a lane's results are 8 adjacent columns
   uint2 bw[NC][KS];
@@ -188,87 +169,50 @@ __global__ void __launch_bounds__(EW * 32) expand_kernel(const Params p) {
   }
   // t of the shrink kernel; also before the first store, so that this grid never ends
   // before the one that still reads x and writes the workspace
-  bool waited = false;
-  for (int m = 0; m * 16 < tile.z; ++m) {
-    int64_t row[2];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (rank > 0) {
+    for (int m = warp; m < msteps; m += EW) {
+      float sc[2];
+      uint4 f[KS][2];
+      split_t<T, KS>(p.t + (int64_t)(tile.y + m * 16) * p.SR + part * p.R, p.SR, tile.z - m * 16, rank, g, c, f, sc);
+      if (!__is_same(T, __nv_bfloat16) && c == 0) row_scale[m * 16 + g] = sc[0], row_scale[m * 16 + 8 + g] = sc[1];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = m * 16 + h * 8 + g;
-      row[h] = r < tile.z ? p.order[tile.y + r] : -1;
+      for (int ks = 0; ks < KS; ++ks) {
+        frag[(m * KS + ks) * 64 + lane] = f[ks][0];
+        frag[(m * KS + ks) * 64 + 32 + lane] = f[ks][1];
+      }
     }
-    uint4 yv[NC / 4][2];
-#pragma unroll
-    for (int q = 0; q < NC / 4; ++q)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (row[h] >= 0 && q * 32 + 8 * c < left)
-          yv[q][h] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.y) + row[h] * p.ys + first + col0 +
-                                                     q * 32 + 8 * c);
+    __syncthreads();   // rank is the same for the whole CTA
+  }
+  if (left <= 0) return;
+  for (int m = 0; m < msteps; ++m) {
+    int64_t next_row[2] = {-1, -1};
+    uint4 next[NC / 4][2];
+    if (m + 1 < msteps) load(m + 1, next_row, next);
     float acc[NC][4];
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-    float un[2] = {1.f, 1.f};
-    if (!waited) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      waited = true;
-    }
+    float sc[2] = {scale, scale};
     if (rank > 0) {
-      float4 tv[KS][2];
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          tv[ks][h] = row[h] >= 0 && ks * 16 < rank
-                          ? *reinterpret_cast<const float4*>(p.t + (int64_t)(tile.y + m * 16 + h * 8 + g) * p.SR +
-                                                             part * p.R + ks * 16 + 4 * c)
-                          : make_float4(0.f, 0.f, 0.f, 0.f);
-      if (sizeof(T) == 2 && !__is_same(T, __nv_bfloat16)) {
-        // f16: the row is scaled by a power of two so that its largest value is near 2^8
-        // (no overflow of the high parts, no underflow of the low parts), and back below
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float mx = 0.f;
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-            mx = fmaxf(fmaxf(fmaxf(fabsf(tv[ks][h].x), fabsf(tv[ks][h].y)), fmaxf(fabsf(tv[ks][h].z), fabsf(tv[ks][h].w))), mx);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          int ex = (int)((__float_as_uint(mx) >> 23) & 0xff) - 127 - 8;
-          ex = max(-118, min(118, ex));
-          const float dn = __uint_as_float((uint32_t)(127 - ex) << 23);
-          un[h] = __uint_as_float((uint32_t)(127 + ex) << 23);
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-            tv[ks][h].x *= dn, tv[ks][h].y *= dn, tv[ks][h].z *= dn, tv[ks][h].w *= dn;
-        }
+      if (!__is_same(T, __nv_bfloat16)) {
+        sc[0] *= row_scale[m * 16 + g];
+        sc[1] *= row_scale[m * 16 + 8 + g];
       }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         if (ks * 16 >= rank) break;
-        uint32_t hi[4], lo[4];   // a0..a3: row g k-pair 0, row g + 8 k-pair 0, row g k-pair 1, row g + 8 k-pair 1
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float4 v = tv[ks][e & 1];
-          const float f0 = e < 2 ? v.x : v.z, f1 = e < 2 ? v.y : v.w;
-          const T h0 = from_f<T>(f0), h1 = from_f<T>(f1);
-          // an infinity has no low part
-          const float l0 = fabsf(to_f(h0)) < INFINITY ? f0 - to_f(h0) : 0.f;
-          const float l1 = fabsf(to_f(h1)) < INFINITY ? f1 - to_f(h1) : 0.f;
-          hi[e] = pack2(h0, h1);
-          lo[e] = pack2(from_f<T>(l0), from_f<T>(l1));
-        }
+        const uint4 hi = frag[(m * KS + ks) * 64 + lane], lo = frag[(m * KS + ks) * 64 + 32 + lane];
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-          mma<T>(acc[n], lo[0], lo[1], lo[2], lo[3], bw[n][ks].x, bw[n][ks].y);
-          mma<T>(acc[n], hi[0], hi[1], hi[2], hi[3], bw[n][ks].x, bw[n][ks].y);
+          mma<T>(acc[n], lo.x, lo.y, lo.z, lo.w, bw[n][ks].x, bw[n][ks].y);
+          mma<T>(acc[n], hi.x, hi.y, hi.z, hi.w, bw[n][ks].x, bw[n][ks].y);
         }
       }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float sc = scale * un[h];
 #pragma unroll
       for (int q = 0; q < NC / 4; ++q) {
         if (row[h] < 0 || q * 32 + 8 * c >= left) continue;
@@ -279,10 +223,16 @@ __global__ void __launch_bounds__(EW * 32) expand_kernel(const Params p) {
           for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              oe[2 * j + e] = from_f<T>(fmaf(sc, acc[4 * q + j][2 * h + e], to_f(oe[2 * j + e])));
+              oe[2 * j + e] = from_f<T>(fmaf(sc[h], acc[4 * q + j][2 * h + e], to_f(oe[2 * j + e])));
         }
         *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row[h] * p.os + first + col0 + q * 32 + 8 * c) = o;
       }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      row[h] = next_row[h];
+#pragma unroll
+      for (int q = 0; q < NC / 4; ++q) yv[q][h] = next[q][h];
     }
   }
 }
@@ -317,19 +267,25 @@ int launch_shrink(const Params& p, int tiles, int groups, int cs, cudaStream_t s
 }
 
 template <typename T, int KS, int NC>
-int launch_expand(const Params& p, int tiles, cudaStream_t st) {
-  int groups = 0;
-  for (int s = 0; s < p.parts; ++s) groups += (p.width[s] + NC * 8 - 1) / (NC * 8);
+int launch_expand(const Params& p, int tiles, int tile_rows, cudaStream_t st) {
+  int cblocks = 0;
+  for (int s = 0; s < p.parts; ++s) cblocks += (p.width[s] + EW * NC * 8 - 1) / (EW * NC * 8);
+  SPX_REQUIRE((int64_t)tiles * cblocks <= 0x7fffffff, SPX_ERR_SHAPE, "spx_lora_add: too many rows");
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)tiles, (unsigned)((groups + EW - 1) / EW));
+  cfg.gridDim = dim3((unsigned)(tiles * cblocks));
   cfg.blockDim = dim3(EW * 32);
+  cfg.dynamicSmemBytes = (size_t)tile_rows / 16 * KS * 1024 + tile_rows * sizeof(float);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, expand_kernel<T, KS, NC>, p);
+  cudaError_t e = cudaSuccess;
+  if (cfg.dynamicSmemBytes > 48 * 1024)
+    e = cudaFuncSetAttribute(expand_kernel<T, KS, NC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)cfg.dynamicSmemBytes);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, expand_kernel<T, KS, NC>, p, cblocks);
   if (e != cudaSuccess) {
     set_error("lora expand_kernel: %s", cudaGetErrorString(e));
     return SPX_ERR_CUDA;
@@ -338,42 +294,54 @@ int launch_expand(const Params& p, int tiles, cudaStream_t st) {
 }
 
 template <typename T>
-int launch(const Params& p, int tiles, int tile_rows, cudaStream_t st) {
+int launch_shrink_rows(const Params& p, int tiles, int tile_rows, cudaStream_t st) {
   const int groups = (p.SR + 63) / 64;                            // of up to 64 columns
   const int nt = ((p.SR / 8 + groups - 1) / groups + 1) / 2 * 2;  // 2, 4, 6 or 8
   // CTAs that share a tile's k: until the grid fills the SMs, with at least two steps of 32
   // for each warp, 8 at most (the portable cluster size).
   int cs = 1;
   while (cs < 8 && (int64_t)tiles * groups * cs < 148 && p.K >= 32 * SW * 2 * cs) cs *= 2;
-  int rc;
   if (tile_rows == 16) {
-    rc = nt == 2   ? launch_shrink<T, 1, 2>(p, tiles, groups, cs, st)
-         : nt == 4 ? launch_shrink<T, 1, 4>(p, tiles, groups, cs, st)
-         : nt == 6 ? launch_shrink<T, 1, 6>(p, tiles, groups, cs, st)
-                   : launch_shrink<T, 1, 8>(p, tiles, groups, cs, st);
-  } else {
-    rc = nt == 2   ? launch_shrink<T, 2, 2>(p, tiles, groups, cs, st)
+    return nt == 2   ? launch_shrink<T, 1, 2>(p, tiles, groups, cs, st)
+           : nt == 4 ? launch_shrink<T, 1, 4>(p, tiles, groups, cs, st)
+           : nt == 6 ? launch_shrink<T, 1, 6>(p, tiles, groups, cs, st)
+                     : launch_shrink<T, 1, 8>(p, tiles, groups, cs, st);
+  }
+  return nt == 2   ? launch_shrink<T, 2, 2>(p, tiles, groups, cs, st)
          : nt == 4 ? launch_shrink<T, 2, 4>(p, tiles, groups, cs, st)
          : nt == 6 ? launch_shrink<T, 2, 6>(p, tiles, groups, cs, st)
                    : launch_shrink<T, 2, 8>(p, tiles, groups, cs, st);
+}
+
+template <typename T>
+int launch(const Params& p, int dtype, int tiles, int tile_rows, cudaStream_t st) {
+  if (tile_rows == 128) {
+    const int rc = shrink_block_launch(p, dtype, tiles, st);
+    return rc == SPX_OK ? expand_block_launch(p, dtype, tiles, st) : rc;
   }
+  const int rc = launch_shrink_rows<T>(p, tiles, tile_rows, st);
   if (rc != SPX_OK) return rc;
   switch (p.R / 16) {
-    case 1: return launch_expand<T, 1, 8>(p, tiles, st);
-    case 2: return launch_expand<T, 2, 8>(p, tiles, st);
-    case 3: return launch_expand<T, 3, 8>(p, tiles, st);
-    case 4: return launch_expand<T, 4, 8>(p, tiles, st);
+    case 1: return launch_expand<T, 1, 8>(p, tiles, tile_rows, st);
+    case 2: return launch_expand<T, 2, 8>(p, tiles, tile_rows, st);
+    case 3: return launch_expand<T, 3, 8>(p, tiles, tile_rows, st);
+    case 4: return launch_expand<T, 4, 8>(p, tiles, tile_rows, st);
     case 5:
-    case 6: return launch_expand<T, 6, 4>(p, tiles, st);
-    default: return launch_expand<T, 8, 4>(p, tiles, st);
+    case 6: return launch_expand<T, 6, 4>(p, tiles, tile_rows, st);
+    default: return launch_expand<T, 8, 4>(p, tiles, tile_rows, st);
   }
+}
+
+// the inner products and the word that says a wait expired
+static size_t workspace_bytes(const spx_lora_args* a) {
+  return ((size_t)a->num_rows * a->parts * a->max_rank + 4) * sizeof(float);
 }
 
 static int validate(const spx_lora_args* a) {
   SPX_REQUIRE(a, SPX_ERR_NULL, "spx_lora_add: args are required");
   SPX_REQUIRE(a->dtype == SPX_F16 || a->dtype == SPX_BF16, SPX_ERR_UNSUPPORTED,
               "spx_lora_add: dtype must be F16 or BF16");
-  SPX_REQUIRE(a->num_tiles >= 0 && a->num_rows >= 0 && (a->tile_rows == 16 || a->tile_rows == 32) &&
+  SPX_REQUIRE(a->num_tiles >= 0 && a->num_rows >= 0 && (a->tile_rows == 16 || a->tile_rows == 32 || a->tile_rows == 128) &&
                   a->num_tiles <= (1 << 27),
               SPX_ERR_SHAPE, "spx_lora_add: bad tiling: %d tiles of %d rows", a->num_tiles, a->tile_rows);
   SPX_REQUIRE(a->in_features >= 8 && a->in_features % 8 == 0 && a->in_features <= (1 << 24), SPX_ERR_SHAPE,
@@ -406,13 +374,13 @@ using namespace spx;
 
 size_t spx_lora_workspace_size(const spx_lora_args* a) {
   if (!a || lora::validate(a) != SPX_OK) return 0;
-  return (size_t)a->num_rows * a->parts * a->max_rank * sizeof(float);
+  return lora::workspace_bytes(a);
 }
 
 int spx_lora_add(const spx_lora_args* a, void* stream) {
   const int rc = lora::validate(a);
   if (rc != SPX_OK || a->num_tiles == 0) return rc;
-  const size_t need = (size_t)a->num_rows * a->parts * a->max_rank * sizeof(float);
+  const size_t need = lora::workspace_bytes(a);
   SPX_REQUIRE(a->workspace && a->workspace_bytes >= need, SPX_ERR_WORKSPACE,
               "spx_lora_add: workspace of %zu bytes needed, %zu given", need, a->workspace ? a->workspace_bytes : 0);
   lora::Params p{};
@@ -421,9 +389,10 @@ int spx_lora_add(const spx_lora_args* a, void* stream) {
   p.ranks = a->ranks, p.scales = a->scales;
   p.tiles = static_cast<const int4*>(static_cast<const void*>(a->tiles));
   p.order = a->order, p.t = a->workspace;
+  p.rows = a->num_rows, p.slots = a->slots;
   p.K = a->in_features, p.parts = a->parts, p.R = a->max_rank, p.SR = a->parts * a->max_rank;
   for (int s = 0; s < a->parts; ++s) p.width[s] = a->part_width[s], p.OUT += a->part_width[s];
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return a->dtype == SPX_BF16 ? lora::launch<__nv_bfloat16>(p, a->num_tiles, a->tile_rows, st)
-                              : lora::launch<__half>(p, a->num_tiles, a->tile_rows, st);
+  return a->dtype == SPX_BF16 ? lora::launch<__nv_bfloat16>(p, a->dtype, a->num_tiles, a->tile_rows, st)
+                              : lora::launch<__half>(p, a->dtype, a->num_tiles, a->tile_rows, st);
 }

@@ -47,21 +47,26 @@ class LoraBatch:
 
     @staticmethod
     def tiles_of(slots: Sequence[int], tokens: int):
-        """Host lists ``(tile_rows, tiles, order)``: rows sorted by slot, cut into tiles of
-        one slot.  16 rows are one MMA tile; groups beyond that use 32, which reads the
-        adapter's weights half as often."""
+        """Host lists ``(tile_rows, tiles, order)``: rows sorted by slot, cut into tiles of one
+        slot.  Prompts: tiles of up to 128 tokens of one sequence (the kernel on the 5th
+        generation's tensor cores).  Few tokens: 16 rows of any sequences, or 32 where a slot
+        has more, which reads the adapter's weights half as often."""
         groups: Dict[int, list] = {}
         for i, s in enumerate(slots):
             groups.setdefault(s, []).append(i)
         most = max((len(g) for g in groups.values()), default=0) * tokens
-        rows = 16 if most <= 16 else 32
+        rows = 128 if tokens >= 64 else 16 if most <= 16 else 32
         order = torch.empty(len(slots) * tokens, dtype=torch.int32)
         tiles, at = [], 0
         for s in sorted(groups):
             seqs = torch.tensor(groups[s], dtype=torch.int32)
             n = len(groups[s]) * tokens
             order[at:at + n] = (seqs[:, None] * tokens + torch.arange(tokens, dtype=torch.int32)[None]).reshape(-1)
-            tiles += [(s, at + i, min(rows, n - i), 0) for i in range(0, n, rows)]
+            if rows == 128:
+                tiles += [(s, at + q * tokens + i, min(rows, tokens - i), 0) for q in range(len(groups[s]))
+                          for i in range(0, tokens, rows)]
+            else:
+                tiles += [(s, at + i, min(rows, n - i), 0) for i in range(0, n, rows)]
             at += n
         return rows, tiles, order
 
@@ -167,7 +172,7 @@ class LoraPool:
         rows, n_tiles, n, tiles, order = batch._plan(tokens)
         # the inner products, a buffer of each call's own: two streams or two captured graphs
         # never share one (the caching allocator hands it out in stream order)
-        size = n * len(self.widths) * self._rank
+        size = n * len(self.widths) * self._rank + 4
         ws = self.scales.new_empty(size)
         N.launch_packed("spx_lora_add", dev, N.LORA_PACK.pack(
             n_tiles, rows, n, *self._pool_args, x.data_ptr(), y.data_ptr(), out.data_ptr(), _row_stride(x),
