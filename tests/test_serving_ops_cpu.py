@@ -141,8 +141,11 @@ def test_qk_norm_python_refusals():
 
 
 def test_lora_batch_groups_rows_by_slot():
-    for slots, tokens in (([2, -1, 2, 0], 1), ([0] * 17, 1), ([1, 0, 1], 33), ([1, -1, 1], 300), ([0, 0], 64), ([], 4), ([5], 0), ([-1], 2)):
-        rows, tiles, order = LoraBatch.tiles_of(slots, tokens)
+    for slots, tokens, blocks in (([2, -1, 2, 0], 1, False), ([0] * 17, 1, False), ([1, 0, 1], 33, False),
+                                  ([1, -1, 1], 300, True), ([0, 0], 64, True), ([0, 0], 64, False), ([], 4, False),
+                                  ([5], 0, False), ([-1], 2, False)):
+        rows, tiles, order = LoraBatch.tiles_of(slots, tokens, blocks)
+        assert (rows == 128) == blocks
         assert sorted(order.tolist()) == list(range(len(slots) * tokens))
         seen = []
         for slot, first, n, _ in tiles:

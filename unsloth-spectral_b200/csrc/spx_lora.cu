@@ -27,10 +27,28 @@ constexpr int EW = 4;    // warps of an expand CTA
 
 // ------------------------------------------------------------------------- shrink ----
 // Tile of 16 * MT rows x 8 * NT of the parts * max_rank columns; the CTAs of a cluster and
-// their warps take the 32-wide steps of k in turn.
+// their warps take the 32-wide steps of k in turn.  Each lane copies the 16-byte vectors that
+// it will use itself into a ring of its own (cp.async, no barrier), so that a warp has several
+// steps in flight without registers: loaded into registers, 64 rows of 24 slots at K = 14336,
+// rank 64 took 19 us, with 10 warps an SM waiting for memory.
+template <int MT, int NT>
+struct Ring {
+  static constexpr int VECS = 2 * MT + NT;                                   // 16 bytes a lane each
+  static constexpr int FIT = 73 * 1024 / (SW * VECS * 512), STAGES = FIT > 6 ? 6 : FIT < 2 ? 2 : FIT;   // three CTAs an SM
+  static constexpr size_t BYTES = (size_t)SW * STAGES * VECS * 512;
+};
+
+__device__ __forceinline__ void copy16(uint4* dst, const void* src, bool in) {   // zeros unless `in`
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+               "r"(in ? 16 : 0)
+               : "memory");
+}
+
 template <typename T, int MT, int NT>
 __global__ void __launch_bounds__(SW * 32) shrink_kernel(const Params p) {
-  extern __shared__ float sums[];   // [SW][MT * 16][NT * 8]
+  using Ri = Ring<MT, NT>;
+  extern __shared__ uint4 ring[];
+  float* const sums = reinterpret_cast<float*>(ring);   // [SW][MT * 16][NT * 8], after the stream
   cg::cluster_group cl = cg::this_cluster();
   const int cs = (int)cl.num_blocks(), cr = (int)cl.block_rank();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -60,38 +78,58 @@ __global__ void __launch_bounds__(SW * 32) shrink_kernel(const Params p) {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
-  const int steps = (p.K + 31) / 32;
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  if (act) {
-#pragma unroll 2
-    for (int s = cr * SW + warp; s < steps; s += cs * SW) {
+  const int steps = (p.K + 31) / 32, first = cr * SW + warp, stride = cs * SW;
+  const int mine = act && first < steps ? (steps - first + stride - 1) / stride : 0;
+  uint4* const own = ring + (size_t)warp * Ri::STAGES * Ri::VECS * 32 + lane;
+  const auto fetch = [&](int i) {
+    if (i < mine) {
+      const int s = first + i * stride;
       const bool in = s * 32 + 8 * c < p.K;
-      uint4 xa[MT][2], bw[NT];
+      uint4* d = own + (i % Ri::STAGES) * Ri::VECS * 32;
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          xa[m][h] = in && xr[m][h] ? *reinterpret_cast<const uint4*>(xr[m][h] + s * 32) : zero;
+          copy16(d + (2 * m + h) * 32, in && xr[m][h] ? (const void*)(xr[m][h] + s * 32) : p.x, in && xr[m][h]);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
-        bw[n] = in && ((act >> n) & 1u) ? *reinterpret_cast<const uint4*>(ar + (int64_t)n * 8 * p.K + s * 32) : zero;
+        if ((act >> n) & 1u)
+          copy16(d + (2 * MT + n) * 32, in ? (const void*)(ar + (int64_t)n * 8 * p.K + s * 32) : p.a, in);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+  for (int i = 0; i < Ri::STAGES - 1; ++i) fetch(i);
+  for (int i = 0; i < mine; ++i) {
+    fetch(i + Ri::STAGES - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(Ri::STAGES - 1) : "memory");
+    const uint4* d = own + (i % Ri::STAGES) * Ri::VECS * 32;
+    uint4 xa[MT][2];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          mma<T>(acc[m][n], xa[m][0].x, xa[m][1].x, xa[m][0].y, xa[m][1].y, bw[n].x, bw[n].y);
-          mma<T>(acc[m][n], xa[m][0].z, xa[m][1].z, xa[m][0].w, xa[m][1].w, bw[n].z, bw[n].w);
-        }
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) xa[m][h] = d[(2 * m + h) * 32];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (!((act >> n) & 1u)) continue;
+      const uint4 bw = d[(2 * MT + n) * 32];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        mma<T>(acc[m][n], xa[m][0].x, xa[m][1].x, xa[m][0].y, xa[m][1].y, bw.x, bw.y);
+        mma<T>(acc[m][n], xa[m][0].z, xa[m][1].z, xa[m][0].w, xa[m][1].w, bw.z, bw.w);
+      }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();   // the ring becomes the sums
   constexpr int N = NT * 8, E = MT * 16 * N;
-  float* mine = sums + warp * E;
+  float* part = sums + warp * E;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      *reinterpret_cast<float2*>(mine + (m * 16 + g) * N + n * 8 + 2 * c) = make_float2(acc[m][n][0], acc[m][n][1]);
-      *reinterpret_cast<float2*>(mine + (m * 16 + g + 8) * N + n * 8 + 2 * c) = make_float2(acc[m][n][2], acc[m][n][3]);
+      *reinterpret_cast<float2*>(part + (m * 16 + g) * N + n * 8 + 2 * c) = make_float2(acc[m][n][0], acc[m][n][1]);
+      *reinterpret_cast<float2*>(part + (m * 16 + g + 8) * N + n * 8 + 2 * c) = make_float2(acc[m][n][2], acc[m][n][3]);
     }
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += SW * 32) {   // each thread its own elements: in place
@@ -239,7 +277,8 @@ __global__ void __launch_bounds__(EW * 32) expand_kernel(const Params p, const i
 
 template <typename T, int MT, int NT>
 int launch_shrink(const Params& p, int tiles, int groups, int cs, cudaStream_t st) {
-  const size_t smem = (size_t)SW * MT * 16 * NT * 8 * sizeof(float);
+  const size_t sums = (size_t)SW * MT * 16 * NT * 8 * sizeof(float);
+  const size_t smem = sums > Ring<MT, NT>::BYTES ? sums : Ring<MT, NT>::BYTES;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(shrink_kernel<T, MT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)smem);
@@ -295,12 +334,15 @@ int launch_expand(const Params& p, int tiles, int tile_rows, cudaStream_t st) {
 
 template <typename T>
 int launch_shrink_rows(const Params& p, int tiles, int tile_rows, cudaStream_t st) {
-  const int groups = (p.SR + 63) / 64;                            // of up to 64 columns
+  // Columns of a CTA: 16 while two CTAs an SM hold the whole grid (one request on q|k|v 5.6 us
+  // against 6.8 with 48), else as many as leave the rows enough warps: each group reads x again.
+  const int cols = (int64_t)tiles * (p.SR / 16) * 8 <= 2 * 148 ? 16 : tile_rows == 16 ? 32 : 64;
+  const int groups = (p.SR + cols - 1) / cols;                 
   const int nt = ((p.SR / 8 + groups - 1) / groups + 1) / 2 * 2;  // 2, 4, 6 or 8
-  // CTAs that share a tile's k: until the grid fills the SMs, with at least two steps of 32
-  // for each warp, 8 at most (the portable cluster size).
+  // CTAs that share a tile's k: until three CTAs an SM hold the grid, with at least two steps of
+  // 32 for each warp, 8 at most (the portable cluster size).
   int cs = 1;
-  while (cs < 8 && (int64_t)tiles * groups * cs < 148 && p.K >= 32 * SW * 2 * cs) cs *= 2;
+  while (cs < 8 && (int64_t)tiles * groups * cs * 2 <= 3 * 148 && p.K >= 32 * SW * 2 * cs) cs *= 2;
   if (tile_rows == 16) {
     return nt == 2   ? launch_shrink<T, 1, 2>(p, tiles, groups, cs, st)
            : nt == 4 ? launch_shrink<T, 1, 4>(p, tiles, groups, cs, st)

@@ -4,8 +4,9 @@
 // (128-byte swizzle) through a ring of stages, one thread issues tcgen05.mma (M = 128 rows,
 // N = parts * rank columns, f32 in tensor memory), and x is read once, whatever the rank.
 // Bound by memory: 2 * N flops a byte of x at most.  Two CTAs an SM keep about 128 KB of x in
-// flight, where the mma.sync kernel (fragments loaded by the warps that use them) had 8 warps
-// an SM.  Few tiles: the CTAs of a cluster split k and add their sums over distributed shared
+// flight: 268 MB of x (8 x 4096 rows of 4096 bf16) take 55 to 61 us, as long as a plain sum
+// over them; the mma.sync kernel (fragments loaded by the warps that use them, 8 warps an SM)
+// took 214.  More stages, or boxes twice as wide, measured level.  Few tiles: the CTAs of a cluster split k and add their sums over distributed shared
 // memory in a fixed order.  Rows of the next sequence that a tile's box covers are computed
 // and not stored.  Every wait is bounded; an expired one leaves NaN in t.
 #include <cooperative_groups.h>
@@ -21,6 +22,7 @@ using namespace sm100;
 namespace cg = cooperative_groups;
 
 constexpr int M = 128, KB = 64;            // rows of a tile, values of k in a stage
+constexpr int MAXSTAGES = 8;               // barriers of a ring
 constexpr int XBYTES = M * KB * 2;
 
 struct Cfg {
@@ -64,20 +66,22 @@ __device__ __forceinline__ void tld16(uint32_t taddr, float (&v)[16]) {
 // 128 threads: thread 0 copies, thread 32 issues the MMAs, all four warps read the sums.
 __global__ void __launch_bounds__(128) shrink_block_kernel(const __grid_constant__ CUtensorMap mx,
                                                            const __grid_constant__ CUtensorMap ma, const Params p,
-                                                           const int nb, const int stages, const uint32_t idesc) {
+                                                           const int nb, const int groups, const int stages, const uint32_t idesc) {
   extern __shared__ uint8_t raw_smem[];
-  __shared__ __align__(8) uint64_t bars[2 * 8 + 1];
+  __shared__ __align__(8) uint64_t bars[2 * MAXSTAGES + 1];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   cg::cluster_group cl = cg::this_cluster();
   const int cs = (int)cl.num_blocks(), cr = (int)cl.block_rank();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int4 tile = p.tiles[blockIdx.x / cs];
+  // the groups of columns of a tile after one another: x comes from memory once
+  const int unit = blockIdx.x / cs, group = unit % groups;
+  const int4 tile = p.tiles[unit / groups];
   if (tile.x < 0) return;   // rows without an adapter: the whole cluster leaves
   const int tid = threadIdx.x, warp = tid >> 5;
-  const int col0 = blockIdx.y * nb, row0 = p.order[tile.y];
+  const int col0 = group * nb, row0 = p.order[tile.y];
   const uint32_t base = (smem_u32(raw_smem) + 1023u) & ~1023u;
-  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * 8, done = full0 + 16 * 8;
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * MAXSTAGES, done = empty0 + 8 * MAXSTAGES;
   const int sbytes = XBYTES + nb * KB * 2;
   uint32_t ncols = 32;
   while ((int)ncols < nb) ncols *= 2;
@@ -183,63 +187,175 @@ __global__ void __launch_bounds__(128) shrink_block_kernel(const __grid_constant
 }
 
 // ------------------------------------------------------------------------- expand ----
-// out = y + scale * B t as a stream of chunks of 128 rows x 64 columns: a fifth warp copies y
-// and the chunk's rows of B through a ring of stages with TMA; four warps take 32 rows each,
-// add the product (mma.sync: 2 * rank flops for 4 bytes of y and out, so the tensor cores
-// idle either way) in the stage itself and store from there with TMA.  The chunks of all
-// tiles are dealt out evenly to a grid that is resident at once.  The stream through registers
-// (16 warps an SM, 2 KB in flight each) reached 4.6 TB/s.
-constexpr int EC = 64, EROWS = 32, YBYTES = M * EC * 2;
+// out = y + scale * B t as a stream of chunks of 128 rows x 128 columns.  One warp copies y
+// and the chunk's rows of B through a ring of stages with TMA; four warps make the A operand
+// of a tile and part (t, its high and low halves in two values of the row type each), one
+// ahead of its use; one thread issues the MMAs (f32 in tensor memory, two buffers); eight
+// warps add the product to y in the stage itself (thread = row, half of the columns) and
+// store from there with TMA.  The chunks of all tiles are dealt out evenly to one CTA an SM.
+// Before: y through registers (16 warps an SM, 2 KB in flight each) 4.6 TB/s; this ring with
+// mma.sync 4.9 TB/s at rank 16, but 1.5 TB/s at rank 64; with t staged by the warps that
+// store, 3 to 4 us of each change of tile or part showed.
+constexpr int EC = 128, EROWS = 32, YBOX = M * 64 * 2, YBYTES = 2 * YBOX, EWARPS = 8, BWARPS = 4;
+constexpr int ETHREADS = (EWARPS + 2 + BWARPS) * 32;
+
+// What the warps need to know of a tile and part: a version of the A operand.
+struct Version {
+  int rank, row0, rows;
+  float scale;
+};
 
 struct Chunks {
   int per_tile, total;                          // chunks of a tile, of all tiles
   int first[SPX_LORA_MAX_PARTS + 1];            // first chunk of each part
+  int kw;                                       // ranks of a box of B: 16, 32 or 64
 };
 
-template <typename T, int KS>
-__global__ void __launch_bounds__(160) expand_block_kernel(const __grid_constant__ CUtensorMap my,
-                                                           const __grid_constant__ CUtensorMap mb,
-                                                           const __grid_constant__ CUtensorMap mo, const Params p,
-                                                           const Chunks ch, const int stages) {
+// K-major operand tiles of rows of 2 * kw bytes, swizzled over that width.
+__device__ __forceinline__ uint64_t desc_kw(uint32_t saddr, int kw) {
+  const uint64_t type = kw == 64 ? 2ull : kw == 32 ? 4ull : 6ull;
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(uint32_t)kw << 32) | (1ull << 46) | (type << 61);
+}
+__device__ __forceinline__ void tld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int u = 0; u < 32; ++u) v[u] = __uint_as_float(r[u]);
+}
+
+// Row r of a tile's t as the high and low parts of the A operand: element (row, k) at
+// (k / 8) * 2048 + row * 16 + (k % 8) * 2, the low parts 256 R bytes on.  Returns what the row
+// of the product is to be multiplied by.
+template <typename T>
+__device__ __forceinline__ float stage_t(const float* t, bool in, int R, int r, uint8_t* a) {
+  float dn = 1.f, up = 1.f;
+  if (!__is_same(T, __nv_bfloat16)) {
+    // f16: scaled by a power of two so that the row's largest value is near 2^8 (no overflow
+    // of the high parts, no underflow of the low parts)
+    float mx = 0.f;
+    for (int k = 0; in && k < R; k += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(t + k);
+      mx = fmaxf(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))), mx);
+    }
+    int ex = (int)((__float_as_uint(mx) >> 23) & 0xff) - 127 - 8;
+    ex = max(-118, min(118, ex));
+    dn = __uint_as_float((uint32_t)(127 - ex) << 23);
+    up = __uint_as_float((uint32_t)(127 + ex) << 23);
+  }
+#pragma unroll 4
+  for (int k8 = 0; k8 < R / 8; ++k8) {
+    uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
+    if (in) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const float4 v = *reinterpret_cast<const float4*>(t + k8 * 8 + q * 4);
+        const float f[4] = {v.x * dn, v.y * dn, v.z * dn, v.w * dn};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const T h = from_f<T>(f[e]);
+          reinterpret_cast<T*>(&hi)[q * 4 + e] = h;
+          // an infinity has no low part
+          reinterpret_cast<T*>(&lo)[q * 4 + e] = from_f<T>(fabsf(to_f(h)) < INFINITY ? f[e] - to_f(h) : 0.f);
+        }
+      }
+    }
+    *reinterpret_cast<uint4*>(a + k8 * 2048 + r * 16) = hi;
+    *reinterpret_cast<uint4*>(a + 256 * R + k8 * 2048 + r * 16) = lo;
+  }
+  return up;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_constant__ CUtensorMap my,
+                                                                         const __grid_constant__ CUtensorMap mb,
+                                                                         const __grid_constant__ CUtensorMap mo,
+                                                                         const Params p, const Chunks ch,
+                                                                         const int stages, const int abufs, const uint32_t idesc) {
   extern __shared__ uint8_t raw_smem[];
-  __shared__ __align__(8) uint64_t bars[2 * 8];
+  __shared__ __align__(8) uint64_t bars[2 * MAXSTAGES + 8];
+  __shared__ Version versions[2];
+  __shared__ float row_scale[2][M];
+  __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (smem_u32(raw_smem) + 1023u) & ~1023u;
   uint8_t* const sm = raw_smem + (base - smem_u32(raw_smem));
-  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * 8;
-  const int bbytes = EC * p.R * 2, sbytes = YBYTES + (bbytes + 1023) / 1024 * 1024;
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * MAXSTAGES, acc_full0 = empty0 + 8 * MAXSTAGES,
+                 acc_empty0 = acc_full0 + 16, t_ready0 = acc_empty0 + 16, t_free0 = t_ready0 + 16;
+  const int bbytes = EC * p.R * 2, sbytes = YBYTES + bbytes;
+  uint8_t* const a_op = sm + stages * sbytes;   // abufs buffers of 512 R bytes
+  if (warp == EWARPS + 1) {
+    tmem_alloc(smem_u32(&s_tmem), 2 * EC);
+    tmem_relinquish();
+  }
   if (tid == 0) {
     s_abort = 0;
-    for (int s = 0; s < stages; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, 4);
+    for (int s = 0; s < stages; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, EWARPS);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(acc_full0 + 8 * s, 1), mbar_init(acc_empty0 + 8 * s, EWARPS);
+      mbar_init(t_ready0 + 8 * s, BWARPS), mbar_init(t_free0 + 8 * s, EWARPS + 1);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async;" ::: "memory");
   }
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
   const Abort ab{&s_abort, reinterpret_cast<int*>(p.t + (int64_t)p.rows * p.SR)};
   const int c0 = (int)((int64_t)ch.total * blockIdx.x / gridDim.x), c1 = (int)((int64_t)ch.total * (blockIdx.x + 1) / gridDim.x);
-  // chunk q: its tile, part, first column within the part's range of y
-  const auto where = [&](int q, int& tile, int& part, int& col) {
-    tile = q / ch.per_tile;
-    const int k = q - tile * ch.per_tile;
-    part = 0;
-    int off = 0;
-    while (k >= ch.first[part + 1]) off += p.width[part++];
-    col = off + (k - ch.first[part]) * EC;
+
+  // The walk over the CTA's chunks, the same in every role.
+  struct Walk {
+    int tl, part, k, col, left;   // tile, part, chunk within the tile, first column, columns of the part from there on
+    bool fresh;                   // another tile or part than the chunk before: a new version
+    __device__ __forceinline__ Walk(const Params& p, const Chunks& ch, int q) {
+      tl = q / ch.per_tile;
+      k = q - tl * ch.per_tile;
+      part = 0, col = 0;
+      while (k >= ch.first[part + 1]) col += p.width[part++];
+      left = p.width[part] - (k - ch.first[part]) * EC;
+      col += (k - ch.first[part]) * EC;
+      fresh = true;
+    }
+    __device__ __forceinline__ void next(const Params& p, const Chunks& ch) {
+      fresh = ++k == ch.first[part + 1];
+      if (!fresh) {
+        col += EC, left -= EC;
+        return;
+      }
+      col += left;
+      if (++part == p.parts) part = 0, k = 0, col = 0, ++tl;
+      left = p.width[part];
+    }
   };
-  if (warp == 4) {
+
+  if (warp == EWARPS) {
     if (lane == 0) {
-      int i = 0;
-      for (; c0 + i < c1; ++i) {
+      int i = 0, row0 = 0;
+      int4 tile = make_int4(0, 0, 0, 0);
+      for (Walk w(p, ch, c0); c0 + i < c1; ++i, w.next(p, ch)) {
+        if (w.fresh) tile = p.tiles[w.tl], row0 = p.order[tile.y];
         const int s = i % stages;
         if (i >= stages && !wait1(empty0 + 8 * s, (uint32_t)((i / stages - 1) & 1), ab)) break;
-        int tl, part, col;
-        where(c0 + i, tl, part, col);
-        const int4 tile = p.tiles[tl];
         const uint32_t dst = base + s * sbytes, bar = full0 + 8 * s;
-        mbar_expect_tx(bar, (uint32_t)(YBYTES + (tile.x >= 0 ? bbytes : 0)));
-        tma_2d(dst, &my, col, p.order[tile.y], bar);
-        if (tile.x >= 0) tma_2d(dst + YBYTES, &mb, 0, tile.x * p.OUT + col, bar);
+        // a box that begins past the part is not wanted (and past the last one lies outside)
+        const bool two = w.left > 64;
+        mbar_expect_tx(bar, (uint32_t)((two ? YBYTES : YBOX) + (tile.x >= 0 ? bbytes : 0)));
+        tma_2d(dst, &my, w.col, row0, bar);
+        if (two) tma_2d(dst + YBOX, &my, w.col + 64, row0, bar);
+        if (tile.x >= 0)
+          for (int b = 0; b < p.R / ch.kw; ++b)
+            tma_2d(dst + YBYTES + b * EC * ch.kw * 2, &mb, b * ch.kw, tile.x * p.OUT + w.col, bar);
       }
       if (c0 + i < c1) {   // given up: the copies in flight land before the shared memory goes
         for (int q = i > stages ? i - stages : 0; q < i; ++q) {
@@ -249,102 +365,141 @@ __global__ void __launch_bounds__(160) expand_block_kernel(const __grid_constant
         }
       }
     }
-    return;
-  }
-  // t of the shrink kernel; also before the first store, so that this grid never ends before
-  // the one that still reads x and writes the workspace
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int g = lane >> 2, c = lane & 3;
-  int held = -1, held_part = -1, rank = 0, row0 = 0;
-  float scale = 0.f, sc[2][2];
-  uint4 f[2][KS][2];
-  int4 tile = make_int4(0, 0, 0, 0);
-  for (int i = 0; c0 + i < c1; ++i) {
-    const int s = i % stages;
-    int tl, part, col;
-    where(c0 + i, tl, part, col);
-    if (tl != held || part != held_part) {   // t of another tile or part
-      held = tl, held_part = part;
-      tile = p.tiles[tl];
-      row0 = p.order[tile.y];
-      rank = tile.x < 0 ? 0 : p.ranks[tile.x * p.parts + part];
-      scale = tile.x < 0 ? 0.f : p.scales[tile.x * p.parts + part];
-      if (rank > 0) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-          split_t<T, KS>(p.t + (int64_t)(tile.y + warp * EROWS + m * 16) * p.SR + part * p.R, p.SR,
-                         tile.z - warp * EROWS - m * 16, rank, g, c, f[m], sc[m]);
-      }
-    }
-    int left = -col;   // columns of the part from here on
-    for (int q = 0; q <= part; ++q) left += p.width[q];
-    if (!waitw(full0 + 8 * s, (uint32_t)((i / stages) & 1), ab)) break;
-    uint8_t* const ys = sm + s * sbytes;
-    const uint8_t* const bs = ys + YBYTES;
-    const int rows = min(tile.z - warp * EROWS, EROWS);
-    const bool tma_out = rows == EROWS && left >= EC;
-    if (rows > 0) {
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        float acc[8][4];
-#pragma unroll
-        for (int n = 0; n < 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-        if (rank > 0) {
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            if (ks * 16 >= rank) break;
-#pragma unroll
-            for (int n = 0; n < 8; ++n) {
-              const int bc = (n / 4) * 32 + 8 * (g >> 1) + 2 * (n % 4) + (g & 1);
-              const uint2 b = *reinterpret_cast<const uint2*>(bs + bc * p.R * 2 + ks * 32 + 8 * c);
-              mma<T>(acc[n], f[m][ks][1].x, f[m][ks][1].y, f[m][ks][1].z, f[m][ks][1].w, b.x, b.y);
-              mma<T>(acc[n], f[m][ks][0].x, f[m][ks][0].y, f[m][ks][0].z, f[m][ks][0].w, b.x, b.y);
-            }
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = warp * EROWS + m * 16 + h * 8 + g;   // row of the tile
-          const float s1 = scale * (rank > 0 ? sc[m][h] : 0.f);
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint4* at = reinterpret_cast<uint4*>(ys + r * 128 + (((q * 4 + c) ^ (r & 7)) << 4));
-            uint4 o = *at;
-            if (rank > 0) {
-              T* oe = reinterpret_cast<T*>(&o);
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                  oe[2 * j + e] = from_f<T>(fmaf(s1, acc[4 * q + j][2 * h + e], to_f(oe[2 * j + e])));
-            }
-            if (tma_out) {
-              if (rank > 0) *at = o;
-            } else if (r < tile.z && q * 32 + 8 * c < left) {   // neither rows of the next sequence nor columns of the next part
-              *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)(row0 + r) * p.os + col + q * 32 + 8 * c) = o;
-            }
-          }
-        }
-      }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
+  } else if (warp == EWARPS + 1) {
     if (lane == 0) {
-      if (tma_out) {
-        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&mo),
-                     "r"(col), "r"(row0 + warp * EROWS), "r"(base + s * sbytes + warp * EROWS * 128)
-                     : "memory");
+      int i = 0, n = 0, v = -1, rank = 0, buf = 0;   // chunk, accumulators used, version
+      for (Walk w(p, ch, c0); c0 + i < c1; ++i, w.next(p, ch)) {
+        if (w.fresh) {
+          if (v >= 0) umma_commit(t_free0 + 8 * buf);   // once the MMAs that read it are done
+          ++v;
+          buf = v % abufs;
+          if (!wait1(t_ready0 + 8 * buf, (uint32_t)((v / abufs) & 1), ab)) break;
+          rank = versions[buf].rank;
+        }
+        if (rank <= 0) continue;
+        const int s = i % stages, a = n & 1;
+        if (!wait1(full0 + 8 * s, (uint32_t)((i / stages) & 1), ab)) break;
+        if (n >= 2 && !wait1(acc_empty0 + 8 * a, (uint32_t)((n / 2 - 1) & 1), ab)) break;
+        tc_fence_after();
+        const uint32_t bo = base + s * sbytes + YBYTES, ao = smem_u32(a_op) + buf * 512 * p.R;
+        for (int ks = 0; ks * 16 < rank; ++ks) {
+          const uint64_t bd = desc_kw(bo + (ks * 16 / ch.kw) * EC * ch.kw * 2 + ks * 16 % ch.kw * 2, ch.kw);
+          umma(tmem + a * EC, umma_desc(ao + 256 * p.R + ks * 4096, 2048, 128), bd, idesc, ks > 0 ? 1u : 0u);
+          umma(tmem + a * EC, umma_desc(ao + ks * 4096, 2048, 128), bd, idesc, 1u);
+        }
+        umma_commit(acc_full0 + 8 * a);
+        ++n;
       }
-      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      // the chunk before this one is read out: its stage is free
-      asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-      if (i > 0) mbar_arrive(empty0 + 8 * ((i - 1) % stages));
+      if (n > 0) {   // the last MMAs are done before their tensor memory goes
+        const uint64_t t0 = gtimer();
+        while (!mbar_try_wait_sleep(acc_full0 + 8 * ((n - 1) & 1), (uint32_t)(((n - 1) / 2) & 1)) && gtimer() - t0 < kWaitNs) {
+        }
+      }
     }
-    __syncwarp();
+  } else if (warp > EWARPS + 1) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // t of the shrink kernel
+    const int r = tid - (EWARPS + 2) * 32;
+    int i = 0, v = -1;
+    for (Walk w(p, ch, c0); c0 + i < c1; ++i, w.next(p, ch)) {
+      if (!w.fresh) continue;
+      ++v;
+      const int buf = v % abufs;
+      const int4 tile = p.tiles[w.tl];
+      Version ver;
+      ver.rank = tile.x < 0 ? 0 : p.ranks[tile.x * p.parts + w.part];
+      ver.scale = tile.x < 0 ? 0.f : p.scales[tile.x * p.parts + w.part];
+      ver.row0 = p.order[tile.y];
+      ver.rows = tile.z;
+      if (v >= abufs && !waitw(t_free0 + 8 * buf, (uint32_t)((v / abufs - 1) & 1), ab)) break;
+      if (ver.rank > 0)
+        row_scale[buf][r] = ver.scale * stage_t<T>(p.t + (int64_t)(tile.y + r) * p.SR + w.part * p.R, r < tile.z, p.R, r,
+                                                   a_op + buf * 512 * p.R);
+      if (r == 0) versions[buf] = ver;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(t_ready0 + 8 * buf);
+    }
+  } else {
+    // before the first store, so that this grid never ends before the one that still reads x
+    // and writes the workspace
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int quad = warp & 3, half = warp >> 2, r = quad * 32 + lane;
+    int i = 0, n = 0, v = -1;
+    Version ver{};
+    float s1 = 0.f;
+    for (Walk w(p, ch, c0); c0 + i < c1; ++i, w.next(p, ch)) {
+      const int s = i % stages, a = n & 1;
+      if (w.fresh) {
+        ++v;
+        const int buf = v % abufs;
+        if (!waitw(t_ready0 + 8 * buf, (uint32_t)((v / abufs) & 1), ab)) break;
+        ver = versions[buf];
+        s1 = row_scale[buf][r];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(t_free0 + 8 * buf);
+      }
+      const bool act = ver.rank > 0;
+      if (!waitw(full0 + 8 * s, (uint32_t)((i / stages) & 1), ab)) break;
+      uint8_t* const yrow = sm + s * sbytes + half * YBOX + r * 128;
+      const int left = w.left - half * 64;   // columns of this half
+      const bool tma_out = ver.rows >= quad * EROWS + EROWS && left >= 64;
+      if (act) {
+        if (!waitw(acc_full0 + 8 * a, (uint32_t)((n / 2) & 1), ab)) break;
+        tc_fence_after();
+        ++n;
+      }
+#pragma unroll
+      for (int hc = 0; hc < 2; ++hc) {
+        float x[32];
+        if (act) tld32(tmem + ((uint32_t)(quad * 32) << 16) + a * EC + half * 64 + hc * 32, x);
+        if (hc == 1 && act) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty0 + 8 * a);
+        }
+        if (!act && tma_out) continue;   // stored as it came
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint4* at = reinterpret_cast<uint4*>(yrow + (((hc * 4 + q) ^ (r & 7)) << 4));
+          uint4 o = *at;
+          if (act) {
+            T* oe = reinterpret_cast<T*>(&o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) oe[e] = from_f<T>(fmaf(s1, x[q * 8 + e], to_f(oe[e])));
+          }
+          if (tma_out) {
+            *at = o;
+          } else if (r < ver.rows && hc * 32 + q * 8 < left) {   // neither rows of the next sequence nor columns of the next part
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)(ver.row0 + r) * p.os + w.col + half * 64 + hc * 32 +
+                                      q * 8) = o;
+          }
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        if (tma_out) {
+          asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&mo),
+                       "r"(w.col + half * 64), "r"(ver.row0 + r),
+                       "r"(base + s * sbytes + half * YBOX + quad * EROWS * 128)
+                       : "memory");
+        }
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        // the chunk before this one is read out: its stage is free
+        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        if (i > 0) mbar_arrive(empty0 + 8 * ((i - 1) % stages));
+      }
+      __syncwarp();
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
-  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == EWARPS + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 2 * EC);
+  }
 }
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -366,7 +521,7 @@ static EncodeTiledFn encode_tiled() {
 
 // Rows of `cols` 16-bit values, `stride` apart, in boxes of box_cols x box_rows.
 static int rows_map(CUtensorMap* m, const void* ptr, int dtype, int64_t rows, int64_t stride, int64_t cols, int box_cols,
-                    int box_rows, bool swizzle) {
+                    int box_rows, CUtensorMapSwizzle swizzle) {
   const EncodeTiledFn enc = encode_tiled();
   if (!enc) {
     set_error("cuTensorMapEncodeTiled is not available from the driver");
@@ -377,8 +532,7 @@ static int rows_map(CUtensorMap* m, const void* ptr, int dtype, int64_t rows, in
   const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
   const CUresult r = enc(m, dtype == SPX_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                          const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled(adapter rows): error %d", (int)r);
     return SPX_ERR_CUDA;
@@ -388,11 +542,11 @@ static int rows_map(CUtensorMap* m, const void* ptr, int dtype, int64_t rows, in
 
 int shrink_block_launch(const Params& p, int dtype, int tiles, cudaStream_t st) {
   Cfg c;
-  c.groups = (p.SR + 127) / 128;
+  c.groups = (p.SR + 255) / 256;
   c.nb = ((p.SR + c.groups - 1) / c.groups + 15) / 16 * 16;
   const int sbytes = XBYTES + c.nb * KB * 2;
-  c.stages = 110 * 1024 / sbytes;          // two CTAs an SM
-  if (c.stages > 8) c.stages = 8;
+  c.stages = 110 * 1024 / sbytes;          // two CTAs an SM: 2 (256 columns) to 6
+  if (c.stages > MAXSTAGES) c.stages = MAXSTAGES;
   // the cluster's CTAs split k until the grid fills the SMs, with at least four steps each
   c.cs = 1;
   while (c.cs < 8 && (int64_t)tiles * c.groups * c.cs * 2 <= 2 * 148 && p.K >= 4 * KB * 2 * c.cs) c.cs *= 2;
@@ -400,15 +554,15 @@ int shrink_block_launch(const Params& p, int dtype, int tiles, cudaStream_t st) 
   c.smem = (size_t)c.stages * sbytes;
   c.smem = (c.smem > sums ? c.smem : sums) + 1024;
   CUtensorMap mx, ma;
-  int rc = rows_map(&mx, p.x, dtype, p.rows, p.xs, p.K, KB, M, true);
-  if (rc == SPX_OK) rc = rows_map(&ma, p.a, dtype, (int64_t)p.slots * p.SR, p.K, p.K, KB, c.nb, true);
+  int rc = rows_map(&mx, p.x, dtype, p.rows, p.xs, p.K, KB, M, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == SPX_OK) rc = rows_map(&ma, p.a, dtype, (int64_t)p.slots * p.SR, p.K, p.K, KB, c.nb, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != SPX_OK) return rc;
   const uint32_t fmt = dtype == SPX_F16 ? 0u : 1u;
   const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(c.nb >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
   cudaError_t e = cudaFuncSetAttribute(shrink_block_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)c.smem);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles * c.cs), (unsigned)c.groups);
+    cfg.gridDim = dim3((unsigned)(tiles * c.groups * c.cs));
     cfg.blockDim = dim3(128);
     cfg.dynamicSmemBytes = c.smem;
     cfg.stream = st;
@@ -417,7 +571,7 @@ int shrink_block_launch(const Params& p, int dtype, int tiles, cudaStream_t st) 
     at[0].val.clusterDim.x = (unsigned)c.cs, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, shrink_block_kernel, mx, ma, p, c.nb, c.stages, idesc);
+    e = cudaLaunchKernelEx(&cfg, shrink_block_kernel, mx, ma, p, c.nb, c.groups, c.stages, idesc);
   }
   if (e != cudaSuccess) {
     set_error("lora shrink_block_kernel: %s", cudaGetErrorString(e));
@@ -426,26 +580,33 @@ int shrink_block_launch(const Params& p, int dtype, int tiles, cudaStream_t st) 
   return launch_status("lora shrink_block_kernel");
 }
 
-template <typename T, int KS>
+template <typename T>
 static int launch_expand_block(const Params& p, int dtype, int tiles, cudaStream_t st) {
   Chunks ch{};
   for (int s = 0; s < p.parts; ++s) ch.first[s + 1] = ch.first[s] + (p.width[s] + EC - 1) / EC;
   ch.per_tile = ch.first[p.parts];
+  ch.kw = p.R % 64 == 0 ? 64 : p.R % 32 == 0 ? 32 : 16;
   SPX_REQUIRE((int64_t)tiles * ch.per_tile <= 0x3fffffff, SPX_ERR_SHAPE, "spx_lora_add: too many rows");
   ch.total = tiles * ch.per_tile;
-  const int sbytes = YBYTES + (EC * p.R * 2 + 1023) / 1024 * 1024;
-  int stages = 108 * 1024 / sbytes;          // two CTAs an SM
-  if (stages > 8) stages = 8;
-  const size_t smem = (size_t)stages * sbytes + 1024;
+  const int abufs = p.R <= 64 ? 2 : 1, sbytes = YBYTES + EC * p.R * 2, abytes = abufs * 2 * M * p.R * 2;
+  int stages = (220 * 1024 - abytes) / sbytes;   // 2 (rank 128) to 5 (rank 16)
+  if (stages > MAXSTAGES) stages = MAXSTAGES;
+  const size_t smem = (size_t)stages * sbytes + abytes + 1024;
   CUtensorMap my, mb, mo;
-  int rc = rows_map(&my, p.y, dtype, p.rows, p.ys, p.OUT, EC, M, true);
-  if (rc == SPX_OK) rc = rows_map(&mb, p.b, dtype, (int64_t)p.slots * p.OUT, p.R, p.R, p.R, EC, false);
-  if (rc == SPX_OK) rc = rows_map(&mo, p.out, dtype, p.rows, p.os, p.OUT, EC, EROWS, true);
+  int rc = rows_map(&my, p.y, dtype, p.rows, p.ys, p.OUT, 64, M, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc == SPX_OK)
+    rc = rows_map(&mb, p.b, dtype, (int64_t)p.slots * p.OUT, p.R, p.R, ch.kw, EC,
+                  ch.kw == 64   ? CU_TENSOR_MAP_SWIZZLE_128B
+                  : ch.kw == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                : CU_TENSOR_MAP_SWIZZLE_32B);
+  if (rc == SPX_OK) rc = rows_map(&mo, p.out, dtype, p.rows, p.os, p.OUT, 64, EROWS, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != SPX_OK) return rc;
-  const int most = 2 * num_sms();
+  const uint32_t fmt = dtype == SPX_F16 ? 0u : 1u;
+  const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(EC >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+  const int most = num_sms();
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(ch.total < most ? ch.total : most));
-  cfg.blockDim = dim3(160);
+  cfg.blockDim = dim3(ETHREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -453,8 +614,8 @@ static int launch_expand_block(const Params& p, int dtype, int tiles, cudaStream
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaFuncSetAttribute(expand_block_kernel<T, KS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, expand_block_kernel<T, KS>, my, mb, mo, p, ch, stages);
+  cudaError_t e = cudaFuncSetAttribute(expand_block_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, expand_block_kernel<T>, my, mb, mo, p, ch, stages, abufs, idesc);
   if (e != cudaSuccess) {
     set_error("lora expand_block_kernel: %s", cudaGetErrorString(e));
     return SPX_ERR_CUDA;
@@ -462,19 +623,9 @@ static int launch_expand_block(const Params& p, int dtype, int tiles, cudaStream
   return launch_status("lora expand_block_kernel");
 }
 
-template <typename T>
-static int expand_block_as(const Params& p, int dtype, int tiles, cudaStream_t st) {
-  switch (p.R / 16) {
-    case 1: return launch_expand_block<T, 1>(p, dtype, tiles, st);
-    case 2: return launch_expand_block<T, 2>(p, dtype, tiles, st);
-    case 3:
-    case 4: return launch_expand_block<T, 4>(p, dtype, tiles, st);
-    default: return launch_expand_block<T, 8>(p, dtype, tiles, st);
-  }
-}
-
 int expand_block_launch(const Params& p, int dtype, int tiles, cudaStream_t st) {
-  return dtype == SPX_F16 ? expand_block_as<__half>(p, dtype, tiles, st) : expand_block_as<__nv_bfloat16>(p, dtype, tiles, st);
+  return dtype == SPX_F16 ? launch_expand_block<__half>(p, dtype, tiles, st)
+                          : launch_expand_block<__nv_bfloat16>(p, dtype, tiles, st);
 }
 
 }  // namespace lora

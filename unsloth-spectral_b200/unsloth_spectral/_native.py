@@ -254,7 +254,7 @@ def launch_packed(what: str, index: int, args: bytes):
         fn = load()[what]                     # a binding of its own: bytes for the struct pointer
         fn.restype, fn.argtypes = C.c_int, [C.c_char_p, C.c_void_p]
         _packed[what] = fn
-    if index not in _device_ok or _device_ok[index] != SPX_OK:
+    if _device_ok.get(index) != SPX_OK:
         lib_for(torch.device("cuda", index))
     if index == torch.cuda.current_device():
         rc = fn(args, _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream)

@@ -35,27 +35,27 @@ class LoraBatch:
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        self._plans: Dict[int, tuple] = {}
+        self._plans: Dict[Tuple[int, bool], tuple] = {}
 
     def __len__(self) -> int:
         return len(self.slots)
 
     def prepare(self, tokens: int = 1) -> "LoraBatch":
         """Group the rows of ``tokens`` tokens per sequence now."""
-        self._plan(tokens)
+        for blocks in (False, True)[:1 + (tokens >= 64)]:
+            self._plan(tokens, blocks)
         return self
 
     @staticmethod
-    def tiles_of(slots: Sequence[int], tokens: int):
+    def tiles_of(slots: Sequence[int], tokens: int, blocks: bool = False):
         """Host lists ``(tile_rows, tiles, order)``: rows sorted by slot, cut into tiles of one
-        slot.  Prompts: tiles of up to 128 tokens of one sequence (the kernel on the 5th
-        generation's tensor cores).  Few tokens: 16 rows of any sequences, or 32 where a slot
-        has more, which reads the adapter's weights half as often."""
+        slot: 16 rows of any sequences, or 32 where a slot has more, which reads the adapter's
+        weights half as often; or ``blocks`` of up to 128 tokens of one sequence."""
         groups: Dict[int, list] = {}
         for i, s in enumerate(slots):
             groups.setdefault(s, []).append(i)
         most = max((len(g) for g in groups.values()), default=0) * tokens
-        rows = 128 if tokens >= 64 else 16 if most <= 16 else 32
+        rows = 128 if blocks else 16 if most <= 16 else 32
         order = torch.empty(len(slots) * tokens, dtype=torch.int32)
         tiles, at = [], 0
         for s in sorted(groups):
@@ -70,15 +70,15 @@ class LoraBatch:
             at += n
         return rows, tiles, order
 
-    def _plan(self, tokens: int):
-        p = self._plans.get(tokens)
+    def _plan(self, tokens: int, blocks: bool):
+        p = self._plans.get((tokens, blocks))
         if p is None:
             if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError(f"call LoraBatch.prepare({tokens}) before capturing a graph that uses the batch")
-            rows, tiles, order = self.tiles_of(self.slots, tokens)
+            rows, tiles, order = self.tiles_of(self.slots, tokens, blocks)
             t = torch.tensor(tiles, dtype=torch.int32).reshape(-1, 4)
             p = (rows, len(tiles), len(order), t.to(self.device), order.to(self.device))
-            self._plans[tokens] = p
+            self._plans[tokens, blocks] = p
         return p
 
 
@@ -169,7 +169,11 @@ class LoraPool:
             N.lib_for(self.device)
         if tokens == 0 or not batch.slots:
             return out
-        rows, n_tiles, n, tiles, order = batch._plan(tokens)
+        # Prompts take the kernels for blocks of adjacent rows: 8 x 4096 tokens on q|k|v at rank 16
+        # 209 us against 410; below about 8M values of x and y their longer start shows
+        # (5 x 77 tokens on 4096 -> 14336 22 us against 14)
+        blocks = tokens >= 64 and len(batch.slots) * tokens * (self.in_features + self.out_features) >= 1 << 23
+        rows, n_tiles, n, tiles, order = batch._plan(tokens, blocks)
         # the inner products, a buffer of each call's own: two streams or two captured graphs
         # never share one (the caching allocator hands it out in stream order)
         size = n * len(self.widths) * self._rank + 4
