@@ -5,6 +5,12 @@
 // norm's output never exists in the row type, so nothing is lost between it and the
 // rotation).  Bound by memory: each value is read once and written once; the tables' rows
 // come from L2 and are held in registers over the heads of a token.
+// What it takes is warps: 8 x 4096 tokens of 32/8 heads of 128 bf16 take 116 us (floor 103)
+// with 32 warps an SM and the next vector fetched ahead; 155 with four vectors at once and 16
+// warps, 126 without fetching ahead; narrower lanes (four values of a half) 150; more warps
+// than the registers allow without spills 150 to 230.
+#include <type_traits>
+
 #include "spx_common.cuh"
 
 namespace spx {
@@ -21,7 +27,7 @@ struct Params {
   int64_t rows;
   int T, Hq, H, D, len, rotk;
   float eps;
-  int wpr;   // warps that share the heads of one token row
+  int slots;   // groups of lanes that share the heads of one token row
 };
 
 __device__ __forceinline__ int64_t position(const Params& p, int64_t b, int64_t t) {
@@ -29,102 +35,110 @@ __device__ __forceinline__ int64_t position(const Params& p, int64_t b, int64_t 
   return v < 0 ? 0 : (v >= p.len ? p.len - 1 : v);
 }
 
-// Eight consecutive values of the row type, as loaded.
-template <typename T>
+// N consecutive values of a type, moved in words of up to 16 bytes.
+template <typename T, int N>
 struct Raw {
-  uint4 v[sizeof(T) / 2];
+  static constexpr int BYTES = N * (int)sizeof(T), WORD = BYTES < 16 ? BYTES : 16;
+  using W = typename std::conditional<WORD == 16, uint4, uint2>::type;
+  W v[BYTES / WORD];
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+    for (int i = 0; i < BYTES / WORD; ++i) v[i] = reinterpret_cast<const W*>(p)[i];
   }
   __device__ __forceinline__ float get(int e) const { return to_f(reinterpret_cast<const T*>(v)[e]); }
   __device__ __forceinline__ void set(int e, float f) { reinterpret_cast<T*>(v)[e] = from_f<T>(f); }
   __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
+    for (int i = 0; i < BYTES / WORD; ++i) reinterpret_cast<W*>(p)[i] = v[i];
   }
 };
 
-// G lanes hold one head vector: lane l its values 8l..8l+7 of both halves, so that the two
-// values of a rotation meet in one lane and only the sum of squares crosses lanes.
-template <typename T, int G, int U>
-__device__ __forceinline__ void heads(const T* src, T* dst, int64_t dst_h, const T* w, int j, int n, int step, int l,
-                                      bool on, int h, const float (&c)[8], const float (&s)[8], float eps) {
+// G lanes hold one head vector: lane l its values Nl..Nl+N-1 of both halves, so that the two
+// values of a rotation meet in one lane and only the sum of squares crosses lanes.  The
+// table row is held in registers over the heads of a token; the weights are read from shared
+// memory for each, which leaves registers for more warps.
+template <typename T, int N, int G>
+__device__ __forceinline__ void heads(const T* src, T* dst, int64_t dst_h, const T* w, const float (&c)[N],
+                                      const float (&s)[N], bool turn, int j, int n, int step, bool on, int h, float eps,
+                                      Raw<T, N>& a, Raw<T, N>& b, bool loaded) {
   if (j >= n) return;   // uniform over the G lanes; the shuffles below name them alone
   const unsigned mask = G == 32 ? 0xffffffffu : ((1u << (G & 31)) - 1u) << ((threadIdx.x & 31) / G * G);
-  float w1[8], w2[8];
-  {
-    Raw<T> a, b;
-    if (on) a.load(w + 8 * l), b.load(w + h + 8 * l);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w1[e] = on ? a.get(e) : 0.f, w2[e] = on ? b.get(e) : 0.f;
-  }
+  src += (int64_t)j * (2 * h);
+  dst += j * dst_h;
+  Raw<T, N> na, nb;
+  if (on && !loaded) a.load(src), b.load(src + h);
   const float inv_d = 1.f / (float)(2 * h);
-  for (; j < n; j += U * step) {
-    Raw<T> a[U], b[U];
+  while (true) {
+    const bool more = j + step < n;
+    src += step * 2 * h;
+    if (on && more) na.load(src), nb.load(src + h);
+    float ss = 0.f;
+    if (on) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (on && j + u * step < n) {
-        const T* p = src + (int64_t)(j + u * step) * (2 * h) + 8 * l;
-        a[u].load(p), b[u].load(p + h);
-      }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int ju = j + u * step;
-      if (ju >= n) break;
-      float ss = 0.f;
-      if (on) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x1 = a[u].get(e), x2 = b[u].get(e);
-          ss = fmaf(x1, x1, ss);
-          ss = fmaf(x2, x2, ss);
-        }
-      }
-#pragma unroll
-      for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-      const float inv = rsqrtf(fmaf(ss, inv_d, eps));
-      if (on) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y1 = a[u].get(e) * inv * w1[e], y2 = b[u].get(e) * inv * w2[e];
-          a[u].set(e, y1 * c[e] - y2 * s[e]);
-          b[u].set(e, y2 * c[e] + y1 * s[e]);
-        }
-        T* o = dst + (int64_t)ju * dst_h + 8 * l;
-        a[u].store(o), b[u].store(o + h);
+      for (int e = 0; e < N; ++e) {
+        const float x1 = a.get(e), x2 = b.get(e);
+        ss = fmaf(x1, x1, ss);
+        ss = fmaf(x2, x2, ss);
       }
     }
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+    const float inv = rsqrtf(fmaf(ss, inv_d, eps));
+    if (on) {
+      Raw<T, N> wa, wb;
+      wa.load(w), wb.load(w + h);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float y1 = a.get(e) * inv * wa.get(e), y2 = b.get(e) * inv * wb.get(e);
+        a.set(e, turn ? y1 * c[e] - y2 * s[e] : y1);
+        b.set(e, turn ? y2 * c[e] + y1 * s[e] : y2);
+      }
+      a.store(dst), b.store(dst + h);
+    }
+    if (!more) break;
+    j += step, dst += step * dst_h;
+    a = na, b = nb;
   }
 }
 
-template <typename T, int G, int U>
-__global__ void __launch_bounds__(WARPS * 32) vec_kernel(const Params p) {
+template <typename T, int N, int G>
+__global__ void __launch_bounds__(WARPS * 32, sizeof(T) == 4 ? 3 : 4) vec_kernel(const Params p) {
   constexpr int NG = 32 / G;
+  __shared__ __align__(16) T weights[2][2 * N * G];
   const int lane = threadIdx.x & 31, l = lane % G, h = p.D / 2;
-  const int64_t wid = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-  const int64_t row = wid / p.wpr;
-  if (row >= p.rows) return;
-  const int64_t b = row / p.T, t = row - b * p.T;
-  const int g = (int)(wid - row * p.wpr) * NG + lane / G, step = p.wpr * NG;
-  const bool on = 8 * l < h;
-  float c[8], s[8];
-  const int64_t at = position(p, b, t) * p.D + 8 * l;
-  Raw<float> cr, sr;
-  if (on) cr.load(p.cosT + at), sr.load(p.sinT + at);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) c[e] = on ? cr.get(e) : 1.f, s[e] = on ? sr.get(e) : 0.f;
-  const int64_t plane = (int64_t)p.T * p.D;
-  heads<T, G, U>(static_cast<const T*>(p.q) + b * p.qsb + t * p.qst, static_cast<T*>(p.qo) + b * p.Hq * plane + t * p.D,
-                 plane, static_cast<const T*>(p.qw), g, p.Hq, step, l, on, h, c, s, p.eps);
-  if (!p.rotk) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = 1.f, s[e] = 0.f;
+  const int64_t gi = ((int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5)) * NG + lane / G;
+  const bool live = gi < p.rows * p.slots;
+  const int64_t row = live ? gi / p.slots : 0, b = row / p.T, t = row - b * p.T;
+  const int g = (int)(gi - row * p.slots), step = p.slots;
+  const bool on = live && N * l < h;
+  const T* q = static_cast<const T*>(p.q) + b * p.qsb + t * p.qst + N * l;
+  const T* k = static_cast<const T*>(p.k) + b * p.ksb + t * p.kst + N * l;
+  // the group's first vector is on its way before its position and table row are looked up
+  Raw<T, N> xa, xb;
+  if (on) {
+    const T* x = g < p.Hq ? q + (int64_t)g * p.D : k + (int64_t)(g - p.Hq) * p.D;
+    xa.load(x), xb.load(x + h);
   }
+  const int64_t at = position(p, b, t) * p.D + N * l, plane = (int64_t)p.T * p.D;
+  for (int i = threadIdx.x; i < p.D; i += WARPS * 32) {
+    weights[0][i] = static_cast<const T*>(p.qw)[i];
+    if (p.H) weights[1][i] = static_cast<const T*>(p.kw)[i];
+  }
+  float c[N], s[N];
+  {
+    Raw<float, N> cr, sr;
+    if (on) cr.load(p.cosT + at), sr.load(p.sinT + at);
+#pragma unroll
+    for (int e = 0; e < N; ++e) c[e] = on ? cr.get(e) : 1.f, s[e] = on ? sr.get(e) : 0.f;
+  }
+  __syncthreads();
+  if (!live) return;
+  heads<T, N, G>(q, static_cast<T*>(p.qo) + b * p.Hq * plane + t * p.D + N * l, plane, weights[0] + N * l, c, s, true,
+                        g, p.Hq, step, on, h, p.eps, xa, xb, true);
   // the group after the last one of the queries takes the first key head
   const int first = (g - p.Hq % step + step) % step;
-  heads<T, G, U>(static_cast<const T*>(p.k) + b * p.ksb + t * p.kst, static_cast<T*>(p.ko) + b * p.kob + t * p.D, p.koh,
-                 static_cast<const T*>(p.kw), first, p.H, step, l, on, h, c, s, p.eps);
+  heads<T, N, G>(k, static_cast<T*>(p.ko) + b * p.kob + t * p.D + N * l, p.koh, weights[1] + N * l, c, s,
+                        p.rotk != 0, first, p.H, step, on, h, p.eps, xa, xb, g >= p.Hq);
 }
 
 // Any even head dim, any alignment: one warp per head vector, read twice (the second time
@@ -170,25 +184,25 @@ int launch(const Params& p, bool vec, cudaStream_t st) {
     any_kernel<T><<<(unsigned)((warps + WARPS - 1) / WARPS), WARPS * 32, 0, st>>>(p);
     return launch_status("qk_norm any_kernel");
   }
+  constexpr int VP = 8;
   int G = 1;
-  while (8 * G < h) G *= 2;
+  while (VP * G < h) G *= 2;
   Params q = p;
-  // Few rows: the heads of a row are spread over several warps, until the grid has about
-  // 16 warps for each SM or every group of lanes has one head.
-  const int ng = 32 / G, most = (p.Hq + p.H + ng - 1) / ng;
-  const int64_t want = (148 * 16 + p.rows - 1) / p.rows;
-  q.wpr = (int)(want < most ? want : most);
-  warps = p.rows * q.wpr;
+  // Few rows: the heads of a row are spread over several groups of lanes, until the grid has
+  // about 16 warps for each SM or every group has one head.
+  const int ng = 32 / G, most = p.Hq + p.H;
+  const int64_t want = ((int64_t)148 * 16 * ng + p.rows - 1) / p.rows;
+  q.slots = (int)(want < most ? want : most);
+  warps = (p.rows * q.slots + ng - 1) / ng;
   SPX_REQUIRE((warps + WARPS - 1) / WARPS <= 0x7fffffff, SPX_ERR_SHAPE, "spx_qk_norm_rope: too many rows");
   const unsigned grid = (unsigned)((warps + WARPS - 1) / WARPS);
-  constexpr int U = sizeof(T) == 4 ? 2 : 4;
   switch (G) {
-    case 1: vec_kernel<T, 1, U><<<grid, WARPS * 32, 0, st>>>(q); break;
-    case 2: vec_kernel<T, 2, U><<<grid, WARPS * 32, 0, st>>>(q); break;
-    case 4: vec_kernel<T, 4, U><<<grid, WARPS * 32, 0, st>>>(q); break;
-    case 8: vec_kernel<T, 8, U><<<grid, WARPS * 32, 0, st>>>(q); break;
-    case 16: vec_kernel<T, 16, U><<<grid, WARPS * 32, 0, st>>>(q); break;
-    default: vec_kernel<T, 32, U><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 1: vec_kernel<T, VP, 1><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 2: vec_kernel<T, VP, 2><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 4: vec_kernel<T, VP, 4><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 8: vec_kernel<T, VP, 8><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 16: vec_kernel<T, VP, 16><<<grid, WARPS * 32, 0, st>>>(q); break;
+    default: vec_kernel<T, VP, 32><<<grid, WARPS * 32, 0, st>>>(q); break;
   }
   return launch_status("qk_norm vec_kernel");
 }
@@ -223,7 +237,7 @@ int spx_qk_norm_rope(const spx_qk_norm_args* a, void* stream) {
   p.kob = a->k_out_stride_b, p.koh = a->k_out_stride_h;
   p.rows = (int64_t)a->batch * a->tokens;
   p.T = a->tokens, p.Hq = a->num_q_heads, p.H = a->num_kv_heads, p.D = a->head_dim, p.len = a->rope_len;
-  p.rotk = a->rotate_keys, p.eps = a->eps, p.wpr = 1;
+  p.rotk = a->rotate_keys, p.eps = a->eps;
   // 16-byte loads: both halves of a head start on 16 bytes and hold whole groups of eight
   const int per = 16 / dtype_size(a->dtype);
   const int64_t strides = a->q_stride_b | a->q_stride_t | (keys ? a->k_stride_b | a->k_stride_t | a->k_out_stride_b |
