@@ -7,7 +7,7 @@ Drop-in for the reference package's decode path: same public names
 ``TRITON_AVAILABLE`` / ``TRITON_VERSION`` and, when the library loads,
 ``spectral_attention_decode`` and ``TritonSpectralConfig``.
 Operators of the serving step beside them: ``qk_norm_rope`` (per-head query/key norms and
-rotation), ``LoraPool`` / ``LoraBatch`` (adapters of many requests), ``LogitsRules``
+rotation), ``LoraPool`` / ``LoraBatch`` / ``LoraAdapters`` (adapters of many requests), ``LogitsRules``
 (penalties, biases, allowed tokens, greedy choice).
 Set ``UNSLOTH_SPECTRAL_QUIET=1`` to silence the import banner.
 """
@@ -20,7 +20,7 @@ from .spectral_attention import (qk_norm_rope, spectral_attention_forward,  # no
                                  validate_spectral_attention)
 from .integration import get_cache_stats, patch_unsloth_attention  # noqa: E402
 from .kernels import TRITON_AVAILABLE, TRITON_VERSION  # noqa: E402
-from .adapters import LoraBatch, LoraPool  # noqa: E402
+from .adapters import LoraAdapters, LoraBatch, LoraPool  # noqa: E402
 from .logits import LogitsRules  # noqa: E402
 from .rsvd import batched_randomized_svd  # noqa: E402
 
@@ -35,6 +35,7 @@ __all__ = [
     "qk_norm_rope",
     "LoraPool",
     "LoraBatch",
+    "LoraAdapters",
     "LogitsRules",
     "TRITON_AVAILABLE",
     "TRITON_VERSION",

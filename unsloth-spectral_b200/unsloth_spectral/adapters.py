@@ -7,6 +7,7 @@ projection's output ``y = x W^T``::
 
     out[r] = y[r] + scale * B (A x[r])        A [rank, in], B [out, rank] of the row's slot
 
+``LoraAdapters`` holds the pools of a whole model whose attention is patched.
 One call serves every adapter of the batch (two launches of ``libspx``), for prompts and
 for single tokens.  A projection whose output is several weights side by side (a packed
 q|k|v projection) has several ``parts``, each with its own A and B.  float16 and bfloat16;
@@ -15,7 +16,7 @@ no gradients.
 from __future__ import annotations
 
 import math
-from typing import Dict, Sequence, Tuple, Union
+from typing import Dict, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -183,6 +184,100 @@ class LoraPool:
             _row_stride(y), _row_stride(out), *self._pool_ptrs, tiles.data_ptr(), order.data_ptr(), ws.data_ptr(),
             4 * size))
         return out
+
+
+def adapted(module, name: str, y: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+    """``y``, the output of projection ``name`` of ``module`` on ``x``, with the adapters of the batch
+    in use added in place when a ``LoraAdapters`` covers it."""
+    lora = getattr(module, "spx_lora", None)
+    if lora is None:
+        return y
+    owner, pools = lora
+    pool = pools.get(name)
+    if pool is None or owner.batch is None:
+        return y
+    if y.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("the adapters' products have no gradients: run the forward under torch.no_grad()")
+    return pool.add(y, x, owner.batch, out=y)
+
+
+class LoraAdapters:
+    """The adapters of a model: a ``LoraPool`` for every projection of its layers named in
+    ``targets``.  ``model`` is a ``SpectralLlama`` or any model that ``patch_unsloth_attention``
+    takes (of the latter the attention projections only: their MLPs run their own code)::
+
+        adapters = LoraAdapters(model, max_rank=16, slots=8)
+        adapters.load(0, {(layer, "q_proj"): (A, B), ...}, scale=alpha / rank)
+        model.generate(ids, 64, adapters=adapters, adapter_slots=[0, -1, 3, 0])
+
+    ``use(slots)`` names the slot of each sequence for the forwards that follow, ``use(None)``
+    switches the adapters off."""
+
+    ATTENTION = ("q_proj", "k_proj", "v_proj", "o_proj")
+    MLP = ("gate_proj", "up_proj", "down_proj")
+
+    def __init__(self, model, max_rank: int = 16, slots: int = 8, targets: Sequence[str] = ATTENTION + MLP):
+        unknown = set(targets) - set(self.ATTENTION + self.MLP)
+        if unknown:
+            raise ValueError(f"unknown projections {sorted(unknown)}; expected some of {self.ATTENTION + self.MLP}")
+        self.batch: Optional[LoraBatch] = None
+        self.slots, self.targets = slots, tuple(targets)
+        self._pools: Dict[Tuple[int, str], Tuple[LoraPool, int]] = {}
+        make = lambda w, out: LoraPool(w.shape[1], out, max_rank, slots, w.dtype, w.device)  # noqa: E731
+        layers = model.model.layers
+        for i, layer in enumerate(layers):
+            attn, mlp = layer.self_attn, layer.mlp
+            if set(targets) & set(self.MLP) and not hasattr(mlp, "spx_lora"):
+                raise ValueError(f"layer {i}: {type(mlp).__name__} takes no adapters; leave {self.MLP} out of targets")
+            held = {}
+            qkv = [n for n in self.ATTENTION[:3] if n in targets]
+            if qkv and getattr(attn, "spx_qkv_weight", None) is not None:
+                widths = [getattr(attn, n).weight.shape[0] for n in self.ATTENTION[:3]]
+                held["qkv"] = make(attn.spx_qkv_weight, widths)
+                for n in qkv:
+                    self._pools[i, n] = held["qkv"], self.ATTENTION.index(n)
+            else:
+                for n in qkv:
+                    held[n] = make(getattr(attn, n).weight, getattr(attn, n).weight.shape[0])
+                    self._pools[i, n] = held[n], 0
+            if "o_proj" in targets:
+                held["o_proj"] = make(attn.o_proj.weight, attn.o_proj.weight.shape[0])
+                self._pools[i, "o_proj"] = held["o_proj"], 0
+            attn.spx_lora = (self, held)
+            held = {}
+            for n in self.MLP:
+                if n in targets:
+                    held[n] = make(getattr(mlp, n).weight, getattr(mlp, n).weight.shape[0])
+                    self._pools[i, n] = held[n], 0
+            if held:
+                mlp.spx_lora = (self, held)
+        self.device = layers[0].self_attn.o_proj.weight.device
+
+    def load(self, slot: int, weights: Dict[Tuple[int, str], Tuple[torch.Tensor, torch.Tensor]], scale: float = 1.0):
+        """Put an adapter into a slot, in place of what it held: ``{(layer, projection): (A, B)}``
+        with ``A [rank, in]``, ``B [out, rank]``; projections left out keep the shared weight alone."""
+        for key in weights:
+            if key not in self._pools:
+                raise KeyError(f"no adapted projection {key}; targets are {self.targets}")
+        self.unload(slot)
+        for key, (A, B) in weights.items():
+            pool, part = self._pools[key]
+            pool.load(slot, A, B, scale, part)
+
+    def unload(self, slot: int):
+        """Empty a slot."""
+        for pool in {id(p): p for p, _ in self._pools.values()}.values():
+            pool.unload(slot)
+
+    def use(self, slots: Optional[Sequence[int]]):
+        """The slot of each sequence of the batch that the next forwards run (-1: none), or None."""
+        if slots is None:
+            self.batch = None
+            return
+        batch = LoraBatch(slots, self.device)
+        if batch.highest >= self.slots:
+            raise IndexError(f"slot {batch.highest} of {self.slots}")
+        self.batch = batch
 
 
 def _row_stride(t: torch.Tensor) -> int:

@@ -11,6 +11,10 @@ Mirrors unsloth_spectral/integration.py:43-938:
   CUDA library loads, as the reference routes to its kernels module.
 * ``patch_unsloth_attention`` / ``get_cache_stats`` -- same arguments and results.
 
+Beyond the reference: attention modules with ``q_norm`` / ``k_norm`` get their per-head norms
+and the rotation in one launch (``qk_norm_rope``; the reference's forwards leave the norms
+out), and modules that a ``LoraAdapters`` covers add each request's low-rank product.
+
 RoPE tables: the reference reads them from ``self.rotary_emb``; modules without one
 (current ``transformers``) get float32 tables built from ``config.rope_theta``.
 """
@@ -24,7 +28,8 @@ import torch
 import torch.nn.functional as F
 
 from . import _ops
-from .spectral_attention import apply_rope, spectral_attention_forward
+from .adapters import adapted
+from .spectral_attention import apply_rope, qk_norm_rope, spectral_attention_forward
 from .spectral_cache import SpectralCache
 
 logger = logging.getLogger("unsloth_spectral.integration")
@@ -101,10 +106,50 @@ def _qkv(self, hidden_states):
     other module runs its own ``q_proj`` / ``k_proj`` / ``v_proj`` as the reference does."""
     w = getattr(self, "spx_qkv_weight", None)
     if w is None:
-        return self.q_proj(hidden_states), self.k_proj(hidden_states), self.v_proj(hidden_states)
+        return tuple(adapted(self, name, getattr(self, name)(hidden_states), hidden_states)
+                     for name in ("q_proj", "k_proj", "v_proj"))
     nq, nk = self.q_proj.weight.shape[0], self.k_proj.weight.shape[0]
-    qkv = torch.nn.functional.linear(hidden_states, w)
+    qkv = adapted(self, "qkv", torch.nn.functional.linear(hidden_states, w), hidden_states)
     return qkv[..., :nq], qkv[..., nq:nq + nk], qkv[..., nq + nk:]
+
+
+def _head_norms(self, head_dim: int, like: torch.Tensor):
+    """``(q weight, k weight, eps)`` when module ``self`` normalises its query and key heads
+    the way ``qk_norm_rope`` does -- ``q_norm`` / ``k_norm`` of ``head_dim`` weights in the dtype of
+    ``like`` with the usual RMS norm (this package's, or one that names its epsilon
+    ``variance_epsilon``) -- else None."""
+    from .llama_loop import RMSNorm
+    found = []
+    for norm in (self.q_norm, self.k_norm):
+        w = getattr(norm, "weight", None)
+        eps = norm.eps if isinstance(norm, RMSNorm) else getattr(norm, "variance_epsilon", None)
+        if w is None or eps is None or w.shape != (head_dim,) or w.dtype != like.dtype or w.device != like.device:
+            return None
+        found.append((w, float(eps)))
+    (qw, eps), (kw, keps) = found
+    return (qw, kw, eps) if eps == keps else None
+
+
+def _own_norm(norm, x: torch.Tensor, heads: int, head_dim: int) -> torch.Tensor:
+    """A module's own norm on projection rows ``[B, T, heads * head_dim]``: of each head, or of
+    whole rows when its weight is that wide; ``[B, heads, T, head_dim]``."""
+    B, T, n = x.shape
+    w = getattr(norm, "weight", None)
+    y = norm(x) if w is not None and w.numel() == n and n != head_dim else norm(x.reshape(B, T, heads, head_dim))
+    return y.reshape(B, T, heads, head_dim).transpose(1, 2)
+
+
+def _normed_qk(self, qp, kp, nh: int, nkv: int, hd: int, cos, sin, positions):
+    """Queries and keys of an attention with ``q_norm`` / ``k_norm``: the queries normalised and
+    rotated, the keys normalised (the cache holds them before the rotation), head-major.
+    ``positions``: int64 ``[1 or B, T]``, or the first one as an int."""
+    norms = _head_norms(self, hd, qp) if qp.is_cuda else None
+    if norms is not None:
+        return qk_norm_rope(qp, kp, norms[0], norms[1], cos, sin, positions, eps=norms[2])
+    q, k = _own_norm(self.q_norm, qp, nh, hd), _own_norm(self.k_norm, kp, nkv, hd)
+    if not isinstance(positions, torch.Tensor):
+        positions = torch.arange(positions, positions + qp.shape[1], device=qp.device)[None]
+    return apply_rope(q.float(), cos[positions][:, None], sin[positions][:, None]).to(q.dtype), k
 
 
 def _mask_is_causal(mask: torch.Tensor, q_pos: torch.Tensor, k_pos: torch.Tensor) -> bool:
@@ -157,8 +202,7 @@ def create_spectral_forward(original_forward, block_size: int = 512, k_rank_keys
         nh, nkv, hd = _attn_dims(self)
         bsz, q_len, _ = hidden_states.size()
         qp, kp, vp = _qkv(self, hidden_states)
-        q = qp.view(bsz, q_len, nh, hd).transpose(1, 2)
-        k_pre = kp.view(bsz, q_len, nkv, hd).transpose(1, 2)
+        normed = getattr(self, "q_norm", None) is not None and getattr(self, "k_norm", None) is not None
         v = vp.view(bsz, q_len, nkv, hd).transpose(1, 2)
         if past_key_value is None:
             past_key_value = getattr(self, "_spectral_cache", None) if use_cache else None
@@ -175,8 +219,13 @@ def create_spectral_forward(original_forward, block_size: int = 512, k_rank_keys
         if position_ids is None:
             position_ids = torch.arange(past_key_value.total_tokens, kv_seq_len,
                                         device=hidden_states.device)[None]
-        cq, sq = cos[position_ids][:, None], sin[position_ids][:, None]
-        q = apply_rope(q.float(), cq, sq).to(q.dtype)
+        if normed:
+            q, k_pre = _normed_qk(self, qp, kp, nh, nkv, hd, cos, sin, position_ids)
+        else:
+            q = qp.view(bsz, q_len, nh, hd).transpose(1, 2)
+            k_pre = kp.view(bsz, q_len, nkv, hd).transpose(1, 2)
+            cq, sq = cos[position_ids][:, None], sin[position_ids][:, None]
+            q = apply_rope(q.float(), cq, sq).to(q.dtype)
         past_key_value.append(k_pre, v, position_ids)
         if use_spectral_attention and past_key_value.total_tokens > block_size and q_len == 1:
             out = spectral_attention_forward(q, past_key_value, cos, sin, kv_seq_len - 1, attention_mask,
@@ -184,7 +233,7 @@ def create_spectral_forward(original_forward, block_size: int = 512, k_rank_keys
         else:
             out = _dense_attention(q, past_key_value, cos, sin, nh // nkv, hd, attention_mask, q.dtype, position_ids)
         out = out.transpose(1, 2).reshape(bsz, q_len, nh * hd)
-        out = self.o_proj(out)
+        out = adapted(self, "o_proj", self.o_proj(out), out)
         if use_cache:
             self._spectral_cache = past_key_value
         return out, None, past_key_value if use_cache else None
@@ -208,6 +257,7 @@ def create_spectral_forward_inference(block_size: int = 512, k_rank_keys: int = 
         q = qp.view(bsz, 1, nh, hd).transpose(1, 2)
         k_pre = kp.view(bsz, 1, nkv, hd).transpose(1, 2)
         v = vp.view(bsz, 1, nkv, hd).transpose(1, 2)
+        normed = getattr(self, "q_norm", None) is not None and getattr(self, "k_norm", None) is not None
         if not isinstance(past_key_value, SpectralCache):
             past_key_value = SpectralCache(nkv, hd, block_size, k_rank_keys, k_rank_values, hot_buffer_size,
                                            device=hidden_states.device, dtype=hidden_states.dtype,
@@ -222,7 +272,9 @@ def create_spectral_forward_inference(block_size: int = 512, k_rank_keys: int = 
         pid = None
         if position_ids is not None:
             pid = position_ids.reshape(-1, position_ids.shape[-1])[:, -1:].to(hidden_states.device)
-        if (hidden_states.is_cuda and cos.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous()
+        if normed:
+            q, k_pre = _normed_qk(self, qp, kp, nh, nkv, hd, cos, sin, qpos if pid is None else pid.long())
+        elif (hidden_states.is_cuda and cos.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous()
                 and qp.stride(-1) == 1 and (pid is None or pid.shape[0] in (1, bsz))):
             # one launch (spx_rope_rows), the same float32 arithmetic as apply_rope below
             q = _ops.rope_rows(qp, nh, hd, cos, sin, pid, qpos)
@@ -241,8 +293,8 @@ def create_spectral_forward_inference(block_size: int = 512, k_rank_keys: int = 
         else:
             out = _dense_attention(q, past_key_value, cos, sin, nh // nkv, hd, attention_mask, q.dtype,
                                    torch.full((1,), qpos, dtype=torch.long, device=hidden_states.device))
-        out = self.o_proj(out.transpose(1, 2).reshape(bsz, 1, nh * hd))
-        return out, past_key_value
+        out = out.transpose(1, 2).reshape(bsz, 1, nh * hd)
+        return adapted(self, "o_proj", self.o_proj(out), out), past_key_value
 
     return spectral_forward_inference
 

@@ -30,13 +30,15 @@ from __future__ import annotations
 import math
 from dataclasses import dataclass, field
 from types import SimpleNamespace
-from typing import List, Optional
+from typing import List, Optional, Sequence
 
 import torch
 import torch.nn.functional as F
 
 from . import _ops
+from .adapters import LoraAdapters, adapted
 from .integration import patch_unsloth_attention, rope_tables_for
+from .logits import LogitsRules
 
 
 @dataclass
@@ -50,6 +52,7 @@ class LlamaShape:
     vocab: int = 32768
     rope_theta: float = 1e6
     eps: float = 1e-5
+    qk_norm: bool = False   # RMS norms of the query and key heads before the rotation
 
 
 MISTRAL_7B = LlamaShape()
@@ -109,6 +112,9 @@ class Attention(torch.nn.Module):
         self.k_proj = _linear_of(w[nq:nq + nk])
         self.v_proj = _linear_of(w[nq + nk:])
         self.register_buffer("spx_qkv_weight", w, persistent=False)
+        if s.qk_norm:
+            self.q_norm = RMSNorm(s.head_dim, s.eps, device, dtype)
+            self.k_norm = RMSNorm(s.head_dim, s.eps, device, dtype)
         self.o_proj = _linear(s.heads * s.head_dim, s.hidden, device, dtype, std, gen)
 
     def forward(self, *a, **k):  # pragma: no cover - replaced by the patch
@@ -116,6 +122,8 @@ class Attention(torch.nn.Module):
 
 
 class MLP(torch.nn.Module):
+    spx_lora = None   # set by LoraAdapters
+
     def __init__(self, s: LlamaShape, device, dtype, std, gen):
         super().__init__()
         self.gate_proj = _linear(s.hidden, s.ffn, device, dtype, std, gen)
@@ -123,7 +131,9 @@ class MLP(torch.nn.Module):
         self.down_proj = _linear(s.ffn, s.hidden, device, dtype, std, gen)
 
     def forward(self, x):
-        return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
+        h = (F.silu(adapted(self, "gate_proj", self.gate_proj(x), x))
+             * adapted(self, "up_proj", self.up_proj(x), x))
+        return adapted(self, "down_proj", self.down_proj(h), h)
 
 
 class DecoderLayer(torch.nn.Module):
@@ -195,29 +205,54 @@ class SpectralLlama(torch.nn.Module):
         return self.lm_head(x[:, -1])
 
     @torch.no_grad()
-    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, timer=None, cuda_graphs: bool = False):
+    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, timer=None, cuda_graphs: bool = False, *,
+                 rules: Optional[LogitsRules] = None, allow: Optional[torch.Tensor] = None,
+                 adapters: Optional[LoraAdapters] = None, adapter_slots: Optional[Sequence[int]] = None):
         """Greedy decoding: the prompt, then ``max_new_tokens`` tokens, each the argmax of
-        the previous step's logits.  Positions stay on the device (no host reads inside
+        the previous step's logits.  ``rules``: each token is the argmax under the batch's
+        ``LogitsRules`` (their history starts with this prompt) and ``allow``, the rules' bit mask
+        of allowed tokens.  ``adapters``, ``adapter_slots``: the requests' low-rank adapters, the
+        slot of each.  Positions stay on the device (no host reads inside
         the loop).  ``cuda_graphs``: replay the decode step from a CUDA graph between block
         compressions (``_decode_graphed``).  ``timer(name)``, if given, is called after
         the prefill ("prefill") and at the end ("decode").  Returns the new tokens
         ``[B, max_new_tokens]``."""
         B, T = input_ids.shape
+        if allow is not None and rules is None:
+            raise ValueError("allow is a mask of LogitsRules: give rules too")
+        if (adapters is None) != (adapter_slots is None):
+            raise ValueError("adapters and adapter_slots are given together")
+        if adapters is not None:
+            if len(adapter_slots) != B:
+                raise ValueError(f"{B} sequences, {len(adapter_slots)} adapter slots")
+            before = adapters.batch
+            adapters.use(adapter_slots)
+            adapters.batch.prepare(T).prepare(1)
+            try:
+                return self.generate(input_ids, max_new_tokens, timer, cuda_graphs, rules=rules, allow=allow)
+            finally:
+                adapters.batch = before
+        if rules is not None:
+            rules.reset()
+            rules.observe_prompt(input_ids)
+            choose = lambda logits: rules.pick(logits, allow, record=True)  # noqa: E731
+        else:
+            choose = lambda logits: logits.argmax(-1)  # noqa: E731
         logits, caches = self.prefill(input_ids)
         if timer is not None:
             timer("prefill")
         out = torch.empty(B, max_new_tokens, dtype=torch.long, device=input_ids.device)
-        tok = logits.argmax(-1)
+        tok = choose(logits)
         pos = torch.full((1, 1), T, dtype=torch.long, device=input_ids.device)
         if cuda_graphs:
-            self._decode_graphed(tok, pos, caches, out)
+            self._decode_graphed(tok, pos, caches, out, choose)
         else:
             for s in range(max_new_tokens):
                 out[:, s] = tok
                 if s + 1 == max_new_tokens:
                     break
                 logits = self.decode_step(tok, pos, caches)
-                tok = logits.argmax(-1)
+                tok = choose(logits)
                 pos += 1
         if timer is not None:
             timer("decode")
@@ -225,7 +260,7 @@ class SpectralLlama(torch.nn.Module):
         return out
 
     @torch.no_grad()
-    def _decode_graphed(self, tok: torch.Tensor, pos: torch.Tensor, caches: List, out: torch.Tensor):
+    def _decode_graphed(self, tok: torch.Tensor, pos: torch.Tensor, caches: List, out: torch.Tensor, choose):
         """The decode loop with the step captured in a CUDA graph.  One step's kernels
         depend on the host only through the cold-tier block count and the tensors'
         addresses; the hot tier grows through its device length (single-token appends
@@ -248,7 +283,7 @@ class SpectralLlama(torch.nn.Module):
                 # host argument: eager steps too
                 if t0.num_blocks == 0 or room < 3 or n - 1 - s < 3:
                     logits = self.decode_step(tok, pos, caches)
-                    tok.copy_(logits.argmax(-1))
+                    tok.copy_(choose(logits))
                     pos.add_(1)
                     s += 1
                     out[:, s] = tok
@@ -264,7 +299,7 @@ class SpectralLlama(torch.nn.Module):
                 for layer in self.model.layers:
                     rope_tables_for(layer.self_attn, caches[0].total_tokens + k + 2, dev)
                 logits = self.decode_step(tok, pos, caches)
-                tok.copy_(logits.argmax(-1))
+                tok.copy_(choose(logits))
                 pos.add_(1)
                 s += 1
                 out[:, s] = tok
@@ -273,7 +308,7 @@ class SpectralLlama(torch.nn.Module):
                 graph = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(graph, stream=stream):
                     g_logits = self.decode_step(tok, pos, caches)
-                    tok.copy_(g_logits.argmax(-1))
+                    tok.copy_(choose(g_logits))
                     pos.add_(1)
                 for r in range(k - 1):
                     if r:
