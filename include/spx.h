@@ -413,9 +413,8 @@ SPX_API int spx_qk_norm_rope(const spx_qk_norm_args* args, void* stream);
 #define SPX_LORA_MAX_RANK 128
 typedef struct spx_lora_args {
   int32_t num_tiles;           /* tiles of up to tile_rows rows of one slot */
-  int32_t tile_rows;           /* 16 or 32; or 128: the rows of a tile are then adjacent
-                                  (order[first + i] = order[first] + i) */
-  int32_t num_rows;            /* entries of order */
+  int32_t tile_rows;           /* 16 or 32; or 128: the rows of a tile are then adjacent */
+  int32_t num_rows;            /* rows of x, y and out */
   int32_t in_features;         /* multiple of 8 */
   int32_t parts;               /* 1..SPX_LORA_MAX_PARTS */
   int32_t part_width[SPX_LORA_MAX_PARTS];  /* columns of each part, multiples of 8; they are adjacent in y and out */
@@ -430,8 +429,9 @@ typedef struct spx_lora_args {
   const void* b;               /* [slots][sum of part_width][max_rank], zero past the slot's rank */
   const int32_t* ranks;        /* [slots][parts]: rank in use, 0 = nothing loaded */
   const float* scales;         /* [slots][parts] */
-  const int32_t* tiles;        /* [num_tiles][4]: slot (-1 none), first entry of order, rows, 0 */
-  const int32_t* order;        /* [num_rows]: row of x, y and out */
+  const int32_t* tiles;        /* [num_tiles][4]: slot (-1 none), first entry of order, rows, and
+                                  with tile_rows 128 the first row of x, y and out (else unused) */
+  const int32_t* order;        /* [num_rows]: row of x, y and out; not read with tile_rows 128 */
   float* workspace;            /* >= spx_lora_workspace_size(args) bytes: the inner products,
                                   f32 [num_rows][parts*max_rank], then an int32 that is set to 1
                                   when a kernel's wait expired (out is not valid then) */

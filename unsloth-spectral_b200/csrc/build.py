@@ -1,4 +1,6 @@
-"""Build libspx.so (the C-ABI CUDA library) in-tree for sm_100a.
+"""Build libspx.so (the C-ABI CUDA library) in-tree for sm_100a, and _spx_front.so (its
+tensor-level entry points for the calls of a decode step, spx_front.cpp, against the torch of
+this interpreter).
 
     python unsloth-spectral_b200/csrc/build.py [--jobs N] [--force]
 
@@ -20,6 +22,7 @@ PKG_ROOT = os.path.dirname(CSRC)
 REPO = os.path.dirname(PKG_ROOT)
 INCLUDE = os.path.join(REPO, "include")
 OUT = os.path.join(PKG_ROOT, "unsloth_spectral", "libspx.so")
+FRONT = os.path.join(PKG_ROOT, "unsloth_spectral", "_spx_front.so")
 BUILD = os.path.join(CSRC, "_build")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -75,7 +78,31 @@ def build(jobs: int = 0, force: bool = False, verbose: bool = False, ptxas_verbo
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
+    build_front(force)
     return OUT
+
+
+def build_front(force: bool = False) -> str:
+    src = os.path.join(CSRC, "spx_front.cpp")
+    if not force and not _stale(FRONT, [src, os.path.join(INCLUDE, "spx.h"), os.path.abspath(__file__)]):
+        return FRONT
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    inc = [INCLUDE, os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    libs = ["c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch", "torch_python"]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           "-DTORCH_EXTENSION_NAME=_spx_front", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *[f"-I{i}" for i in inc], src, "-o", FRONT, f"-L{os.path.join(root, 'lib')}", *[f"-l{n}" for n in libs],
+           f"-L{os.path.dirname(OUT)}", "-lspx", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("g++ failed for spx_front.cpp")
+    return FRONT
 
 
 if __name__ == "__main__":

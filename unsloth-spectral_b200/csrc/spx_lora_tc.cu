@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(128) shrink_block_kernel(const __grid_constant
   const int4 tile = p.tiles[unit / groups];
   if (tile.x < 0) return;   // rows without an adapter: the whole cluster leaves
   const int tid = threadIdx.x, warp = tid >> 5;
-  const int col0 = group * nb, row0 = p.order[tile.y];
+  const int col0 = group * nb, row0 = tile.w;
   const uint32_t base = (smem_u32(raw_smem) + 1023u) & ~1023u;
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * MAXSTAGES, done = empty0 + 8 * MAXSTAGES;
   const int sbytes = XBYTES + nb * KB * 2;
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
       int i = 0, row0 = 0;
       int4 tile = make_int4(0, 0, 0, 0);
       for (Walk w(p, ch, c0); c0 + i < c1; ++i, w.next(p, ch)) {
-        if (w.fresh) tile = p.tiles[w.tl], row0 = p.order[tile.y];
+        if (w.fresh) tile = p.tiles[w.tl], row0 = tile.w;
         const int s = i % stages;
         if (i >= stages && !wait1(empty0 + 8 * s, (uint32_t)((i / stages - 1) & 1), ab)) break;
         const uint32_t dst = base + s * sbytes, bar = full0 + 8 * s;
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
       Version ver;
       ver.rank = tile.x < 0 ? 0 : p.ranks[tile.x * p.parts + w.part];
       ver.scale = tile.x < 0 ? 0.f : p.scales[tile.x * p.parts + w.part];
-      ver.row0 = p.order[tile.y];
+      ver.row0 = tile.w;
       ver.rows = tile.z;
       if (v >= abufs && !waitw(t_free0 + 8 * buf, (uint32_t)((v / abufs - 1) & 1), ab)) break;
       if (ver.rank > 0)

@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-import struct
 
 import torch
 
@@ -125,13 +124,6 @@ class LogitsArgs(C.Structure):
             "bias_first", "bias_values", "allow")] + [("allow_stride", C.c_int64)]
 
 
-# The three structs above as `struct` formats, field by field: the entry points that a decode
-# step calls for every layer take them packed (bytes), which costs about 1 us a call where
-# filling a ctypes.Structure costs 6 to 8.
-QK_NORM_PACK = struct.Struct("@8ifi2P4q5P3q2P2q0q")
-LORA_PACK = struct.Struct("@5i4i3i3P3q7PN0q")
-LOGITS_PACK = struct.Struct("@4iPqPq11Pq0q")
-
 EXPORTS = {
     "spx_decode_workspace_size": (C.c_size_t, [C.POINTER(DecodeArgs)]),
     "spx_decode_attn": (C.c_int, [C.POINTER(DecodeArgs), C.c_void_p]),
@@ -241,28 +233,15 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-_packed = {}
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
-def launch_packed(what: str, index: int, args: bytes):
-    """Call the entry point ``what`` with its packed args struct on the current stream of CUDA
-    device ``index``, with that device current (a launch goes to the current device,
-    whatever device its pointers and stream belong to); raises unless it returns SPX_OK."""
-    fn = _packed.get(what)
-    if fn is None:
-        fn = load()[what]                     # a binding of its own: bytes for the struct pointer
-        fn.restype, fn.argtypes = C.c_int, [C.c_char_p, C.c_void_p]
-        _packed[what] = fn
-    if _device_ok.get(index) != SPX_OK:
-        lib_for(torch.device("cuda", index))
-    if index == torch.cuda.current_device():
-        rc = fn(args, _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(args, torch.cuda.current_stream(index).cuda_stream)
-    if rc != SPX_OK:
-        check(_lib, rc, what)
+def front():
+    """The module of tensor-level entry points (``csrc/spx_front.cpp``) over the library."""
+    load()
+    try:
+        from . import _spx_front
+    except ImportError as e:
+        raise SpxUnavailable(f"_spx_front.so is missing or does not fit this torch ({e}); build it with "
+                             f"`python unsloth-spectral_b200/csrc/build.py`") from e
+    return _spx_front
 
 
 def on_device(device: torch.device, fn, *args):

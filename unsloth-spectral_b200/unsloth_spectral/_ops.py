@@ -162,79 +162,17 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optiona
     return out if residual is None else (out, h)
 
 
+_qk_norm_rope = None
+
+
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, position_ids, eps: float, rotate_keys: bool):
-    """``spx_qk_norm_rope``; arguments and results as ``spectral_attention.qk_norm_rope``.
-    Runs for every layer of a decode step, so each property of a tensor is looked up once."""
-    dt, dev, qshape, wshape = q.dtype, q.get_device(), q.shape, q_weight.shape
-    code = N.dtype_code(dt)
-    if len(qshape) != 3 or len(wshape) != 1:
-        raise ValueError(f"q must be [B, T, H * D] and q_weight [D], got {tuple(qshape)} and {tuple(wshape)}")
-    B, T, n = qshape
-    D, = wshape
-    if D == 0 or D % 2 or n == 0 or n % D:
-        raise ValueError(f"{n} query columns are no whole heads of {D} (an even number)")
-    if not eps >= 0:
-        raise ValueError(f"eps must not be negative, got {eps}")
-    fits = q_weight.dtype == dt and q_weight.get_device() == dev
-    if k is not None:
-        if k_weight is None:
-            raise ValueError("k needs k_weight")
-        kshape = k.shape
-        if len(kshape) != 3 or kshape[0] != B or kshape[1] != T or k_weight.shape != wshape or kshape[2] % D:
-            raise ValueError(f"k {tuple(kshape)} / k_weight {tuple(k_weight.shape)} do not fit q {tuple(qshape)} "
-                             f"with heads of {D}")
-        H = kshape[2] // D
-        fits = (fits and k.dtype == dt and k_weight.dtype == dt and k.get_device() == dev
-                and k_weight.get_device() == dev)
-    if not fits:
-        raise ValueError(f"q, k and their weights must share dtype and device: q has {dt} on {q.device}")
-    if dev < 0:
-        N.lib_for(q.device)
-    if cos.dtype != torch.float32 or not cos.is_contiguous() or cos.get_device() != dev or cos.dim() != 2:
-        cos = rope_table_f32(cos, q.device)
-    if sin.dtype != torch.float32 or not sin.is_contiguous() or sin.get_device() != dev or sin.dim() != 2:
-        sin = rope_table_f32(sin, q.device)
-    tshape = cos.shape
-    if sin.shape != tshape or tshape[1] != D or tshape[0] == 0:
-        raise ValueError(f"cos/sin must be [len, {D}] tables, got {tuple(tshape)} and {tuple(sin.shape)}")
-    pos_ptr = psb = pst = start = 0
+    """``spx_qk_norm_rope``; arguments and results as ``spectral_attention.qk_norm_rope``."""
+    global _qk_norm_rope
+    if _qk_norm_rope is None:
+        _qk_norm_rope = N.front().qk_norm_rope
     if isinstance(position_ids, torch.Tensor):
-        pshape, pstride = position_ids.shape, position_ids.stride()
-        if len(pshape) == 1:
-            pshape, pstride = (1, *pshape), (0, *pstride)
-        if len(pshape) != 2 or pshape[1] != T or (pshape[0] != 1 and pshape[0] != B) \
-                or position_ids.dtype != torch.int64 or position_ids.get_device() != dev:
-            raise ValueError(f"position_ids must be int64 [{T}], [1, {T}] or [{B}, {T}] on {q.device}, got "
-                             f"{position_ids.dtype} {tuple(position_ids.shape)} on {position_ids.device}")
-        pos_ptr, pst = position_ids.data_ptr(), pstride[1]
-        if pshape[0] > 1:
-            psb = pstride[0]
-    else:
-        start = int(position_ids)
-    qsb, qst, one = q.stride()
-    if one != 1:
-        q = q.contiguous()
-        qsb, qst, one = q.stride()
-    if not q_weight.is_contiguous():
-        q_weight = q_weight.contiguous()
-    qo = q.new_empty((B, n // D, T, D))
-    if k is None:
-        H, ko, kp, kwp, kop, ksb, kst = 0, None, 0, 0, 0, 0, 0
-    else:
-        ksb, kst, one = k.stride()
-        if one != 1:
-            k = k.contiguous()
-            ksb, kst, one = k.stride()
-        if not k_weight.is_contiguous():
-            k_weight = k_weight.contiguous()
-        ko = k.new_empty((B, H, T, D))
-        kp, kwp, kop = k.data_ptr(), k_weight.data_ptr(), ko.data_ptr()
-    if B and T:
-        N.launch_packed("spx_qk_norm_rope", dev, N.QK_NORM_PACK.pack(
-            B, T, n // D, H, D, code, tshape[0], 1 if rotate_keys else 0, eps, 0, q.data_ptr(), kp, qsb, qst, ksb, kst,
-            q_weight.data_ptr(), kwp, cos.data_ptr(), sin.data_ptr(), pos_ptr, psb, pst, start, qo.data_ptr(), kop,
-            H * T * D, T * D))
-    return qo, ko
+        return _qk_norm_rope(q, k, q_weight, k_weight, cos, sin, position_ids, 0, eps, rotate_keys)
+    return _qk_norm_rope(q, k, q_weight, k_weight, cos, sin, None, int(position_ids), eps, rotate_keys)
 
 
 def quantize_int8(x: torch.Tensor):

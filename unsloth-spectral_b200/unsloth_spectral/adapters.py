@@ -18,6 +18,7 @@ from __future__ import annotations
 import math
 from typing import Dict, Optional, Sequence, Tuple, Union
 
+import numpy as np
 import torch
 
 from . import _native as N
@@ -36,7 +37,7 @@ class LoraBatch:
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        self._plans: Dict[Tuple[int, bool], tuple] = {}
+        self._front = N.front().Batch(len(self.slots), self.highest, self.device)
 
     def __len__(self) -> int:
         return len(self.slots)
@@ -49,38 +50,38 @@ class LoraBatch:
 
     @staticmethod
     def tiles_of(slots: Sequence[int], tokens: int, blocks: bool = False):
-        """Host lists ``(tile_rows, tiles, order)``: rows sorted by slot, cut into tiles of one
-        slot: 16 rows of any sequences, or 32 where a slot has more, which reads the adapter's
-        weights half as often; or ``blocks`` of up to 128 tokens of one sequence."""
-        groups: Dict[int, list] = {}
-        for i, s in enumerate(slots):
-            groups.setdefault(s, []).append(i)
-        most = max((len(g) for g in groups.values()), default=0) * tokens
-        rows = 128 if blocks else 16 if most <= 16 else 32
-        order = torch.empty(len(slots) * tokens, dtype=torch.int32)
+        """Host arrays ``(tile_rows, tiles [n, 4], order)``: rows sorted by slot, cut into tiles of
+        one slot: 16 rows of any sequences, or 32 where a slot has more, which reads the
+        adapter's weights half as often; or ``blocks`` of up to 128 tokens of one sequence,
+        which name their first row themselves (``order`` is empty)."""
+        ids = np.asarray(slots, dtype=np.int32)
+        seqs = np.argsort(ids, kind="stable").astype(np.int32)
+        n = len(ids) * tokens
+        if blocks:
+            cut = np.arange(0, tokens, 128, dtype=np.int32)
+            row0 = (seqs[:, None] * np.int32(tokens) + cut).reshape(-1)
+            rows = np.tile(np.minimum(128, tokens - cut), len(ids))
+            first = (np.arange(len(ids), dtype=np.int32)[:, None] * np.int32(tokens) + cut).reshape(-1)
+            tiles = np.stack([np.repeat(ids[seqs], len(cut)), first, rows, row0], 1)
+            return 128, tiles.astype(np.int32), np.empty(0, np.int32)
+        order = (seqs[:, None] * np.int32(tokens) + np.arange(tokens, dtype=np.int32)).reshape(-1)
+        used, counts = np.unique(ids, return_counts=True)
+        counts = counts * tokens
+        tile_rows = 16 if n == 0 or counts.max() <= 16 else 32
         tiles, at = [], 0
-        for s in sorted(groups):
-            seqs = torch.tensor(groups[s], dtype=torch.int32)
-            n = len(groups[s]) * tokens
-            order[at:at + n] = (seqs[:, None] * tokens + torch.arange(tokens, dtype=torch.int32)[None]).reshape(-1)
-            if rows == 128:
-                tiles += [(s, at + q * tokens + i, min(rows, tokens - i), 0) for q in range(len(groups[s]))
-                          for i in range(0, tokens, rows)]
-            else:
-                tiles += [(s, at + i, min(rows, n - i), 0) for i in range(0, n, rows)]
-            at += n
-        return rows, tiles, order
+        for s, m in zip(used.tolist(), counts.tolist()):
+            tiles += [(s, at + i, min(tile_rows, m - i), 0) for i in range(0, m, tile_rows)]
+            at += m
+        return tile_rows, np.asarray(tiles, dtype=np.int32).reshape(-1, 4), order
 
     def _plan(self, tokens: int, blocks: bool):
-        p = self._plans.get((tokens, blocks))
-        if p is None:
-            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(f"call LoraBatch.prepare({tokens}) before capturing a graph that uses the batch")
-            rows, tiles, order = self.tiles_of(self.slots, tokens, blocks)
-            t = torch.tensor(tiles, dtype=torch.int32).reshape(-1, 4)
-            p = (rows, len(tiles), len(order), t.to(self.device), order.to(self.device))
-            self._plans[tokens, blocks] = p
-        return p
+        if self._front.has(tokens, blocks):
+            return
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"call LoraBatch.prepare({tokens}) before capturing a graph that uses the batch")
+        tile_rows, tiles, order = self.tiles_of(self.slots, tokens, blocks)
+        held = torch.from_numpy(np.concatenate([tiles.reshape(-1), order])).to(self.device)
+        self._front.put(tokens, blocks, tile_rows, len(tiles), len(self.slots) * tokens, held)
 
 
 class LoraPool:
@@ -108,11 +109,7 @@ class LoraPool:
         self.ranks = torch.zeros(slots, parts, dtype=torch.int32, device=device)
         self.scales = torch.zeros(slots, parts, dtype=torch.float32, device=device)
         self.device = self.a.device
-        self._index = self.a.get_device()
-        # what of spx_lora_args does not change from call to call
-        self._pool_args = (in_features, parts, *widths, *(0,) * (N.LORA_MAX_PARTS - parts), self._rank, slots,
-                           N.dtype_code(dtype))
-        self._pool_ptrs = (self.a.data_ptr(), self.b.data_ptr(), self.ranks.data_ptr(), self.scales.data_ptr())
+        self._add = N.front().Pool(self.a, self.b, self.ranks, self.scales, list(widths)).add
 
     def _slot(self, slot: int, part: int):
         if not 0 <= slot < self.slots or not 0 <= part < len(self.widths):
@@ -148,42 +145,11 @@ class LoraPool:
         """``y + scale * B (A x)`` of each sequence's slot.  ``x [B, T, in]`` (or ``[B, in]``:
         one token each) and ``y [B, T, out]`` in the pool's dtype, rows on 16 bytes and evenly
         spaced; ``out`` may be ``y`` itself (in place), else a new tensor is returned."""
-        dev, dt = self._index, self.dtype
-        xs, ys = x.shape, y.shape
-        tokens = xs[1] if len(xs) == 3 else 1
-        if len(xs) not in (2, 3) or len(ys) != len(xs) or xs[-1] != self.in_features or ys[-1] != self.out_features \
-                or ys[:-1] != xs[:-1] or xs[0] != len(batch.slots):
-            raise ValueError(f"x [B, T, {self.in_features}] and y [B, T, {self.out_features}] of {len(batch)} sequences "
-                             f"expected, got {tuple(xs)} and {tuple(ys)}")
-        if batch.highest >= self.slots:
-            raise IndexError(f"the batch names slot {batch.highest}, the pool has {self.slots}")
-        if out is None:
-            out = x.new_empty(ys)
-        elif out.shape != ys:
-            raise ValueError(f"out {tuple(out.shape)} must have the shape of y {tuple(ys)}")
-        if not (x.dtype == dt and y.dtype == dt and out.dtype == dt and x.get_device() == dev and y.get_device() == dev
-                and out.get_device() == dev):
-            raise ValueError(f"x, y and out must be {dt} on {self.device}")
-        if batch.device != self.device:
-            raise ValueError(f"the batch is on {batch.device}, the pool on {self.device}")
-        if dev < 0:
-            N.lib_for(self.device)
-        if tokens == 0 or not batch.slots:
-            return out
-        # Prompts take the kernels for blocks of adjacent rows: 8 x 4096 tokens on q|k|v at rank 16
-        # 209 us against 410; below about 8M values of x and y their longer start shows
-        # (5 x 77 tokens on 4096 -> 14336 22 us against 14)
-        blocks = tokens >= 64 and len(batch.slots) * tokens * (self.in_features + self.out_features) >= 1 << 23
-        rows, n_tiles, n, tiles, order = batch._plan(tokens, blocks)
-        # the inner products, a buffer of each call's own: two streams or two captured graphs
-        # never share one (the caching allocator hands it out in stream order)
-        size = n * len(self.widths) * self._rank + 4
-        ws = self.scales.new_empty(size)
-        N.launch_packed("spx_lora_add", dev, N.LORA_PACK.pack(
-            n_tiles, rows, n, *self._pool_args, x.data_ptr(), y.data_ptr(), out.data_ptr(), _row_stride(x),
-            _row_stride(y), _row_stride(out), *self._pool_ptrs, tiles.data_ptr(), order.data_ptr(), ws.data_ptr(),
-            4 * size))
-        return out
+        r = self._add(y, x, batch._front, out)
+        if type(r) is tuple:      # (tokens, blocks): a grouping of rows that the batch has not made yet
+            batch._plan(*r)
+            r = self._add(y, x, batch._front, out)
+        return r
 
 
 def adapted(module, name: str, y: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
@@ -278,15 +244,3 @@ class LoraAdapters:
         if batch.highest >= self.slots:
             raise IndexError(f"slot {batch.highest} of {self.slots}")
         self.batch = batch
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    """The distance between the rows of ``t [.., n]``, which must be even."""
-    shape, stride = t.shape, t.stride()
-    if stride[-1] != 1:
-        raise ValueError(f"the last dimension must be contiguous, got strides {stride}")
-    if len(shape) == 2 or shape[1] == 1:
-        return stride[0] if shape[0] > 1 else max(stride[0], shape[-1])
-    if shape[0] > 1 and stride[0] != shape[1] * stride[1]:
-        raise ValueError(f"rows must be evenly spaced, got strides {stride} of {tuple(shape)}")
-    return stride[1]

@@ -45,7 +45,7 @@ class LogitsRules:
         if batch < 1 or batch > 65535 or not 1 <= vocab <= 1 << 30:
             raise ValueError(f"batch 1..65535 and vocab 1..2^30 expected, got {batch} and {vocab}")
         self.batch, self.vocab = batch, vocab
-        words = self._words = allow_words(vocab)
+        words = allow_words(vocab)
         rep = _setting("repetition_penalty", repetition_penalty, batch)
         if any(v <= 0 for v in rep):
             raise ValueError("repetition_penalty must be positive")
@@ -73,10 +73,8 @@ class LogitsRules:
         b = self._bias or (None,) * 3
         # the tokens that a rule touches: seen ones and, where there are any, biased ones
         self._touched = self.seen_bits if b[0] is None else b[0].clone()
-        self._index = self.counts.get_device()
-        # what of spx_logits_args does not change from call to call
-        self._state_ptrs = (N.ptr(self._rep), N.ptr(self._freq), N.ptr(self._pres), N.ptr(self.seen_bits),
-                            N.ptr(self._touched), N.ptr(self.counts), *(N.ptr(t) for t in b))
+        self._front = N.front().Rules(batch, vocab, self._rep, self._freq, self._pres, self.seen_bits, self._touched,
+                                      self.counts, *b)
 
     def reset(self):
         """Forget the history (a new generation with the same settings)."""
@@ -111,44 +109,11 @@ class LogitsRules:
         """``(processed logits, token)`` of ``logits [batch, vocab]``: float32, float16 or
         bfloat16; the processed ones are rounded to that dtype, into ``out`` when given
         (``out`` may be ``logits``).  The history is left as it is."""
-        if out is None:
-            out = logits.new_empty((self.batch, self.vocab))
-        return out, self._run(logits, allow, out, False)
+        return self._front.apply(logits, allow, out)
 
     def pick(self, logits: torch.Tensor, allow: Optional[torch.Tensor] = None, record: bool = False) -> torch.Tensor:
         """The token ``[batch]`` (int64) alone; ``record`` adds it to the history."""
-        return self._run(logits, allow, None, record)
-
-    def _run(self, logits, allow, out, record):
-        shape, dev, dt = (self.batch, self.vocab), self._index, logits.dtype
-        code = N.dtype_code(dt)
-        stride = logits.stride()
-        if logits.shape != shape or logits.get_device() != dev or stride[1] != 1 and self.vocab > 1:
-            raise ValueError(f"logits must be [{self.batch}, {self.vocab}] rows on {self.device}, got "
-                             f"{tuple(logits.shape)} (strides {stride}) on {logits.device}")
-        out_ptr = out_stride = 0
-        if out is not None:
-            out_ptr, out_stride = out.data_ptr(), out.stride(0)
-            if out.shape != shape or out.get_device() != dev or out.dtype != dt or out.stride(1) != 1 and self.vocab > 1:
-                raise ValueError(f"out must be [{self.batch}, {self.vocab}] {dt} rows on {self.device}, got {out.dtype} "
-                                 f"{tuple(out.shape)} (strides {out.stride()}) on {out.device}")
-        allow_ptr = allow_stride = 0
-        if allow is not None:
-            ashape, astride = allow.shape, allow.stride()
-            if len(ashape) == 1:
-                ashape, astride = (1, *ashape), (0, *astride)
-            if len(ashape) != 2 or ashape[0] not in (1, self.batch) or allow.dtype != torch.int32 \
-                    or ashape[1] < self._words or astride[1] != 1 or allow.get_device() != dev:
-                raise ValueError(f"allow must be int32 [{self.batch} or 1, {self._words}] on {self.device}, got "
-                                 f"{allow.dtype} {tuple(allow.shape)} on {allow.device}")
-            allow_ptr, allow_stride = allow.data_ptr(), astride[0] if ashape[0] > 1 else 0
-        if dev < 0:
-            N.lib_for(self.device)
-        token = logits.new_empty(self.batch, dtype=torch.int64)
-        N.launch_packed("spx_logits_rules", dev, N.LOGITS_PACK.pack(
-            self.batch, self.vocab, code, 1 if record else 0, logits.data_ptr(), stride[0], out_ptr, out_stride,
-            token.data_ptr(), *self._state_ptrs, allow_ptr, allow_stride))
-        return token
+        return self._front.run(logits, allow, None, record)
 
 
 def _setting(name: str, v: Setting, batch: int):
