@@ -127,6 +127,11 @@ def test_strided_rows_and_what_lies_between_them(dtype):
     from unsloth_spectral import _native as N
     with pytest.raises(N.SpxError):                                # rows off 16 bytes
         pool.add(y, wide[..., 1:129], LoraBatch(ids))
+    flat = torch.zeros(3 * 5 * 64 + 8, dtype=dtype, device="cuda")
+    with pytest.raises(RuntimeError):                              # out a shifted view of y
+        pool.add(flat[:-8].view(3, 5, 64), x, LoraBatch(ids), out=flat[8:].view(3, 5, 64))
+    with pytest.raises(N.SpxError):                                # out the same row for every sequence
+        pool.add(y[:, :1], x[:, :1], LoraBatch(ids), out=room[:1, :1, 8:72].expand(3, 1, 64))
     with pytest.raises(ValueError):                                # rows not evenly spaced
         pool.add(y[:, :3], wide[:, :3, 16:144], LoraBatch(ids))
 

@@ -3,6 +3,7 @@
 // current stream and device, then the C call.  In Python, on ctypes, the same took 11 to 14 us
 // a call, of which the GPU needs 3 to 6; here it takes 5 to 8.  No CUDA code: the kernels are
 // libspx.so's, called through include/spx.h.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -176,6 +177,8 @@ struct Pool {
     TORCH_CHECK_VALUE(batch.device == a.device(), "the batch is on ", batch.device, ", the pool on ", a.device());
     require_device(a.device());
     const int64_t tokens = d == 3 ? x.size(1) : 1, rows = batch.sequences * tokens;
+    TORCH_CHECK_VALUE(rows <= 1 << 30, rows, " rows in one call");
+    if (out_) at::assert_no_partial_overlap(*out_, y);
     if (rows == 0) return out_ ? *out_ : at::empty_like(y);
     // Prompts take the kernels for blocks of adjacent rows: 8 x 4096 tokens on q|k|v at rank 16
     // 207 us against 410; below about 8M values of x and y their longer start shows
@@ -246,6 +249,7 @@ struct Rules {
       v.allow = reinterpret_cast<const uint32_t*>(allow->const_data_ptr<int32_t>());
       v.allow_stride = rows > 1 ? allow->stride(0) : 0;
     }
+    if (out) at::assert_no_partial_overlap(*out, logits);
     require_device(device);
     Tensor token = at::empty({args.batch}, logits.options().dtype(at::kLong));
     v.record = record, v.logits = logits.const_data_ptr(), v.logits_stride = logits.stride(0);

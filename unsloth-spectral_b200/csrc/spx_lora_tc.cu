@@ -427,7 +427,8 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
     int i = 0, n = 0, v = -1;
     Version ver{};
     float s1 = 0.f;
-    for (Walk w(p, ch, c0); c0 + i < c1; ++i, w.next(p, ch)) {
+    Walk w(p, ch, c0);
+    for (; c0 + i < c1; ++i, w.next(p, ch)) {
       const int s = i % stages, a = n & 1;
       if (w.fresh) {
         ++v;
@@ -492,6 +493,11 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
       __syncwarp();
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    for (; c0 + i < c1; ++i, w.next(p, ch)) {   // a wait expired: what is left is NaN, not what lay there
+      const int4 tile = p.tiles[w.tl];
+      T* o = static_cast<T*>(p.out) + (int64_t)(tile.w + r) * p.os + w.col + half * 64;
+      for (int e = 0; r < tile.z && e < 64 && half * 64 + e < w.left; ++e) o[e] = from_f<T>(__int_as_float(0x7fc00000));
+    }
   }
   __syncwarp();
   tc_fence_before();

@@ -37,6 +37,8 @@ class LogitsRules:
 
     The chosen token is the largest of these float32 values, the lowest index among equals;
     a NaN counts as largest; a request whose every token is at -inf gets token 0.
+
+    The calls on one object share its history: make them on one stream, or order them.
     """
 
     def __init__(self, batch: int, vocab: int, device="cuda", *, repetition_penalty: Setting = 1.0,
