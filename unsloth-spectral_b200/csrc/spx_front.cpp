@@ -181,7 +181,7 @@ struct Pool {
     if (out_) at::assert_no_partial_overlap(*out_, y);
     if (rows == 0) return out_ ? *out_ : at::empty_like(y);
     // Prompts take the kernels for blocks of adjacent rows: 8 x 4096 tokens on q|k|v at rank 16
-    // 207 us against 410; below about 8M values of x and y their longer start shows
+    // 196 us against 410; below about 8M values of x and y their longer start shows
     // (5 x 77 tokens on 4096 -> 14336 22 us against 12).
     const bool blocks = tokens >= 64 && rows * (in + out) >= (int64_t)1 << 23;
     const auto plan = batch.plans.find({tokens, blocks});

@@ -187,16 +187,19 @@ __global__ void __launch_bounds__(128) shrink_block_kernel(const __grid_constant
 }
 
 // ------------------------------------------------------------------------- expand ----
-// out = y + scale * B t as a stream of chunks of 128 rows x 128 columns.  One warp copies y
-// and the chunk's rows of B through a ring of stages with TMA; four warps make the A operand
-// of a tile and part (t, its high and low halves in two values of the row type each), one
-// ahead of its use; one thread issues the MMAs (f32 in tensor memory, two buffers); eight
-// warps add the product to y in the stage itself (thread = row, half of the columns) and
-// store from there with TMA.  The chunks of all tiles are dealt out evenly to one CTA an SM.
-// Before: y through registers (16 warps an SM, 2 KB in flight each) 4.6 TB/s; this ring with
-// mma.sync 4.9 TB/s at rank 16, but 1.5 TB/s at rank 64; with t staged by the warps that
-// store, 3 to 4 us of each change of tile or part showed.
-constexpr int EC = 128, EROWS = 32, YBOX = M * 64 * 2, YBYTES = 2 * YBOX, EWARPS = 8, BWARPS = 4;
+// out = y + scale * B t as a stream of chunks of 128 rows x 128 columns, one CTA an SM.  One
+// warp copies y and the chunk's rows of B through a ring of stages with TMA; four warps make
+// the A operand of a tile and part (t, its high and low halves in two values of the row type
+// each), one ahead of its use; one thread issues the MMAs (f32 in tensor memory, two buffers);
+// two groups of eight warps take the chunks in turn, add the product to y in the stage itself
+// (thread = row, half of the columns) and store from there with TMA.
+// Bound by memory: 8 x 4096 rows of 6144 bf16 take 135 to 140 us, at rank 16 as at rank 0 (the
+// ring alone), where a copy of y takes 125.  What it took: y through registers (16 warps an SM)
+// 174; this ring with mma.sync 165 (500 at rank 64); tcgen05 with one group of eight warps 147
+// (a chunk's waits, 1.7 us, were longer than its share of the stream, 1.4); the chunks dealt
+// out so that the CTAs move along whole rows, four chunks (1 KB) each at a time, instead of
+// each its own rows (128 pages open a CTA): 6 us less; eight chunks 4 us more, two 8.
+constexpr int EC = 128, EROWS = 32, YBOX = M * 64 * 2, YBYTES = 2 * YBOX, EGROUP = 8, EWARPS = 2 * EGROUP, BWARPS = 4;
 constexpr int ETHREADS = (EWARPS + 2 + BWARPS) * 32;
 
 // What the warps need to know of a tile and part: a version of the A operand.
@@ -206,7 +209,7 @@ struct Version {
 };
 
 struct Chunks {
-  int per_tile, total;                          // chunks of a tile, of all tiles
+  int per_tile, unit, units_per_tile, units;    // chunks of a tile, of a unit, units of a tile, of all tiles
   int first[SPX_LORA_MAX_PARTS + 1];            // first chunk of each part
   int kw;                                       // ranks of a box of B: 16, 32 or 64
 };
@@ -232,45 +235,62 @@ __device__ __forceinline__ void tld32(uint32_t taddr, float (&v)[32]) {
   for (int u = 0; u < 32; ++u) v[u] = __uint_as_float(r[u]);
 }
 
+// A row of t on its way to the A operand: its first 16 values in registers, the others into L2.
+struct TRow {
+  static constexpr int HELD = 4;
+  const float* t;
+  float4 v[HELD];
+  __device__ __forceinline__ float4 at(int q) const { return reinterpret_cast<const float4*>(t)[q]; }
+  __device__ __forceinline__ void load(const float* row, bool in, int R) {
+    t = row;
+#pragma unroll
+    for (int q = 0; q < HELD; ++q) v[q] = in && 4 * q < R ? at(q) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = HELD; in && 4 * q < R; q += 8) asm volatile("prefetch.global.L2 [%0];" ::"l"(t + 4 * q));
+  }
+};
+
 // Row r of a tile's t as the high and low parts of the A operand: element (row, k) at
 // (k / 8) * 2048 + row * 16 + (k % 8) * 2, the low parts 256 R bytes on.  Returns what the row
 // of the product is to be multiplied by.
 template <typename T>
-__device__ __forceinline__ float stage_t(const float* t, bool in, int R, int r, uint8_t* a) {
+__device__ __forceinline__ float stage_t(const TRow& row, bool in, int R, int r, uint8_t* a) {
   float dn = 1.f, up = 1.f;
   if (!__is_same(T, __nv_bfloat16)) {
     // f16: scaled by a power of two so that the row's largest value is near 2^8 (no overflow
     // of the high parts, no underflow of the low parts)
     float mx = 0.f;
-    for (int k = 0; in && k < R; k += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(t + k);
+    const auto see = [&](const float4& v) {
       mx = fmaxf(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))), mx);
-    }
+    };
+#pragma unroll
+    for (int q = 0; q < TRow::HELD; ++q) see(row.v[q]);
+#pragma unroll 4
+    for (int q = TRow::HELD; q < R / 4; ++q)
+      if (in) see(row.at(q));
     int ex = (int)((__float_as_uint(mx) >> 23) & 0xff) - 127 - 8;
     ex = max(-118, min(118, ex));
     dn = __uint_as_float((uint32_t)(127 - ex) << 23);
     up = __uint_as_float((uint32_t)(127 + ex) << 23);
   }
-#pragma unroll 4
-  for (int k8 = 0; k8 < R / 8; ++k8) {
-    uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
-    if (in) {
+  const auto put = [&](int k8, const float4& u, const float4& w) {
+    uint4 hi, lo;
+    const float f[8] = {u.x * dn, u.y * dn, u.z * dn, u.w * dn, w.x * dn, w.y * dn, w.z * dn, w.w * dn};
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const float4 v = *reinterpret_cast<const float4*>(t + k8 * 8 + q * 4);
-        const float f[4] = {v.x * dn, v.y * dn, v.z * dn, v.w * dn};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const T h = from_f<T>(f[e]);
-          reinterpret_cast<T*>(&hi)[q * 4 + e] = h;
-          // an infinity has no low part
-          reinterpret_cast<T*>(&lo)[q * 4 + e] = from_f<T>(fabsf(to_f(h)) < INFINITY ? f[e] - to_f(h) : 0.f);
-        }
-      }
+    for (int e = 0; e < 8; ++e) {
+      const T h = from_f<T>(f[e]);
+      reinterpret_cast<T*>(&hi)[e] = h;
+      // an infinity has no low part
+      reinterpret_cast<T*>(&lo)[e] = from_f<T>(fabsf(to_f(h)) < INFINITY ? f[e] - to_f(h) : 0.f);
     }
     *reinterpret_cast<uint4*>(a + k8 * 2048 + r * 16) = hi;
     *reinterpret_cast<uint4*>(a + 256 * R + k8 * 2048 + r * 16) = lo;
-  }
+  };
+#pragma unroll
+  for (int k8 = 0; k8 < TRow::HELD / 2; ++k8)
+    if (8 * k8 < R) put(k8, row.v[2 * k8], row.v[2 * k8 + 1]);
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k8 = TRow::HELD / 2; k8 < R / 8; ++k8) put(k8, in ? row.at(2 * k8) : zero, in ? row.at(2 * k8 + 1) : zero);
   return up;
 }
 
@@ -299,9 +319,9 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
   }
   if (tid == 0) {
     s_abort = 0;
-    for (int s = 0; s < stages; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, EWARPS);
+    for (int s = 0; s < stages; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, EGROUP);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(acc_full0 + 8 * s, 1), mbar_init(acc_empty0 + 8 * s, EWARPS);
+      mbar_init(acc_full0 + 8 * s, 1), mbar_init(acc_empty0 + 8 * s, EGROUP);
       mbar_init(t_ready0 + 8 * s, BWARPS), mbar_init(t_free0 + 8 * s, EWARPS + 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -312,15 +332,18 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   const Abort ab{&s_abort, reinterpret_cast<int*>(p.t + (int64_t)p.rows * p.SR)};
-  const int c0 = (int)((int64_t)ch.total * blockIdx.x / gridDim.x), c1 = (int)((int64_t)ch.total * (blockIdx.x + 1) / gridDim.x);
 
-  // The walk over the CTA's chunks, the same in every role.
+  // The walk over the CTA's chunks, the same in every role: every gridDim-th unit of `unit`
+  // chunks that follow one another in a tile, so that the CTAs together move along whole rows.
   struct Walk {
-    int tl, part, k, col, left;   // tile, part, chunk within the tile, first column, columns of the part from there on
-    bool fresh;                   // another tile or part than the chunk before: a new version
-    __device__ __forceinline__ Walk(const Params& p, const Chunks& ch, int q) {
-      tl = q / ch.per_tile;
-      k = q - tl * ch.per_tile;
+    int u, tl, part, k, end, col, left;   // unit, tile, part, chunk, end of the unit; first column, columns of the part from there
+    bool fresh;                           // another unit or part than the chunk before: a new version
+    __device__ __forceinline__ Walk(const Params& p, const Chunks& ch) : u(blockIdx.x) { start(p, ch); }
+    __device__ __forceinline__ bool valid(const Chunks& ch) const { return u < ch.units; }
+    __device__ __forceinline__ void start(const Params& p, const Chunks& ch) {
+      tl = u / ch.units_per_tile;
+      k = (u - tl * ch.units_per_tile) * ch.unit;
+      end = min(k + ch.unit, ch.per_tile);
       part = 0, col = 0;
       while (k >= ch.first[part + 1]) col += p.width[part++];
       left = p.width[part] - (k - ch.first[part]) * EC;
@@ -328,36 +351,43 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
       fresh = true;
     }
     __device__ __forceinline__ void next(const Params& p, const Chunks& ch) {
-      fresh = ++k == ch.first[part + 1];
-      if (!fresh) {
-        col += EC, left -= EC;
+      if (++k == end) {
+        u += gridDim.x;
+        if (u < ch.units) start(p, ch);
         return;
       }
-      col += left;
-      if (++part == p.parts) part = 0, k = 0, col = 0, ++tl;
-      left = p.width[part];
+      fresh = k == ch.first[part + 1];
+      if (fresh) {
+        col += left;
+        left = p.width[++part];
+      } else {
+        col += EC, left -= EC;
+      }
     }
   };
 
   if (warp == EWARPS) {
     if (lane == 0) {
-      int i = 0, row0 = 0;
-      int4 tile = make_int4(0, 0, 0, 0);
-      for (Walk w(p, ch, c0); c0 + i < c1; ++i, w.next(p, ch)) {
-        if (w.fresh) tile = p.tiles[w.tl], row0 = tile.w;
+      // the tile of the unit after this one is looked up ahead: the ring never waits for it
+      const auto tile_of = [&](int u) { return p.tiles[min(u, ch.units - 1) / ch.units_per_tile]; };
+      int i = 0, unit = -1;
+      int4 tile, ahead = tile_of(blockIdx.x);
+      Walk w(p, ch);
+      for (; w.valid(ch); ++i, w.next(p, ch)) {
+        if (w.u != unit) unit = w.u, tile = ahead, ahead = tile_of(w.u + gridDim.x);
         const int s = i % stages;
         if (i >= stages && !wait1(empty0 + 8 * s, (uint32_t)((i / stages - 1) & 1), ab)) break;
         const uint32_t dst = base + s * sbytes, bar = full0 + 8 * s;
         // a box that begins past the part is not wanted (and past the last one lies outside)
         const bool two = w.left > 64;
         mbar_expect_tx(bar, (uint32_t)((two ? YBYTES : YBOX) + (tile.x >= 0 ? bbytes : 0)));
-        tma_2d(dst, &my, w.col, row0, bar);
-        if (two) tma_2d(dst + YBOX, &my, w.col + 64, row0, bar);
+        tma_2d(dst, &my, w.col, tile.w, bar);
+        if (two) tma_2d(dst + YBOX, &my, w.col + 64, tile.w, bar);
         if (tile.x >= 0)
           for (int b = 0; b < p.R / ch.kw; ++b)
             tma_2d(dst + YBYTES + b * EC * ch.kw * 2, &mb, b * ch.kw, tile.x * p.OUT + w.col, bar);
       }
-      if (c0 + i < c1) {   // given up: the copies in flight land before the shared memory goes
+      if (w.valid(ch)) {   // given up: the copies in flight land before the shared memory goes
         for (int q = i > stages ? i - stages : 0; q < i; ++q) {
           const uint64_t t0 = gtimer();
           while (!mbar_try_wait_sleep(full0 + 8 * (q % stages), (uint32_t)((q / stages) & 1)) && gtimer() - t0 < kWaitNs) {
@@ -368,7 +398,7 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
   } else if (warp == EWARPS + 1) {
     if (lane == 0) {
       int i = 0, n = 0, v = -1, rank = 0, buf = 0;   // chunk, accumulators used, version
-      for (Walk w(p, ch, c0); c0 + i < c1; ++i, w.next(p, ch)) {
+      for (Walk w(p, ch); w.valid(ch); ++i, w.next(p, ch)) {
         if (w.fresh) {
           if (v >= 0) umma_commit(t_free0 + 8 * buf);   // once the MMAs that read it are done
           ++v;
@@ -398,38 +428,62 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
     }
   } else if (warp > EWARPS + 1) {
     asm volatile("griddepcontrol.wait;" ::: "memory");   // t of the shrink kernel
+    // Under the stream a load takes microseconds: what a version needs is fetched while the one
+    // before it is staged, its tile while the one before that is.
+    struct Next {
+      bool ok;
+      int part;
+      int4 tile;
+    };
     const int r = tid - (EWARPS + 2) * 32;
-    int i = 0, v = -1;
-    for (Walk w(p, ch, c0); c0 + i < c1; ++i, w.next(p, ch)) {
-      if (!w.fresh) continue;
-      ++v;
+    Walk w(p, ch);
+    const auto take = [&]() {
+      Next n{w.valid(ch), w.part, make_int4(-1, 0, 0, 0)};
+      if (n.ok) {
+        n.tile = p.tiles[w.tl];
+        do w.next(p, ch);
+        while (w.valid(ch) && !w.fresh);
+      }
+      return n;
+    };
+    const auto fetch = [&](const Next& n, Version& ver, TRow& t) {
+      const bool slot = n.ok && n.tile.x >= 0;
+      ver.rank = slot ? p.ranks[n.tile.x * p.parts + n.part] : 0;
+      ver.scale = slot ? p.scales[n.tile.x * p.parts + n.part] : 0.f;
+      ver.row0 = n.tile.w;
+      ver.rows = n.tile.z;
+      t.load(p.t + (int64_t)(n.tile.y + r) * p.SR + n.part * p.R, slot && r < n.tile.z, p.R);
+    };
+    Next now = take(), next = take();
+    Version ver, ver_next;
+    TRow t, t_next;
+    fetch(now, ver, t);
+    for (int v = 0; now.ok; ++v) {
+      fetch(next, ver_next, t_next);
+      const Next after = take();
       const int buf = v % abufs;
-      const int4 tile = p.tiles[w.tl];
-      Version ver;
-      ver.rank = tile.x < 0 ? 0 : p.ranks[tile.x * p.parts + w.part];
-      ver.scale = tile.x < 0 ? 0.f : p.scales[tile.x * p.parts + w.part];
-      ver.row0 = tile.w;
-      ver.rows = tile.z;
       if (v >= abufs && !waitw(t_free0 + 8 * buf, (uint32_t)((v / abufs - 1) & 1), ab)) break;
       if (ver.rank > 0)
-        row_scale[buf][r] = ver.scale * stage_t<T>(p.t + (int64_t)(tile.y + r) * p.SR + w.part * p.R, r < tile.z, p.R, r,
-                                                   a_op + buf * 512 * p.R);
+        row_scale[buf][r] = ver.scale * stage_t<T>(t, r < ver.rows, p.R, r, a_op + buf * 512 * p.R);
       if (r == 0) versions[buf] = ver;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(t_ready0 + 8 * buf);
+      now = next, next = after, ver = ver_next, t = t_next;
     }
   } else {
     // before the first store, so that this grid never ends before the one that still reads x
     // and writes the workspace
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int quad = warp & 3, half = warp >> 2, r = quad * 32 + lane;
+    // two groups of eight warps take the chunks in turn, so that the waits of one chunk (its sums,
+    // its store) pass while the other is worked on
+    const int quad = warp & 3, half = (warp >> 2) & 1, group = warp / EGROUP, r = quad * 32 + lane;
     int i = 0, n = 0, v = -1;
     Version ver{};
     float s1 = 0.f;
-    Walk w(p, ch, c0);
-    for (; c0 + i < c1; ++i, w.next(p, ch)) {
-      const int s = i % stages, a = n & 1;
+    Walk w(p, ch);
+    for (; w.valid(ch); ++i, w.next(p, ch)) {
+      const int s = i % stages;
       if (w.fresh) {
         ++v;
         const int buf = v % abufs;
@@ -440,14 +494,17 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
         if (lane == 0) mbar_arrive(t_free0 + 8 * buf);
       }
       const bool act = ver.rank > 0;
+      const int acc = n;
+      n += act;
+      if ((i & 1) != group) continue;
+      const int a = acc & 1;
       if (!waitw(full0 + 8 * s, (uint32_t)((i / stages) & 1), ab)) break;
       uint8_t* const yrow = sm + s * sbytes + half * YBOX + r * 128;
       const int left = w.left - half * 64;   // columns of this half
       const bool tma_out = ver.rows >= quad * EROWS + EROWS && left >= 64;
       if (act) {
-        if (!waitw(acc_full0 + 8 * a, (uint32_t)((n / 2) & 1), ab)) break;
+        if (!waitw(acc_full0 + 8 * a, (uint32_t)((acc / 2) & 1), ab)) break;
         tc_fence_after();
-        ++n;
       }
 #pragma unroll
       for (int hc = 0; hc < 2; ++hc) {
@@ -486,14 +543,14 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
                        : "memory");
         }
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        // the chunk before this one is read out: its stage is free
-        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-        if (i > 0) mbar_arrive(empty0 + 8 * ((i - 1) % stages));
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // read out: the stage is free
+        mbar_arrive(empty0 + 8 * s);
       }
       __syncwarp();
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-    for (; c0 + i < c1; ++i, w.next(p, ch)) {   // a wait expired: what is left is NaN, not what lay there
+    for (; w.valid(ch); ++i, w.next(p, ch)) {   // a wait expired: what is left is NaN, not what lay there
+      if ((i & 1) != group) continue;
       const int4 tile = p.tiles[w.tl];
       T* o = static_cast<T*>(p.out) + (int64_t)(tile.w + r) * p.os + w.col + half * 64;
       for (int e = 0; r < tile.z && e < 64 && half * 64 + e < w.left; ++e) o[e] = from_f<T>(__int_as_float(0x7fc00000));
@@ -593,7 +650,12 @@ static int launch_expand_block(const Params& p, int dtype, int tiles, cudaStream
   ch.per_tile = ch.first[p.parts];
   ch.kw = p.R % 64 == 0 ? 64 : p.R % 32 == 0 ? 32 : 16;
   SPX_REQUIRE((int64_t)tiles * ch.per_tile <= 0x3fffffff, SPX_ERR_SHAPE, "spx_lora_add: too many rows");
-  ch.total = tiles * ch.per_tile;
+  // Four chunks (1 KB of a row) to a unit while every SM gets four units or more.
+  const int most = num_sms();
+  ch.unit = 4;
+  while (ch.unit > 1 && (int64_t)tiles * ch.per_tile < (int64_t)4 * ch.unit * most) ch.unit /= 2;
+  ch.units_per_tile = (ch.per_tile + ch.unit - 1) / ch.unit;
+  ch.units = tiles * ch.units_per_tile;
   const int abufs = p.R <= 64 ? 2 : 1, sbytes = YBYTES + EC * p.R * 2, abytes = abufs * 2 * M * p.R * 2;
   int stages = (220 * 1024 - abytes) / sbytes;   // 2 (rank 128) to 5 (rank 16)
   if (stages > MAXSTAGES) stages = MAXSTAGES;
@@ -609,9 +671,8 @@ static int launch_expand_block(const Params& p, int dtype, int tiles, cudaStream
   if (rc != SPX_OK) return rc;
   const uint32_t fmt = dtype == SPX_F16 ? 0u : 1u;
   const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(EC >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-  const int most = num_sms();
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(ch.total < most ? ch.total : most));
+  cfg.gridDim = dim3((unsigned)(ch.units < most ? ch.units : most));
   cfg.blockDim = dim3(ETHREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
