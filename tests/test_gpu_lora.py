@@ -71,15 +71,14 @@ CASES = [
     (4, 100, 256, (512,), [40, 48], [-1, 1, 1, 0]),
     (2, 300, 4096, (520, 128, 128), [64, 32], [1, 0]),
     (1, 515, 40, (24,), [24], [0]),
-    # blocks of adjacent rows (8M values of x and y, or more): ragged tiles and parts, every stored rank
-    (3, 1037, 2056, (520, 128, 136), [16, (5, 0, 16)], [1, 0, -1]),
-    (2, 2100, 1048, (1000,), [32, 20], [0, 1]),
-    (1, 4100, 64, (2056, 8), [48], [0]),
+    # blocks of adjacent rows: ragged tiles and parts, every stored rank
+    (3, 3137, 2056, (1520, 128, 136), [16, (5, 0, 16)], [1, 0, -1]),
+    (2, 4500, 1048, (1000,), [32, 20], [0, 1]),
+    (1, 6100, 64, (2056, 8), [48], [0]),
     (2, 1100, 4096, (264, 64, 64), [64, 33], [1, 0]),
     (5, 700, 1024, (1400,), [128, 80, 3], [2, 1, 0, -1, 1]),
-    (64, 64, 1032, (1040,), [16, 9], [i % 3 - 1 for i in range(64)]),
-    (2, 130, 14336, (18000,), [7, 16], [0, 1]),
-    (3, 4, 64, (64,), [16, 0], [1, -1, 1]),
+    (64, 64, 4104, (4136,), [16, 9], [i % 3 - 1 for i in range(64)]),
+    (2, 530, 14336, (18000,), [7, 16], [0, 1]),
 ]
 
 

@@ -180,10 +180,11 @@ struct Pool {
     TORCH_CHECK_VALUE(rows <= 1 << 30, rows, " rows in one call");
     if (out_) at::assert_no_partial_overlap(*out_, y);
     if (rows == 0) return out_ ? *out_ : at::empty_like(y);
-    // Prompts take the kernels for blocks of adjacent rows: 8 x 4096 tokens on q|k|v at rank 16
-    // 196 us against 410; below about 8M values of x and y their longer start shows
-    // (5 x 77 tokens on 4096 -> 14336 22 us against 12).
-    const bool blocks = tokens >= 64 && rows * (in + out) >= (int64_t)1 << 23;
+    // Prompts take the kernels for blocks of adjacent rows, whose start takes longer and whose
+    // time does not grow with the rank.  They meet at about 30M values of x and y at rank 16 and
+    // 32 (4096 -> 6144 columns at rank 16: 2048 rows 24 us against 27, 4096 rows 45 against 42,
+    // 16384 rows 162 against 109) and 8M at rank 64 (4096 -> 4096: 1024 rows 31 against 23).
+    const bool blocks = tokens >= 64 && rows * (in + out) * args.max_rank >= (int64_t)1 << 29;
     const auto plan = batch.plans.find({tokens, blocks});
     if (plan == batch.plans.end()) return std::make_pair(tokens, blocks);
     const Batch::Plan& p = plan->second;

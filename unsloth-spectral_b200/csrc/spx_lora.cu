@@ -13,14 +13,10 @@
 // gives 16-byte accesses of y and out.
 // t is kept in float32; for the second product it is split into a high and a low value of
 // the row type (two MMAs), which keeps about 16 (bf16) or 22 (f16) bits of it.
-#include <cooperative_groups.h>
-
 #include "spx_lora.cuh"
 
 namespace spx {
 namespace lora {
-
-namespace cg = cooperative_groups;
 
 constexpr int SW = 8;    // warps of a shrink CTA
 constexpr int EW = 4;    // warps of an expand CTA
@@ -35,7 +31,9 @@ template <int MT, int NT>
 struct Ring {
   static constexpr int VECS = 2 * MT + NT;                                   // 16 bytes a lane each
   static constexpr int FIT = 73 * 1024 / (SW * VECS * 512), STAGES = FIT > 6 ? 6 : FIT < 2 ? 2 : FIT;   // three CTAs an SM
-  static constexpr size_t BYTES = (size_t)SW * STAGES * VECS * 512;
+  static constexpr int SUMS = SW * MT * 16 * NT * 8, COPIES = SW * STAGES * VECS * 128;   // floats
+  static constexpr int FLOATS = SUMS > COPIES ? SUMS : COPIES;
+  static constexpr size_t BYTES = 4 * ((size_t)FLOATS + MT * 16 * NT * 8);
 };
 
 __device__ __forceinline__ void copy16(uint4* dst, const void* src, bool in) {   // zeros unless `in`
@@ -48,9 +46,11 @@ template <typename T, int MT, int NT>
 __global__ void __launch_bounds__(SW * 32) shrink_kernel(const Params p) {
   using Ri = Ring<MT, NT>;
   extern __shared__ uint4 ring[];
-  float* const sums = reinterpret_cast<float*>(ring);   // [SW][MT * 16][NT * 8], after the stream
-  cg::cluster_group cl = cg::this_cluster();
-  const int cs = (int)cl.num_blocks(), cr = (int)cl.block_rank();
+  constexpr int N = NT * 8, E = MT * 16 * N;
+  float* const sums = reinterpret_cast<float*>(ring);   // [SW][MT * 16][N], after the stream
+  float* const got = reinterpret_cast<float*>(ring) + Ri::FLOATS;   // [cs][E / cs]: the cluster's sums of this CTA's share
+  cluster_arrive_relaxed();
+  const int cs = (int)cluster_size(), cr = (int)cluster_rank();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int4 tile = p.tiles[blockIdx.x / cs];
   if (tile.x < 0) return;   // rows without an adapter: the whole cluster leaves
@@ -122,7 +122,6 @@ __global__ void __launch_bounds__(SW * 32) shrink_kernel(const Params p) {
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();   // the ring becomes the sums
-  constexpr int N = NT * 8, E = MT * 16 * N;
   float* part = sums + warp * E;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -132,24 +131,26 @@ __global__ void __launch_bounds__(SW * 32) shrink_kernel(const Params p) {
       *reinterpret_cast<float2*>(part + (m * 16 + g + 8) * N + n * 8 + 2 * c) = make_float2(acc[m][n][2], acc[m][n][3]);
     }
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += SW * 32) {   // each thread its own elements: in place
+  cluster_started();
+  const int share = E / cs;   // cs is a power of two up to 8, E a multiple of 256
+  for (int e = threadIdx.x; e < E; e += SW * 32) {
     float v = sums[e];
 #pragma unroll
     for (int w = 1; w < SW; ++w) v += sums[w * E + e];
-    sums[e] = v;
+    const int owner = e / share;
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(in_cta(got + cr * share + e - owner * share, owner)), "f"(v) : "memory");
   }
-  cl.sync();
-  for (int e = cr * SW * 32 + threadIdx.x; e < E; e += cs * SW * 32) {
-    const int r = e / N, col = col0 + e % N;
-    float v = 0.f;
-    for (int k = 0; k < cs; ++k) v += cl.map_shared_rank(sums, k)[e];
+  cluster_pushed();
+  for (int i = threadIdx.x; i < share; i += SW * 32) {
+    const int e = cr * share + i, r = e / N, col = col0 + e % N;
+    float v = got[i];
+    for (int k = 1; k < cs; ++k) v += got[k * share + i];
     if (r < tile.z && col < p.SR) {
       // past the rank: exact zeros, also where x holds an infinity
       if (col % p.R >= p.ranks[tile.x * p.parts + col / p.R]) v = 0.f;
       p.t[(int64_t)(tile.y + r) * p.SR + col] = v;
     }
   }
-  cl.sync();   // no CTA leaves while its shared memory may be read
 }
 
 // ------------------------------------------------------------------------- expand ----
@@ -277,8 +278,7 @@ __global__ void __launch_bounds__(EW * 32) expand_kernel(const Params p, const i
 
 template <typename T, int MT, int NT>
 int launch_shrink(const Params& p, int tiles, int groups, int cs, cudaStream_t st) {
-  const size_t sums = (size_t)SW * MT * 16 * NT * 8 * sizeof(float);
-  const size_t smem = sums > Ring<MT, NT>::BYTES ? sums : Ring<MT, NT>::BYTES;
+  const size_t smem = Ring<MT, NT>::BYTES;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(shrink_kernel<T, MT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)smem);

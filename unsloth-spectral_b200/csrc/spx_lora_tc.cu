@@ -6,10 +6,10 @@
 // Bound by memory: 2 * N flops a byte of x at most.  Two CTAs an SM keep about 128 KB of x in
 // flight: 268 MB of x (8 x 4096 rows of 4096 bf16) take 55 to 61 us, as long as a plain sum
 // over them; the mma.sync kernel (fragments loaded by the warps that use them, 8 warps an SM)
-// took 214.  More stages, or boxes twice as wide, measured level.  Few tiles: the CTAs of a cluster split k and add their sums over distributed shared
-// memory in a fixed order.  Rows of the next sequence that a tile's box covers are computed
-// and not stored.  Every wait is bounded; an expired one leaves NaN in t.
-#include <cooperative_groups.h>
+// took 214.  More stages, or boxes twice as wide, measured level.  Few tiles: the CTAs of a
+// cluster split k and push their sums into one another's shared memory, added in a fixed
+// order.  Rows of the next sequence that a tile's box covers are computed and not stored.
+// Every wait is bounded; an expired one leaves NaN in t.
 #include <cuda.h>
 
 #include "spx_lora.cuh"
@@ -19,7 +19,6 @@ namespace spx {
 namespace lora {
 
 using namespace sm100;
-namespace cg = cooperative_groups;
 
 constexpr int M = 128, KB = 64;            // rows of a tile, values of k in a stage
 constexpr int MAXSTAGES = 8;               // barriers of a ring
@@ -70,9 +69,9 @@ __global__ void __launch_bounds__(128) shrink_block_kernel(const __grid_constant
   extern __shared__ uint8_t raw_smem[];
   __shared__ __align__(8) uint64_t bars[2 * MAXSTAGES + 1];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort;
-  cg::cluster_group cl = cg::this_cluster();
-  const int cs = (int)cl.num_blocks(), cr = (int)cl.block_rank();
+  __shared__ int s_abort, s_rank[16];   // ranks in use of each 16 columns
+  cluster_arrive_relaxed();
+  const int cs = (int)cluster_size(), cr = (int)cluster_rank();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // the groups of columns of a tile after one another: x comes from memory once
   const int unit = blockIdx.x / cs, group = unit % groups;
@@ -88,6 +87,10 @@ __global__ void __launch_bounds__(128) shrink_block_kernel(const __grid_constant
   if (warp == 0) {
     tmem_alloc(smem_u32(&s_tmem), ncols);
     tmem_relinquish();
+  }
+  if (tid >= 64 && tid < 64 + nb / 16) {
+    const int col = col0 + (tid - 64) * 16;
+    s_rank[tid - 64] = col < p.SR ? p.ranks[tile.x * p.parts + col / p.R] - col % p.R : 0;
   }
   if (tid == 0) {
     s_abort = 0;
@@ -142,8 +145,14 @@ __global__ void __launch_bounds__(128) shrink_block_kernel(const __grid_constant
   // thread = row (tensor memory lane); the sums of a part past its slot's rank are exact zeros
   const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
   const float nanv = __int_as_float(0x7fc00000);
-  float* part = reinterpret_cast<float*>(raw_smem + (base - smem_u32(raw_smem)));   // [128][nb + 4]
-  const int ld = nb + 4;
+  // [cs][128 / cs][nb + 4], behind the ring: the cluster's sums of this CTA's share of the rows
+  float* const got = reinterpret_cast<float*>(raw_smem + (base - smem_u32(raw_smem)) + stages * sbytes);
+  const int ld = nb + 4, share = M / cs;
+  uint32_t to = 0;
+  if (cs > 1) {
+    cluster_started();
+    to = in_cta(got + (cr * share + tid % share) * ld, tid / share);
+  }
   for (int c = 0; c < nb; c += 16) {
     float v[16];
     if (mine > 0) {
@@ -152,14 +161,15 @@ __global__ void __launch_bounds__(128) shrink_block_kernel(const __grid_constant
 #pragma unroll
       for (int e = 0; e < 16; ++e) v[e] = 0.f;
     }
-    const int col = col0 + c;
-    const int rank = col < p.SR ? p.ranks[tile.x * p.parts + col / p.R] - col % p.R : 0;   // in use of these 16
+    const int col = col0 + c, rank = s_rank[c / 16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = !ok ? nanv : e < rank ? v[e] : 0.f;
     if (cs > 1) {
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
-        *reinterpret_cast<float4*>(part + tid * ld + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + 4 * (c + e)), "f"(v[e]), "f"(v[e + 1]),
+                     "f"(v[e + 2]), "f"(v[e + 3])
+                     : "memory");
     } else if (tid < tile.z && col < p.SR) {
       float4* o = reinterpret_cast<float4*>(p.t + (int64_t)(tile.y + tid) * p.SR + col);
 #pragma unroll
@@ -167,19 +177,17 @@ __global__ void __launch_bounds__(128) shrink_block_kernel(const __grid_constant
     }
   }
   if (cs > 1) {
-    cl.sync();
-    const int quads = M * nb / 4;
-    for (int q = cr * 128 + tid; q < quads; q += cs * 128) {
+    cluster_pushed();
+    for (int q = tid; q < share * nb / 4; q += 128) {
       const int r = q / (nb / 4), c = q % (nb / 4) * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = 0; k < cs; ++k) {
-        const float4 w = *reinterpret_cast<const float4*>(cl.map_shared_rank(part, k) + r * ld + c);
+      float4 v = *reinterpret_cast<const float4*>(got + r * ld + c);
+      for (int k = 1; k < cs; ++k) {
+        const float4 w = *reinterpret_cast<const float4*>(got + (k * share + r) * ld + c);
         v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
       }
-      if (r < tile.z && col0 + c < p.SR)
-        *reinterpret_cast<float4*>(p.t + (int64_t)(tile.y + r) * p.SR + col0 + c) = v;
+      if (cr * share + r < tile.z && col0 + c < p.SR)
+        *reinterpret_cast<float4*>(p.t + (int64_t)(tile.y + cr * share + r) * p.SR + col0 + c) = v;
     }
-    cl.sync();   // no CTA leaves while its shared memory may be read
   }
   tc_fence_before();
   __syncthreads();
@@ -605,17 +613,19 @@ static int rows_map(CUtensorMap* m, const void* ptr, int dtype, int64_t rows, in
 
 int shrink_block_launch(const Params& p, int dtype, int tiles, cudaStream_t st) {
   Cfg c;
-  c.groups = (p.SR + 255) / 256;
-  c.nb = ((p.SR + c.groups - 1) / c.groups + 15) / 16 * 16;
-  const int sbytes = XBYTES + c.nb * KB * 2;
-  c.stages = 110 * 1024 / sbytes;          // two CTAs an SM: 2 (256 columns) to 6
-  if (c.stages > MAXSTAGES) c.stages = MAXSTAGES;
-  // the cluster's CTAs split k until the grid fills the SMs, with at least four steps each
+  // The cluster's CTAs split k while the grid takes three quarters of the SMs at most (clusters
+  // of eight SMs do not fill every GPC), with at least four steps each; then a CTA has an SM to
+  // itself.  Else two an SM, and all columns in one group up to 256: x is read once (rank 64 in
+  // three parts: 77 us against 109 in two groups).
   c.cs = 1;
-  while (c.cs < 8 && (int64_t)tiles * c.groups * c.cs * 2 <= 2 * 148 && p.K >= 4 * KB * 2 * c.cs) c.cs *= 2;
-  const size_t sums = c.cs > 1 ? (size_t)M * (c.nb + 4) * 4 : 0;
-  c.smem = (size_t)c.stages * sbytes;
-  c.smem = (c.smem > sums ? c.smem : sums) + 1024;
+  while (c.cs < 8 && (int64_t)tiles * ((p.SR + 127) / 128) * c.cs * 8 <= 3 * num_sms() && p.K >= 4 * KB * 2 * c.cs) c.cs *= 2;
+  const int widest = c.cs > 1 ? 128 : 256;
+  c.groups = (p.SR + widest - 1) / widest;
+  c.nb = ((p.SR + c.groups - 1) / c.groups + 15) / 16 * 16;
+  const int sbytes = XBYTES + c.nb * KB * 2, got = c.cs > 1 ? M * (c.nb + 4) * 4 : 0;
+  c.stages = c.cs > 1 ? (220 * 1024 - got) / sbytes : 110 * 1024 / sbytes;   // 2 (256 columns) to 8
+  if (c.stages > MAXSTAGES) c.stages = MAXSTAGES;
+  c.smem = (size_t)c.stages * sbytes + got + 1024;
   CUtensorMap mx, ma;
   int rc = rows_map(&mx, p.x, dtype, p.rows, p.xs, p.K, KB, M, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == SPX_OK) rc = rows_map(&ma, p.a, dtype, (int64_t)p.slots * p.SR, p.K, p.K, KB, c.nb, CU_TENSOR_MAP_SWIZZLE_128B);
