@@ -613,12 +613,13 @@ static int rows_map(CUtensorMap* m, const void* ptr, int dtype, int64_t rows, in
 
 int shrink_block_launch(const Params& p, int dtype, int tiles, cudaStream_t st) {
   Cfg c;
-  // The cluster's CTAs split k while the grid takes three quarters of the SMs at most (clusters
-  // of eight SMs do not fill every GPC), with at least four steps each; then a CTA has an SM to
-  // itself.  Else two an SM, and all columns in one group up to 256: x is read once (rank 64 in
-  // three parts: 77 us against 109 in two groups).
+  // The cluster's CTAs split k until the grid fills the SMs, with at least four steps each; then
+  // a CTA has an SM to itself (and clusters of eight do not fill every GPC: 12 of them at most).
+  // Else two an SM, and all columns in one group up to 256: x is read once (rank 64 in three
+  // parts: 77 us against 109 in two groups).
   c.cs = 1;
-  while (c.cs < 8 && (int64_t)tiles * ((p.SR + 127) / 128) * c.cs * 8 <= 3 * num_sms() && p.K >= 4 * KB * 2 * c.cs) c.cs *= 2;
+  const int units = tiles * ((p.SR + 127) / 128);
+  while (c.cs < 8 && (int64_t)units * c.cs * 2 <= (c.cs < 4 ? num_sms() : 96) && p.K >= 4 * KB * 2 * c.cs) c.cs *= 2;
   const int widest = c.cs > 1 ? 128 : 256;
   c.groups = (p.SR + widest - 1) / widest;
   c.nb = ((p.SR + c.groups - 1) / c.groups + 15) / 16 * 16;
@@ -660,10 +661,18 @@ static int launch_expand_block(const Params& p, int dtype, int tiles, cudaStream
   ch.per_tile = ch.first[p.parts];
   ch.kw = p.R % 64 == 0 ? 64 : p.R % 32 == 0 ? 32 : 16;
   SPX_REQUIRE((int64_t)tiles * ch.per_tile <= 0x3fffffff, SPX_ERR_SHAPE, "spx_lora_add: too many rows");
-  // Four chunks (1 KB of a row) to a unit while every SM gets four units or more.
+  // Four chunks (1 KB of a row) to a unit; with few units an SM the size whose slowest CTA is
+  // done first, a change of unit (another A operand) counted as three quarters of a chunk:
+  // 8 x 512 rows of 4096 columns at rank 64 45 us with one chunk, 36 with eight.
   const int most = num_sms();
   ch.unit = 4;
-  while (ch.unit > 1 && (int64_t)tiles * ch.per_tile < (int64_t)4 * ch.unit * most) ch.unit /= 2;
+  if ((int64_t)tiles * ch.per_tile < (int64_t)64 * most) {
+    int best = 0x7fffffff;
+    for (int u = 1; u <= 16; u *= 2) {
+      const int units = tiles * ((ch.per_tile + u - 1) / u), cost = (units + most - 1) / most * (4 * (u < ch.per_tile ? u : ch.per_tile) + 3);
+      if (cost < best) best = cost, ch.unit = u;
+    }
+  }
   ch.units_per_tile = (ch.per_tile + ch.unit - 1) / ch.unit;
   ch.units = tiles * ch.units_per_tile;
   const int abufs = p.R <= 64 ? 2 : 1, sbytes = YBYTES + EC * p.R * 2, abytes = abufs * 2 * M * p.R * 2;
