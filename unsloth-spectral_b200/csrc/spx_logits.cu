@@ -337,9 +337,11 @@ int launch_tiles(const Params& p, int batch, cudaStream_t st) {
 
 template <typename T>
 int launch(const Params& p, int batch, cudaStream_t st) {
-  // One unit a lane while every unit of the batch has a lane of its own (32 warps an SM):
-  // 8 x 32768 bf16 5.4 us against 5.9 with four units; 128 x 131072 f32 51 us against 31.
-  if ((int64_t)batch * (p.V / Tile<T, 1>::N) <= 148 * 1024) return launch_tiles<T, 1>(p, batch, st);
+  // Loads that a lane has in flight: as many as its CTAs need for the row at once, at most four
+  // (128 x 131072 f32: 51 us with one, 31 with four).
+  const int cs = 4 * 148 / batch, row = (cs > 8 ? 8 : cs < 1 ? 1 : cs) * NT * Tile<T, 1>::N;
+  if (p.V <= row) return launch_tiles<T, 1>(p, batch, st);
+  if (p.V <= 2 * row) return launch_tiles<T, 2>(p, batch, st);
   return launch_tiles<T, 4>(p, batch, st);
 }
 
