@@ -135,6 +135,37 @@ def test_strided_rows_and_what_lies_between_them(dtype):
         pool.add(y[:, :3], wide[:, :3, 16:144], LoraBatch(ids))
 
 
+@pytest.mark.parametrize("B,T,K,W,parts", [(67, 386, 1576, 8000, 1), (40, 400, 1032, 1160, 3), (12, 1500, 520, 2440, 2)])
+def test_blocks_with_and_without_adapters_in_turn(B, T, K, W, parts):
+    """Blocks of rows where requests without an adapter, with one on some parts only and with
+    one everywhere follow one another, over odd numbers of column chunks: rows without are
+    copied, the others equal the kernels for few rows (whose order of sums differs: each within
+    the tolerance of the formula), and every run gives the same."""
+    from unsloth_spectral import LoraBatch
+    dt = torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(W)
+    widths = (W,) * parts
+    ranks = [tuple((8 if (s + p) % 3 else 0) for p in range(parts)) for s in range(6)]
+    pool, held = _adapters(g, 6, K, widths, ranks, dt)
+    ids = [i % 7 - 1 for i in range(B)]
+    assert B * T * (K + W * parts) * 16 >= 1 << 29
+    x = torch.randn(B, T, K, generator=g, device="cuda").to(dt)
+    y = torch.randn(B, T, W * parts, generator=g, device="cuda").to(dt)
+    batch = LoraBatch(ids)
+    first = pool.add(y, x, batch)
+    for _ in range(8):
+        assert torch.equal(pool.add(y, x, batch), first)
+    for b in range(B):
+        at = 0
+        for p, w in enumerate(widths):
+            if (ids[b], p) not in held:
+                assert torch.equal(first[b, :, at:at + w], y[b, :, at:at + w])
+            at += w
+    for b in (0, 1, 2, B // 2, B - 1):
+        ref, tol = _ref(y[b:b + 1], x[b:b + 1], held, ids[b:b + 1], widths)
+        _check(first[b:b + 1], ref, tol)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_large_and_small_values(dtype):
     """Inner products past float16's range and rows of tiny values keep their precision; an

@@ -11,6 +11,10 @@
 // terms in any order, so lane c of a quad takes k = 8c..8c+7 of 32 as the k of two
 // m16n8k16 steps (16-byte loads, whole sectors); the same choice over the output columns
 // gives 16-byte accesses of y and out.
+// These are the kernels for few rows of a slot; prompts take spx_lora_tc.cu's.  Bound by latency
+// and by the weights: one request on q|k|v at rank 16 takes 5.3 us (two launches, the second
+// one waiting for the first inside the GPU), 64 requests with 24 adapters of rank 64 and 32 at
+// K = 14336 17.7 us, of which 50 MB of weights need 7.6.
 // t is kept in float32; for the second product it is split into a high and a low value of
 // the row type (two MMAs), which keeps about 16 (bf16) or 22 (f16) bits of it.
 #include "spx_lora.cuh"

@@ -405,7 +405,10 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
     }
   } else if (warp == EWARPS + 1) {
     if (lane == 0) {
-      int i = 0, n = 0, v = -1, rank = 0, buf = 0;   // chunk, accumulators used, version
+      // Every chunk takes its turn at the accumulators, also one without an adapter (its barriers
+      // are then arrived at without an MMA): so a group of warps always has the same buffer, and
+      // the sums of chunk i being there means that the copies of every chunk up to i are.
+      int i = 0, v = -1, rank = 0, buf = 0;   // chunk, version of the A operand
       for (Walk w(p, ch); w.valid(ch); ++i, w.next(p, ch)) {
         if (w.fresh) {
           if (v >= 0) umma_commit(t_free0 + 8 * buf);   // once the MMAs that read it are done
@@ -414,10 +417,13 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
           if (!wait1(t_ready0 + 8 * buf, (uint32_t)((v / abufs) & 1), ab)) break;
           rank = versions[buf].rank;
         }
-        if (rank <= 0) continue;
-        const int s = i % stages, a = n & 1;
+        const int s = i % stages, a = i & 1;
         if (!wait1(full0 + 8 * s, (uint32_t)((i / stages) & 1), ab)) break;
-        if (n >= 2 && !wait1(acc_empty0 + 8 * a, (uint32_t)((n / 2 - 1) & 1), ab)) break;
+        if (i >= 2 && !wait1(acc_empty0 + 8 * a, (uint32_t)((i / 2 - 1) & 1), ab)) break;
+        if (rank <= 0) {
+          mbar_arrive(acc_full0 + 8 * a);
+          continue;
+        }
         tc_fence_after();
         const uint32_t bo = base + s * sbytes + YBYTES, ao = smem_u32(a_op) + buf * 512 * p.R;
         for (int ks = 0; ks * 16 < rank; ++ks) {
@@ -426,11 +432,10 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
           umma(tmem + a * EC, umma_desc(ao + ks * 4096, 2048, 128), bd, idesc, 1u);
         }
         umma_commit(acc_full0 + 8 * a);
-        ++n;
       }
-      if (n > 0) {   // the last MMAs are done before their tensor memory goes
+      if (i > 0) {   // the last MMAs are done before their tensor memory goes
         const uint64_t t0 = gtimer();
-        while (!mbar_try_wait_sleep(acc_full0 + 8 * ((n - 1) & 1), (uint32_t)(((n - 1) / 2) & 1)) && gtimer() - t0 < kWaitNs) {
+        while (!mbar_try_wait_sleep(acc_full0 + 8 * ((i - 1) & 1), (uint32_t)(((i - 1) / 2) & 1)) && gtimer() - t0 < kWaitNs) {
         }
       }
     }
@@ -486,7 +491,7 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
     // two groups of eight warps take the chunks in turn, so that the waits of one chunk (its sums,
     // its store) pass while the other is worked on
     const int quad = warp & 3, half = (warp >> 2) & 1, group = warp / EGROUP, r = quad * 32 + lane;
-    int i = 0, n = 0, v = -1;
+    int i = 0, v = -1;
     Version ver{};
     float s1 = 0.f;
     Walk w(p, ch);
@@ -502,26 +507,21 @@ __global__ void __launch_bounds__(ETHREADS) expand_block_kernel(const __grid_con
         if (lane == 0) mbar_arrive(t_free0 + 8 * buf);
       }
       const bool act = ver.rank > 0;
-      const int acc = n;
-      n += act;
       if ((i & 1) != group) continue;
-      const int a = acc & 1;
       if (!waitw(full0 + 8 * s, (uint32_t)((i / stages) & 1), ab)) break;
       uint8_t* const yrow = sm + s * sbytes + half * YBOX + r * 128;
       const int left = w.left - half * 64;   // columns of this half
       const bool tma_out = ver.rows >= quad * EROWS + EROWS && left >= 64;
-      if (act) {
-        if (!waitw(acc_full0 + 8 * a, (uint32_t)((acc / 2) & 1), ab)) break;
-        tc_fence_after();
-      }
+      if (!waitw(acc_full0 + 8 * group, (uint32_t)((i / 2) & 1), ab)) break;
+      tc_fence_after();
 #pragma unroll
       for (int hc = 0; hc < 2; ++hc) {
         float x[32];
-        if (act) tld32(tmem + ((uint32_t)(quad * 32) << 16) + a * EC + half * 64 + hc * 32, x);
-        if (hc == 1 && act) {
+        if (act) tld32(tmem + ((uint32_t)(quad * 32) << 16) + group * EC + half * 64 + hc * 32, x);
+        if (hc == 1) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty0 + 8 * a);
+          if (lane == 0) mbar_arrive(acc_empty0 + 8 * group);
         }
         if (!act && tma_out) continue;   // stored as it came
 #pragma unroll
