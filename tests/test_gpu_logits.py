@@ -120,6 +120,26 @@ def test_ties_nan_and_empty_rows(dtype, V):
     assert biased.pick(torch.zeros_like(x)).tolist() == [V - 1] * 6
 
 
+@pytest.mark.parametrize("V", [1000, 1003])
+def test_touched_tokens_at_minus_infinity(V):
+    """Seen and biased tokens that end at -inf (their logit, their bias, their mask) are chosen as
+    little as any other: token 0 when nothing is left, the only finite one when one is."""
+    from unsloth_spectral import LogitsRules
+    rules = LogitsRules(3, V, repetition_penalty=1.3, frequency_penalty=0.5,
+                        logit_bias=[{77: -float("inf")}, {77: -float("inf"), 500: 1.0}, {V - 1: -float("inf")}])
+    rules.observe(torch.tensor([[5, 900], [77, 900], [900, 900]], device="cuda"))
+    x = torch.full((3, V), -float("inf"), device="cuda")
+    x[:, 77] = 3.0
+    x[2, 900], x[2, 77] = -2.0, -float("inf")
+    allow = torch.zeros(3, V, dtype=torch.bool)
+    allow[:, [5, 77, 500, 900, V - 1]] = True
+    for mask in (None, _pack(allow, V).cuda()):
+        out, tok = rules.apply(x, allow=mask)
+        assert tok.tolist() == [0, 0, 900]
+        assert (out[:2] == -float("inf")).all() and int(out[2].isfinite().sum()) == 1
+        assert rules.pick(x, allow=mask).tolist() == [0, 0, 900]
+
+
 def test_record_counts_the_choice_and_reset_forgets():
     from unsloth_spectral import LogitsRules
     V = 97

@@ -21,7 +21,7 @@ namespace lgt {
 
 constexpr int NT = 256, WARPS = NT / 32;
 constexpr int BATCH = 3;     // listed tokens that a thread takes together
-constexpr int SEG = 16384;   // tokens of a CTA between two runs through its list (16 bits an entry)
+constexpr int SEG = 16384;   // tokens of a CTA between two runs through its list (16 bits an entry, 32 KB)
 
 __device__ __forceinline__ uint32_t cluster_dim() {
   uint32_t r;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(NT, 4) rules_kernel(const Params p) {
         // the biases lie by row and token: the first one of this word, then by the bits before this one
         if ((bw[q] >> sh) & 1u) f = __fadd_rn(f, p.bvals[bf[q] + __popc(bw[q] & ((1u << sh) - 1u))]);
         if (out) out[t[q]] = from_f<T>(f);
-        const unsigned long long other = key(f, t[q]);
+        const unsigned long long other = f == -INFINITY ? 0ull : key(f, t[q]);   // -inf: as if not there
         k = other > k ? other : k;
       }
     }
@@ -271,6 +271,7 @@ __global__ void __launch_bounds__(NT, 4) rules_kernel(const Params p) {
     const uint32_t at = mapa((uint32_t)__cvta_generic_to_shared(&tops[cr]), 0);
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(k) : "memory");
   }
+  __syncwarp();
   // every CTA's best lies with the first one, and every read of the history is done
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -310,13 +311,6 @@ int launch_tiles(const Params& p, int batch, cudaStream_t st) {
   cs = cs > 8 ? 8 : cs < 1 ? 1 : cs;
   const int64_t mine = (int64_t)((most + cs - 1) / cs) * ROUND;
   const size_t smem = p.touched ? 2 * (size_t)(mine < SEG ? mine : SEG) : 0;
-  if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(rules_kernel<T, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * SEG);
-    if (e != cudaSuccess) {
-      set_error("logits rules_kernel: %s", cudaGetErrorString(e));
-      return SPX_ERR_CUDA;
-    }
-  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(batch * cs));
   cfg.blockDim = dim3(NT);

@@ -192,7 +192,7 @@ class LoraAdapters:
         make = lambda w, out: LoraPool(w.shape[1], out, max_rank, slots, w.dtype, w.device)  # noqa: E731
         layers = model.model.layers
         for i, layer in enumerate(layers):
-            attn, mlp = layer.self_attn, layer.mlp
+            attn, mlp = layer.self_attn, getattr(layer, "mlp", None)
             if set(targets) & set(self.MLP) and not hasattr(mlp, "spx_lora"):
                 raise ValueError(f"layer {i}: {type(mlp).__name__} takes no adapters; leave {self.MLP} out of targets")
             held = {}
@@ -226,9 +226,13 @@ class LoraAdapters:
             if key not in self._pools:
                 raise KeyError(f"no adapted projection {key}; targets are {self.targets}")
         self.unload(slot)
-        for key, (A, B) in weights.items():
-            pool, part = self._pools[key]
-            pool.load(slot, A, B, scale, part)
+        try:
+            for key, (A, B) in weights.items():
+                pool, part = self._pools[key]
+                pool.load(slot, A, B, scale, part)
+        except Exception:
+            self.unload(slot)     # not half an adapter
+            raise
 
     def unload(self, slot: int):
         """Empty a slot."""
