@@ -283,14 +283,8 @@ __global__ void __launch_bounds__(EW * 32) expand_kernel(const Params p, const i
 template <typename T, int MT, int NT>
 int launch_shrink(const Params& p, int tiles, int groups, int cs, cudaStream_t st) {
   const size_t smem = Ring<MT, NT>::BYTES;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(shrink_kernel<T, MT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)smem);
-    if (e != cudaSuccess) {
-      set_error("lora shrink_kernel: %s", cudaGetErrorString(e));
-      return SPX_ERR_CUDA;
-    }
-  }
+  static std::atomic<int> have[64];
+  cudaError_t e = allow_smem(shrink_kernel<T, MT, NT>, (int)smem, have);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(tiles * cs), (unsigned)groups);
   cfg.blockDim = dim3(SW * 32);
@@ -301,7 +295,7 @@ int launch_shrink(const Params& p, int tiles, int groups, int cs, cudaStream_t s
   at[0].val.clusterDim.x = (unsigned)cs, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, shrink_kernel<T, MT, NT>, p);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, shrink_kernel<T, MT, NT>, p);
   if (e != cudaSuccess) {
     set_error("lora shrink_kernel: %s", cudaGetErrorString(e));
     return SPX_ERR_CUDA;
@@ -317,18 +311,14 @@ int launch_expand(const Params& p, int tiles, int tile_rows, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(tiles * cblocks));
   cfg.blockDim = dim3(EW * 32);
-  cfg.dynamicSmemBytes = (size_t)tile_rows / 16 * KS * 1024 + tile_rows * sizeof(float);
+  cfg.dynamicSmemBytes = (size_t)tile_rows / 16 * KS * 1024 + tile_rows * sizeof(float);   // up to 16.1 KB
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaSuccess;
-  if (cfg.dynamicSmemBytes > 48 * 1024)
-    e = cudaFuncSetAttribute(expand_kernel<T, KS, NC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)cfg.dynamicSmemBytes);
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, expand_kernel<T, KS, NC>, p, cblocks);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, expand_kernel<T, KS, NC>, p, cblocks);
   if (e != cudaSuccess) {
     set_error("lora expand_kernel: %s", cudaGetErrorString(e));
     return SPX_ERR_CUDA;

@@ -2,6 +2,8 @@
 #pragma once
 #include <math.h>
 
+#include <atomic>
+
 #include "spx_common.cuh"
 
 namespace spx {
@@ -45,6 +47,19 @@ __device__ __forceinline__ uint32_t pack2(__half lo, __half hi) {
 }
 __device__ __forceinline__ uint32_t pack2(__nv_bfloat16 lo, __nv_bfloat16 hi) {
   return (uint32_t)__bfloat16_as_ushort(lo) | ((uint32_t)__bfloat16_as_ushort(hi) << 16);
+}
+
+// Lets a kernel have `bytes` of dynamic shared memory (asked for once for a device and size: the
+// call takes about 1 us of a launch).  `have`: what each device allows so far, one array a kernel.
+template <typename F>
+inline cudaError_t allow_smem(F kernel, int bytes, std::atomic<int> (&have)[64]) {
+  int dev = 0;
+  const cudaError_t d = cudaGetDevice(&dev);
+  if (d != cudaSuccess) return d;
+  if (dev >= 0 && dev < 64 && have[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) have[dev].store(bytes, std::memory_order_relaxed);
+  return e;
 }
 
 // Cluster helpers: partial sums are pushed into the shared memory of the CTA that adds them up

@@ -633,7 +633,8 @@ int shrink_block_launch(const Params& p, int dtype, int tiles, cudaStream_t st) 
   if (rc != SPX_OK) return rc;
   const uint32_t fmt = dtype == SPX_F16 ? 0u : 1u;
   const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(c.nb >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-  cudaError_t e = cudaFuncSetAttribute(shrink_block_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)c.smem);
+  static std::atomic<int> have[64];
+  cudaError_t e = allow_smem(shrink_block_kernel, (int)c.smem, have);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(tiles * c.groups * c.cs));
@@ -700,7 +701,8 @@ static int launch_expand_block(const Params& p, int dtype, int tiles, cudaStream
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaFuncSetAttribute(expand_block_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<int> have[64];
+  cudaError_t e = allow_smem(expand_block_kernel<T>, (int)smem, have);
   if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, expand_block_kernel<T>, my, mb, mo, p, ch, stages, abufs, idesc);
   if (e != cudaSuccess) {
     set_error("lora expand_block_kernel: %s", cudaGetErrorString(e));
