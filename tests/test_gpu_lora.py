@@ -228,3 +228,24 @@ def test_streams_graphs_and_reloading():
     with torch.cuda.graph(torch.cuda.CUDAGraph()):
         with pytest.raises(RuntimeError):
             pool.add(ys[0], xs[0], fresh)
+
+
+def test_a_batch_dropped_while_another_stream_still_reads_it():
+    """Its grouping of rows is not handed out again before that stream is done."""
+    from unsloth_spectral import LoraBatch
+    g = torch.Generator(device="cuda").manual_seed(11)
+    pool, held = _adapters(g, 2, 128, (64,), [16, 16], torch.bfloat16)
+    x = torch.randn(3, 1, 128, generator=g, device="cuda").bfloat16()
+    y = torch.randn(3, 1, 64, generator=g, device="cuda").bfloat16()
+    ids = [1, -1, 0]
+    batch = LoraBatch(ids).prepare(1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)            # about 10 ms
+        out = pool.add(y, x, batch)
+    del batch
+    taken = [torch.zeros(n, dtype=torch.int32, device="cuda") for n in range(1, 40)]
+    torch.cuda.synchronize()
+    _check(out, *_ref(y, x, held, ids, (64,)))
+    assert len(taken) == 39

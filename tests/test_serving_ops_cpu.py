@@ -73,7 +73,7 @@ def _lora(**kw):
 @pytest.mark.parametrize("status,kw", [
     (0, dict(num_tiles=0, x=None)), (1, dict(x=None)), (1, dict(tiles=None)), (2, dict(in_features=60)),
     (2, dict(parts=0)), (2, dict(parts=5)), (2, dict(parts=3)), (2, dict(max_rank=24)), (2, dict(max_rank=144)),
-    (2, dict(tile_rows=8)), (2, dict(x_stride=56)), (2, dict(y_stride=88)), (3, dict(dtype=N.SPX_F32)), (4, dict(x=264)),
+    (2, dict(tile_rows=8)), (2, dict(slots=1 << 25)), (2, dict(x_stride=56)), (2, dict(y_stride=88)), (3, dict(dtype=N.SPX_F32)), (4, dict(x=264)),
     (4, dict(out_stride=100)), (5, dict(workspace=None)), (5, dict(workspace_bytes=20 * 32 * 4 + 15))])
 def test_lora_c_refusals(status, kw):
     lib = N.load()
@@ -201,3 +201,29 @@ def test_logits_python_refusals():
         r.pick(x.double())
     with pytest.raises(N.SpxUnavailable):
         r.pick(x)
+
+
+def test_out_over_another_place_of_the_input_is_refused():
+    """Rows of an out tensor that lie on the input's, but not on the same ones; rows side by side pass
+    (and are then refused for the device)."""
+    pool, b = LoraPool(16, 32, max_rank=4, slots=2, device="cpu"), LoraBatch([0, -1], device="cpu")
+    x = torch.zeros(2, 3, 16, dtype=torch.bfloat16)
+    wide = torch.zeros(2, 3, 64, dtype=torch.bfloat16)
+    flat = torch.zeros(12 * 32, dtype=torch.bfloat16)
+    rules = LogitsRules(4, 10, device="cpu")
+    room, line = torch.zeros(4, 24), torch.zeros(80)
+    cases = [(pool.add, wide[..., :32], dict(x=x, batch=b), wide[..., 8:40]),
+             (pool.add, flat[:192].view(2, 3, 32), dict(x=x, batch=b), flat[32:224].view(2, 3, 32)),
+             (pool.add, wide[..., :32], dict(x=x, batch=b), wide.view(-1)[:192].view(2, 3, 32)),
+             (pool.add, wide[:, :1, :32], dict(x=x[:, :1], batch=b), wide[:, :1, 24:56]),
+             (rules.apply, room[:, :10], {}, room[:, 9:19]),
+             (rules.apply, line[:40].view(4, 10), {}, line[10:50].view(4, 10)),
+             (rules.apply, room[:, 5:15], {}, room.view(-1)[:40].view(4, 10))]
+    for call, y, more, out in cases:
+        with pytest.raises(RuntimeError, match="overlaps"):
+            call(y, **more, out=out)
+    for call, y, more, out in ((pool.add, wide[..., :32], dict(x=x, batch=b), wide[..., 32:]),
+                               (pool.add, wide[..., :32], dict(x=x, batch=b), wide[..., :32]),
+                               (rules.apply, room[:, :10], {}, room[:, 10:20]), (rules.apply, room[:, :10], {}, room[:, :10])):
+        with pytest.raises(N.SpxUnavailable):
+            call(y, **more, out=out)

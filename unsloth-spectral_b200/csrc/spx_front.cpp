@@ -3,7 +3,6 @@
 // current stream and device, then the C call.  In Python, on ctypes, the same took 11 to 14 us
 // a call, of which the GPU needs 3 to 6; here it takes 5 to 8.  No CUDA code: the kernels are
 // libspx.so's, called through include/spx.h.
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -46,6 +45,20 @@ void launch(F fn, const A& args, const at::Device& d, const char* what) {
   c10::cuda::CUDAGuard guard(d);   // a launch goes to the current device
   const int rc = fn(&args, at::cuda::getCurrentCUDAStream(d.index()).stream());
   if (rc != SPX_OK) raise_status(rc, what);
+}
+
+// Rows of `width` values, `os` and `ys` apart: out may be y itself or lie beside it (also between
+// y's rows), but a row of it must not fall on another place of y, which is still to be read.
+void no_partial_overlap(const Tensor& out, int64_t os, const Tensor& y, int64_t ys, int64_t rows, int64_t width) {
+  const int64_t size = y.element_size(), d = (static_cast<const char*>(out.const_data_ptr()) -
+                                              static_cast<const char*>(y.const_data_ptr())) / size;
+  if (d >= (rows - 1) * ys + width || -d >= (rows - 1) * os + width) return;
+  bool fine = d == 0 && (rows == 1 || os == ys);
+  if (!fine && rows > 1 && os == ys && os > 0) {
+    const int64_t m = (d % os + os) % os;
+    fine = m >= width && os - m >= width;
+  }
+  TORCH_CHECK(fine, "out overlaps the input without being the same rows");
 }
 
 // A contiguous float32 [len, D] table on the device.
@@ -124,6 +137,13 @@ struct Batch {
   struct Plan {
     int tile_rows, tiles, rows;
     Tensor held;   // int32: tiles [n][4], then the order of rows
+    c10::Stream made;
+    // on another stream than the one it was made on: its memory is not given away, when the batch
+    // goes, before that stream's work is done (callers cannot record it, they never see it)
+    void use(const at::Device& d) const {
+      const auto now = at::cuda::getCurrentCUDAStream(d.index());
+      if (now.unwrap() != made) held.record_stream(now);
+    }
   };
   int64_t sequences, highest;
   at::Device device;
@@ -131,7 +151,9 @@ struct Batch {
 
   Batch(int64_t n, int64_t top, const at::Device& d) : sequences(n), highest(top), device(d) {}
   void put(int64_t tokens, bool blocks, int tile_rows, int tiles, int rows, Tensor held) {
-    plans[{tokens, blocks}] = Plan{tile_rows, tiles, rows, std::move(held)};
+    const c10::Stream made = held.is_cuda() ? at::cuda::getCurrentCUDAStream(held.get_device()).unwrap()
+                                            : c10::Stream(c10::Stream::DEFAULT, held.device());
+    plans.insert_or_assign({tokens, blocks}, Plan{tile_rows, tiles, rows, std::move(held), made});
   }
   bool has(int64_t tokens, bool blocks) const { return plans.count({tokens, blocks}) > 0; }
 };
@@ -175,10 +197,14 @@ struct Pool {
     TORCH_CHECK_VALUE(fits(x) && fits(y) && (!out_ || fits(*out_)), "x, y and out must be ", a.scalar_type(), " on ",
                       a.device());
     TORCH_CHECK_VALUE(batch.device == a.device(), "the batch is on ", batch.device, ", the pool on ", a.device());
-    require_device(a.device());
     const int64_t tokens = d == 3 ? x.size(1) : 1, rows = batch.sequences * tokens;
     TORCH_CHECK_VALUE(rows <= 1 << 30, rows, " rows in one call");
-    if (out_) at::assert_no_partial_overlap(*out_, y);
+    spx_lora_args v = args;
+    if (rows) {
+      v.x_stride = row_stride(x), v.y_stride = row_stride(y);
+      if (out_) no_partial_overlap(*out_, v.out_stride = row_stride(*out_), y, v.y_stride, rows, out);
+    }
+    require_device(a.device());
     if (rows == 0) return out_ ? *out_ : at::empty_like(y);
     // Prompts take the kernels for blocks of adjacent rows, whose start takes longer and whose
     // time does not grow with the rank.  They meet at about 30M values of x and y at rank 16 and
@@ -188,10 +214,9 @@ struct Pool {
     const auto plan = batch.plans.find({tokens, blocks});
     if (plan == batch.plans.end()) return std::make_pair(tokens, blocks);
     const Batch::Plan& p = plan->second;
-    spx_lora_args v = args;
-    v.x_stride = row_stride(x), v.y_stride = row_stride(y);
     Tensor o = out_ ? *out_ : at::empty(y.sizes(), y.options());
-    v.out_stride = row_stride(o);
+    if (!out_) v.out_stride = out;
+    p.use(a.device());
     v.num_tiles = p.tiles, v.tile_rows = p.tile_rows, v.num_rows = p.rows;
     v.tiles = p.held.const_data_ptr<int32_t>(), v.order = v.tiles + 4 * (int64_t)p.tiles;
     // the inner products, a buffer of each call's own: two streams or two captured graphs never
@@ -250,7 +275,7 @@ struct Rules {
       v.allow = reinterpret_cast<const uint32_t*>(allow->const_data_ptr<int32_t>());
       v.allow_stride = rows > 1 ? allow->stride(0) : 0;
     }
-    if (out) at::assert_no_partial_overlap(*out, logits);
+    if (out) no_partial_overlap(*out, out->stride(0), logits, logits.stride(0), args.batch, args.vocab);
     require_device(device);
     Tensor token = at::empty({args.batch}, logits.options().dtype(at::kLong));
     v.record = record, v.logits = logits.const_data_ptr(), v.logits_stride = logits.stride(0);

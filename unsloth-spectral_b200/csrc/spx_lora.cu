@@ -331,7 +331,7 @@ int launch_shrink_rows(const Params& p, int tiles, int tile_rows, cudaStream_t s
   // Columns of a CTA: 16 while two CTAs an SM hold the whole grid (one request on q|k|v 5.6 us
   // against 6.8 with 48), else as many as leave the rows enough warps: each group reads x again.
   const int cols = (int64_t)tiles * (p.SR / 16) * 8 <= 2 * 148 ? 16 : tile_rows == 16 ? 32 : 64;
-  const int groups = (p.SR + cols - 1) / cols;                 
+  const int groups = (p.SR + cols - 1) / cols;
   const int nt = ((p.SR / 8 + groups - 1) / groups + 1) / 2 * 2;  // 2, 4, 6 or 8
   // CTAs that share a tile's k: until three CTAs an SM hold the grid, with at least two steps of
   // 32 for each warp, 8 at most (the portable cluster size).
@@ -391,6 +391,9 @@ static int validate(const spx_lora_args* a) {
                 "spx_lora_add: width %d of part %d must be a multiple of 8", a->part_width[s], s);
     out += a->part_width[s];
   }
+  // the rows of A and B are counted in 32 bits (the coordinates of a copy's box)
+  SPX_REQUIRE(a->slots * (out > a->parts * a->max_rank ? out : (int64_t)a->parts * a->max_rank) <= 0x7fffffff, SPX_ERR_SHAPE,
+              "spx_lora_add: %d slots of %lld columns are too many", a->slots, (long long)out);
   if (a->num_tiles == 0) return SPX_OK;
   SPX_REQUIRE(a->x && a->y && a->out && a->a && a->b && a->ranks && a->scales && a->tiles && a->order, SPX_ERR_NULL,
               "spx_lora_add: every pointer is required");

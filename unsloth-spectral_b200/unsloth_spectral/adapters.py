@@ -27,7 +27,8 @@ from . import _native as N
 class LoraBatch:
     """The adapter slot of each sequence of a batch (-1: none), as host integers.  The rows
     are grouped by slot once, on first use for a number of tokens per sequence, and kept on
-    ``device``; build the batch before capturing a CUDA graph that uses it (``prepare``)."""
+    ``device``; build the batch before capturing a CUDA graph that uses it (``prepare``) and
+    keep it as long as the graph is replayed."""
 
     def __init__(self, slots: Sequence[int], device="cuda"):
         self.slots: Tuple[int, ...] = tuple(int(s) for s in slots)
@@ -144,7 +145,8 @@ class LoraPool:
     def add(self, y: torch.Tensor, x: torch.Tensor, batch: LoraBatch, out=None) -> torch.Tensor:
         """``y + scale * B (A x)`` of each sequence's slot.  ``x [B, T, in]`` (or ``[B, in]``:
         one token each) and ``y [B, T, out]`` in the pool's dtype, rows on 16 bytes and evenly
-        spaced; ``out`` may be ``y`` itself (in place), else a new tensor is returned."""
+        spaced; ``out`` may be ``y`` itself (in place) or lie beside it, without it a new tensor is
+        returned."""
         r = self._add(y, x, batch._front, out)
         if type(r) is tuple:      # (tokens, blocks): a grouping of rows that the batch has not made yet
             batch._plan(*r)
