@@ -249,3 +249,32 @@ def test_a_batch_dropped_while_another_stream_still_reads_it():
     torch.cuda.synchronize()
     _check(out, *_ref(y, x, held, ids, (64,)))
     assert len(taken) == 39
+
+
+def test_a_new_batch_does_not_wait_for_the_gpu_and_is_there_for_streams_and_graphs():
+    from unsloth_spectral import LoraBatch
+    g = torch.Generator(device="cuda").manual_seed(12)
+    pool, held = _adapters(g, 2, 128, (64,), [16, 16], torch.float16)
+    x = torch.randn(3, 1, 128, generator=g, device="cuda").half()
+    y = torch.randn(3, 1, 64, generator=g, device="cuda").half()
+    ids = [1, -1, 0]
+    pool.add(y, x, LoraBatch(ids))               # the host memory of its copy is there from now on
+    torch.cuda.synchronize()
+    first, side = LoraBatch(ids), torch.cuda.Stream()
+    busy = torch.cuda.Event()
+    torch.cuda._sleep(100_000_000)               # about 50 ms
+    busy.record()
+    outs = [pool.add(y, x, first)]
+    assert not busy.query()
+    with torch.cuda.stream(side):                # x and y have been there since before the sleep
+        outs.append(pool.add(y, x, first))
+    second = LoraBatch(ids)
+    outs.append(pool.add(y, x, second))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs.append(pool.add(y, x, second))
+    graph.replay()
+    torch.cuda.synchronize()
+    ref = _ref(y, x, held, ids, (64,))
+    for o in outs:
+        _check(o, *ref)

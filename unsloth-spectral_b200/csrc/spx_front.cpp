@@ -4,14 +4,18 @@
 // a call, of which the GPU needs 3 to 6; here it takes 4 to 7.5.  No CUDA code: the kernels are
 // libspx.so's, called through include/spx.h.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAEvent.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <map>
+#include <numeric>
 #include <optional>
-#include <sstream>
+#include <vector>
 
 #include "spx.h"
 
@@ -139,30 +143,111 @@ std::pair<Tensor, OptTensor> qk_norm_rope(Tensor q, OptTensor k, Tensor qw, cons
 }
 
 // ---------------------------------------------------------------------- adapters ----
-// Which rows use which slot: the plans of a LoraBatch, by tokens per sequence.
+constexpr int64_t kBlockTokens = 64;   // tokens of a sequence from which on its rows may be taken as blocks
+
+bool capturing() {   // the current stream, into a graph
+  return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+}
+
+// Rows grouped by slot, cut into tiles of one slot: int32 tiles [n][4], then the order of rows.
+// Tiles of 16 rows of any sequences, or 32 where a slot has more, which reads the adapter's weights
+// half as often; or blocks of up to 128 tokens of one sequence, which name their first row
+// themselves (no order).
+struct Grouping {
+  int tile_rows = 16, tiles = 0;
+  std::vector<int32_t> held;
+};
+
+Grouping group_rows(const std::vector<int32_t>& slots, int64_t tokens, bool blocks) {
+  const int n = (int)slots.size(), T = (int)tokens;
+  std::vector<int32_t> seqs(n);
+  std::iota(seqs.begin(), seqs.end(), 0);
+  std::stable_sort(seqs.begin(), seqs.end(), [&](int a, int b) { return slots[a] < slots[b]; });
+  Grouping g;
+  const auto put = [&](int slot, int first, int rows, int row0) {
+    g.held.insert(g.held.end(), {slot, first, rows, row0});
+    ++g.tiles;
+  };
+  if (blocks) {
+    g.tile_rows = 128;
+    for (int i = 0; i < n; ++i)
+      for (int t = 0; t < T; t += 128) put(slots[seqs[i]], i * T + t, std::min(128, T - t), seqs[i] * T + t);
+    return g;
+  }
+  std::vector<std::pair<int, int>> runs;   // sequences of one slot: from, to
+  for (int i = 0; i < n; ++i) {
+    if (!i || slots[seqs[i]] != slots[seqs[i - 1]]) runs.emplace_back(i, i);
+    ++runs.back().second;
+  }
+  for (const auto& r : runs)
+    if ((r.second - r.first) * (int64_t)T > 16) g.tile_rows = 32;
+  for (const auto& r : runs)
+    for (int at = r.first * T; at < r.second * T; at += g.tile_rows)
+      put(slots[seqs[r.first]], at, std::min(g.tile_rows, r.second * T - at), 0);
+  for (int i = 0; i < n; ++i)
+    for (int t = 0; t < T; ++t) g.held.push_back(seqs[i] * T + t);
+  return g;
+}
+
+// Which rows use which slot: the groupings of a LoraBatch, by tokens per sequence.
 struct Batch {
   struct Plan {
     int tile_rows, tiles, rows;
-    Tensor held;   // int32: tiles [n][4], then the order of rows
+    Tensor held;
     c10::Stream made;
-    // on another stream than the one it was made on: its memory is not given away, when the batch
-    // goes, before that stream's work is done (callers cannot record it, they never see it)
-    void use(const at::Device& d) const {
-      const auto now = at::cuda::getCurrentCUDAStream(d.index());
-      if (now.unwrap() != made) held.record_stream(now);
+    at::cuda::CUDAEvent copied;
+    bool there = false;   // the copy to the device is known to be done
+
+    // Before a launch.  The copy was queued without waiting for it (a new batch does not hold up
+    // the host): work on the stream that it was queued on follows it anyway; other streams, and
+    // graphs, whose replays follow nothing, wait for it here, once.  On another stream the memory is
+    // also kept until that stream's work is done (callers cannot record it, they never see it).
+    void use(const at::cuda::CUDAStream& now) {
+      const bool other = now.unwrap() != made;
+      if (other) held.record_stream(now);
+      if (there) return;
+      const bool wait = other || capturing();
+      const c10::cuda::CUDAStreamCaptureModeGuard allowed(cudaStreamCaptureModeRelaxed);
+      if (wait) copied.synchronize();
+      there = wait || copied.query();
     }
   };
+  std::vector<int32_t> slots;
   int64_t sequences, highest;
   at::Device device;
   std::map<std::pair<int64_t, bool>, Plan> plans;
 
-  Batch(int64_t n, int64_t top, const at::Device& d) : sequences(n), highest(top), device(d) {}
-  void put(int64_t tokens, bool blocks, int tile_rows, int tiles, int rows, Tensor held) {
-    const c10::Stream made = held.is_cuda() ? at::cuda::getCurrentCUDAStream(held.get_device()).unwrap()
-                                            : c10::Stream(c10::Stream::DEFAULT, held.device());
-    plans.insert_or_assign({tokens, blocks}, Plan{tile_rows, tiles, rows, std::move(held), made});
+  Batch(std::vector<int32_t> s, const at::Device& d) : slots(std::move(s)), sequences((int64_t)slots.size()), highest(-1), device(d) {
+    for (const int32_t v : slots) highest = std::max<int64_t>(highest, v);
   }
-  bool has(int64_t tokens, bool blocks) const { return plans.count({tokens, blocks}) > 0; }
+
+  Plan& plan(int64_t tokens, bool blocks) {
+    const auto found = plans.find({tokens, blocks});
+    if (found != plans.end()) return found->second;
+    TORCH_CHECK_VALUE(tokens >= 0 && tokens <= 1 << 30 && sequences * tokens <= 1 << 30, sequences, " x ", tokens, " rows in one call");
+    require_device(device);
+    const c10::cuda::CUDAGuard guard(device);
+    const auto now = at::cuda::getCurrentCUDAStream(device.index());
+    TORCH_CHECK(!capturing(), "call LoraBatch.prepare(", tokens, ") before capturing a graph that uses the batch");
+    const Grouping g = group_rows(slots, tokens, blocks);
+    const int64_t n = (int64_t)g.held.size();
+    Plan p{g.tile_rows, g.tiles, (int)(sequences * tokens), fresh({n}, at::kInt, device), now.unwrap()};
+    if (n) {
+      const Tensor host = at::empty({n}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
+      std::copy(g.held.begin(), g.held.end(), host.mutable_data_ptr<int32_t>());
+      p.held.copy_(host, true);
+    }
+    p.copied.record(now);
+    return plans.emplace(std::make_pair(tokens, blocks), std::move(p)).first->second;
+  }
+  void prepare(int64_t tokens) {
+    for (const bool blocks : {false, true})
+      if (!blocks || tokens >= kBlockTokens) {
+        Plan& p = plan(tokens, blocks);
+        p.copied.synchronize();
+        p.there = true;
+      }
+  }
 };
 
 // The distance between the rows of t [.., n], which must be even.
@@ -189,9 +274,7 @@ struct Pool {
     args.ranks = ranks.const_data_ptr<int32_t>(), args.scales = scales.const_data_ptr<float>();
   }
 
-  // y + scale * B (A x); none when the batch has no plan for these tokens yet: (tokens, blocks).
-  std::variant<Tensor, std::pair<int64_t, bool>> add(const Tensor& y, const Tensor& x, const Batch& batch,
-                                                     const OptTensor& out_) const {
+  Tensor add(const Tensor& y, const Tensor& x, Batch& batch, const OptTensor& out_) const {
     const int64_t d = x.dim();
     TORCH_CHECK_VALUE((d == 2 || d == 3) && y.dim() == d && x.size(-1) == in && y.size(-1) == out && x.size(0) == y.size(0) &&
                           (d == 2 || x.size(1) == y.size(1)) && x.size(0) == batch.sequences,
@@ -217,18 +300,16 @@ struct Pool {
     // time does not grow with the rank.  They meet at about 30M values of x and y at rank 16 and
     // 32 (4096 -> 6144 columns at rank 16: 2048 rows 24 us against 27, 4096 rows 45 against 42,
     // 16384 rows 162 against 109) and 8M at rank 64 (4096 -> 4096: 1024 rows 31 against 23).
-    const bool blocks = tokens >= 64 && rows * (in + out) * args.max_rank >= (int64_t)1 << 29;
-    const auto plan = batch.plans.find({tokens, blocks});
-    if (plan == batch.plans.end()) return std::make_pair(tokens, blocks);
-    const Batch::Plan& p = plan->second;
+    const bool blocks = tokens >= kBlockTokens && rows * (in + out) * args.max_rank >= (int64_t)1 << 29;
+    const c10::cuda::CUDAGuard guard(a.device());
+    Batch::Plan& p = batch.plan(tokens, blocks);
+    p.use(at::cuda::getCurrentCUDAStream(a.device().index()));
     Tensor o = out_ ? *out_ : fresh(y.sizes(), y.scalar_type(), a.device());
     if (!out_) v.out_stride = out;
-    p.use(a.device());
     v.num_tiles = p.tiles, v.tile_rows = p.tile_rows, v.num_rows = p.rows;
     v.tiles = p.held.const_data_ptr<int32_t>(), v.order = v.tiles + 4 * (int64_t)p.tiles;
     // the inner products, a buffer of each call's own: two streams or two captured graphs never
     // share one (the caching allocator hands it out in stream order)
-    const c10::cuda::CUDAGuard guard(a.device());
     v.workspace_bytes = ((size_t)p.rows * args.parts * args.max_rank + 4) * sizeof(float);
     const at::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate(v.workspace_bytes);
     v.workspace = static_cast<float*>(ws.get());
@@ -309,9 +390,13 @@ struct Rules {
 PYBIND11_MODULE(_spx_front, m) {
   m.def("qk_norm_rope", &qk_norm_rope);
   py::class_<Batch>(m, "Batch")
-      .def(py::init<int64_t, int64_t, const at::Device&>())
-      .def("put", &Batch::put)
-      .def("has", &Batch::has);
+      .def(py::init<std::vector<int32_t>, const at::Device&>())
+      .def_readonly("highest", &Batch::highest)
+      .def("prepare", &Batch::prepare);
+  m.def("group_rows", [](const std::vector<int32_t>& slots, int64_t tokens, bool blocks) {
+    const Grouping g = group_rows(slots, tokens, blocks);
+    return std::make_tuple(g.tile_rows, g.tiles, g.held);
+  });
   py::class_<Pool>(m, "Pool")
       .def(py::init<Tensor, Tensor, Tensor, Tensor, const std::vector<int>&>())
       .def("add", &Pool::add);

@@ -26,8 +26,8 @@ from . import _native as N
 
 class LoraBatch:
     """The adapter slot of each sequence of a batch (-1: none), as host integers.  The rows
-    are grouped by slot once, on first use for a number of tokens per sequence, and kept on
-    ``device``; build the batch before capturing a CUDA graph that uses it (``prepare``) and
+    are grouped by slot once, on first use for a number of tokens per sequence (the host does
+    not wait for the GPU), and kept on ``device``; build the batch before capturing a CUDA graph that uses it (``prepare``) and
     keep it as long as the graph is replayed."""
 
     def __init__(self, slots: Sequence[int], device="cuda"):
@@ -38,51 +38,26 @@ class LoraBatch:
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        self._front = N.front().Batch(len(self.slots), self.highest, self.device)
+        self._front = N.front().Batch(self.slots, self.device)
+        self.highest = self._front.highest
 
     def __len__(self) -> int:
         return len(self.slots)
 
     def prepare(self, tokens: int = 1) -> "LoraBatch":
-        """Group the rows of ``tokens`` tokens per sequence now."""
-        for blocks in (False, True)[:1 + (tokens >= 64)]:
-            self._plan(tokens, blocks)
+        """Group the rows of ``tokens`` tokens per sequence now, and wait until the grouping is on
+        the device."""
+        self._front.prepare(tokens)
         return self
 
     @staticmethod
     def tiles_of(slots: Sequence[int], tokens: int, blocks: bool = False):
         """Host arrays ``(tile_rows, tiles [n, 4], order)``: rows sorted by slot, cut into tiles of
-        one slot: 16 rows of any sequences, or 32 where a slot has more, which reads the
-        adapter's weights half as often; or ``blocks`` of up to 128 tokens of one sequence,
-        which name their first row themselves (``order`` is empty)."""
-        ids = np.asarray(slots, dtype=np.int32)
-        seqs = np.argsort(ids, kind="stable").astype(np.int32)
-        n = len(ids) * tokens
-        if blocks:
-            cut = np.arange(0, tokens, 128, dtype=np.int32)
-            row0 = (seqs[:, None] * np.int32(tokens) + cut).reshape(-1)
-            rows = np.tile(np.minimum(128, tokens - cut), len(ids))
-            first = (np.arange(len(ids), dtype=np.int32)[:, None] * np.int32(tokens) + cut).reshape(-1)
-            tiles = np.stack([np.repeat(ids[seqs], len(cut)), first, rows, row0], 1)
-            return 128, tiles.astype(np.int32), np.empty(0, np.int32)
-        order = (seqs[:, None] * np.int32(tokens) + np.arange(tokens, dtype=np.int32)).reshape(-1)
-        used, counts = np.unique(ids, return_counts=True)
-        counts = counts * tokens
-        tile_rows = 16 if n == 0 or counts.max() <= 16 else 32
-        tiles, at = [], 0
-        for s, m in zip(used.tolist(), counts.tolist()):
-            tiles += [(s, at + i, min(tile_rows, m - i), 0) for i in range(0, m, tile_rows)]
-            at += m
-        return tile_rows, np.asarray(tiles, dtype=np.int32).reshape(-1, 4), order
-
-    def _plan(self, tokens: int, blocks: bool):
-        if self._front.has(tokens, blocks):
-            return
-        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError(f"call LoraBatch.prepare({tokens}) before capturing a graph that uses the batch")
-        tile_rows, tiles, order = self.tiles_of(self.slots, tokens, blocks)
-        held = torch.from_numpy(np.concatenate([tiles.reshape(-1), order])).to(self.device)
-        self._front.put(tokens, blocks, tile_rows, len(tiles), len(self.slots) * tokens, held)
+        one slot: 16 rows of any sequences, or 32 where a slot has more; or ``blocks`` of up to 128
+        tokens of one sequence, which name their first row themselves (``order`` is empty)."""
+        tile_rows, n, held = N.front().group_rows(list(slots), tokens, blocks)
+        held = np.asarray(held, dtype=np.int32)
+        return tile_rows, held[:4 * n].reshape(n, 4), held[4 * n:]
 
 
 class LoraPool:
@@ -147,11 +122,7 @@ class LoraPool:
         one token each) and ``y [B, T, out]`` in the pool's dtype, rows on 16 bytes and evenly
         spaced; ``out`` may be ``y`` itself (in place) or lie beside it, without it a new tensor is
         returned."""
-        r = self._add(y, x, batch._front, out)
-        if type(r) is tuple:      # (tokens, blocks): a grouping of rows that the batch has not made yet
-            batch._plan(*r)
-            r = self._add(y, x, batch._front, out)
-        return r
+        return self._add(y, x, batch._front, out)
 
 
 def adapted(module, name: str, y: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
