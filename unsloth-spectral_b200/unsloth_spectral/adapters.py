@@ -27,14 +27,13 @@ from . import _native as N
 class LoraBatch:
     """The adapter slot of each sequence of a batch (-1: none), as host integers.  The rows
     are grouped by slot once, on first use for a number of tokens per sequence (the host does
-    not wait for the GPU), and kept on ``device``; build the batch before capturing a CUDA graph that uses it (``prepare``) and
-    keep it as long as the graph is replayed."""
+    not wait for the GPU), and kept on ``device``; ``prepare`` the batch before capturing a CUDA
+    graph that uses it and keep it as long as the graph is replayed."""
 
     def __init__(self, slots: Sequence[int], device="cuda"):
         self.slots: Tuple[int, ...] = tuple(int(s) for s in slots)
         if any(s < -1 for s in self.slots):
             raise ValueError(f"a slot is -1 (none) or a pool's slot number, got {min(self.slots)}")
-        self.highest = max(self.slots, default=-1)
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
