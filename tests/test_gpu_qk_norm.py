@@ -48,7 +48,8 @@ def _check(got, ref, mag, dt):
 
 SHAPES = [(1, 1, 32, 8, 128), (3, 1, 32, 8, 128), (64, 1, 5, 1, 64), (2, 37, 9, 3, 80), (1, 700, 4, 4, 96), (2, 5, 2, 1, 256),
           (1, 3, 7, 2, 512), (2, 3, 3, 1, 1024), (2, 9, 3, 2, 2), (1, 4, 5, 5, 6), (2, 3, 4, 2, 16), (1, 11, 6, 2, 48),
-          (1, 2, 1, 1, 32), (300, 9, 3, 1, 128)]
+          (1, 2, 1, 1, 32), (300, 9, 3, 1, 128), (1, 33, 5, 2, 144), (3, 11, 4, 2, 160), (2, 301, 3, 1, 112),
+          (8, 2049, 5, 2, 80), (3, 4001, 3, 1, 96), (2, 2400, 13, 3, 64)]
 
 
 @pytest.mark.parametrize("dtype", DT)

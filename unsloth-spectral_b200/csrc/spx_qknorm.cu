@@ -5,7 +5,7 @@
 // norm's output never exists in the row type, so nothing is lost between it and the
 // rotation).  Bound by memory: each value is read once and written once; the tables' rows
 // come from L2 and are held in registers over the heads of a token.
-// What it takes is warps: 8 x 4096 tokens of 32/8 heads of 128 bf16 take 116 us (floor 103)
+// What it takes is warps: 8 x 4096 tokens of 32/8 heads of 128 bf16 take 115 us (floor 103)
 // with 32 warps an SM and the next vector fetched ahead; 155 with four vectors at once and 16
 // warps, 126 without fetching ahead; narrower lanes (four values of a half) 150; more warps
 // than the registers allow without spills 150 to 230.
@@ -16,7 +16,12 @@
 namespace spx {
 namespace qkn {
 
-constexpr int WARPS = 8;
+// Warps of a CTA.  Small ones: where the grid is about one wave, what counts is the SM that got the
+// most (8 x 2048 rows of 12 heads of 128: bf16 21.4 us with eight warps, 20.0 with four; float32
+// 42.9 with eight, 42.1 with four, 41.3 with two).
+template <typename T>
+constexpr int kWarps = sizeof(T) == 4 ? 2 : 4;
+constexpr int ANY_WARPS = 8;
 
 struct Params {
   const void *q, *k, *qw, *kw;
@@ -53,6 +58,25 @@ struct Raw {
   }
 };
 
+// The sum of ss over the G lanes of a group, the same in all of them.
+template <int G>
+__device__ __forceinline__ float group_sum(float ss, unsigned mask) {
+  if ((G & (G - 1)) == 0) {
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+    return ss;
+  }
+  constexpr int P = G <= 2 ? 2 : G <= 4 ? 4 : G <= 8 ? 8 : G <= 16 ? 16 : 32;
+  const int lane = threadIdx.x & 31, l = lane % G, base = lane - l;
+#pragma unroll
+  for (int o = P / 2; o; o >>= 1) {   // complete in the first lane; the missing lanes are zeros
+    const bool there = (l ^ o) < G;
+    const float v = __shfl_sync(mask, ss, there ? base + (l ^ o) : lane);
+    ss += there ? v : 0.f;
+  }
+  return __shfl_sync(mask, ss, base);
+}
+
 // G lanes hold one head vector: lane l its values Nl..Nl+N-1 of both halves, so that the two
 // values of a rotation meet in one lane and only the sum of squares crosses lanes.  The
 // table row is held in registers over the heads of a token; the weights are read from shared
@@ -81,8 +105,7 @@ __device__ __forceinline__ void heads(const T* src, T* dst, int64_t dst_h, const
         ss = fmaf(x2, x2, ss);
       }
     }
-#pragma unroll
-    for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+    ss = group_sum<G>(ss, mask);
     const float inv = rsqrtf(fmaf(ss, inv_d, eps));
     if (on) {
       Raw<T, N> wa, wb;
@@ -102,14 +125,16 @@ __device__ __forceinline__ void heads(const T* src, T* dst, int64_t dst_h, const
 }
 
 template <typename T, int N, int G>
-__global__ void __launch_bounds__(WARPS * 32, sizeof(T) == 4 ? 3 : 4) vec_kernel(const Params p) {
+__global__ void __launch_bounds__(kWarps<T> * 32, (sizeof(T) == 4 ? 24 : 32) / kWarps<T>) vec_kernel(const Params p) {
+  constexpr int WARPS = kWarps<T>;
   constexpr int NG = 32 / G;
   __shared__ __align__(16) T weights[2][2 * N * G];
   const int lane = threadIdx.x & 31, l = lane % G, h = p.D / 2;
-  const int64_t gi = ((int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5)) * NG + lane / G;
-  const bool live = gi < p.rows * p.slots;
-  const int64_t row = live ? gi / p.slots : 0, b = row / p.T, t = row - b * p.T;
-  const int g = (int)(gi - row * p.slots), step = p.slots;
+  const uint32_t gi = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * NG + lane / G;
+  const bool live = lane < NG * G && gi < (uint32_t)p.rows * p.slots;
+  const uint32_t row = live ? gi / (uint32_t)p.slots : 0u;
+  const int64_t b = row / (uint32_t)p.T, t = row - (uint32_t)b * (uint32_t)p.T;
+  const int g = (int)(gi - row * (uint32_t)p.slots), step = p.slots;
   const bool on = live && N * l < h;
   const T* q = static_cast<const T*>(p.q) + b * p.qsb + t * p.qst + N * l;
   const T* k = static_cast<const T*>(p.k) + b * p.ksb + t * p.kst + N * l;
@@ -144,9 +169,9 @@ __global__ void __launch_bounds__(WARPS * 32, sizeof(T) == 4 ? 3 : 4) vec_kernel
 // Any even head dim, any alignment: one warp per head vector, read twice (the second time
 // from L1).
 template <typename T>
-__global__ void __launch_bounds__(WARPS * 32) any_kernel(const Params p) {
+__global__ void __launch_bounds__(ANY_WARPS * 32) any_kernel(const Params p) {
   const int lane = threadIdx.x & 31, h = p.D / 2, n = p.Hq + p.H;
-  const int64_t wid = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  const int64_t wid = (int64_t)blockIdx.x * ANY_WARPS + (threadIdx.x >> 5);
   const int64_t row = wid / n;
   if (row >= p.rows) return;
   const int64_t b = row / p.T, t = row - b * p.T;
@@ -180,28 +205,46 @@ int launch(const Params& p, bool vec, cudaStream_t st) {
   int64_t warps;
   if (!vec) {
     warps = p.rows * (p.Hq + p.H);
-    SPX_REQUIRE((warps + WARPS - 1) / WARPS <= 0x7fffffff, SPX_ERR_SHAPE, "spx_qk_norm_rope: too many rows");
-    any_kernel<T><<<(unsigned)((warps + WARPS - 1) / WARPS), WARPS * 32, 0, st>>>(p);
+    const int64_t grid = (warps + ANY_WARPS - 1) / ANY_WARPS;
+    SPX_REQUIRE(grid <= 0x7fffffff, SPX_ERR_SHAPE, "spx_qk_norm_rope: too many rows");
+    any_kernel<T><<<(unsigned)grid, ANY_WARPS * 32, 0, st>>>(p);
     return launch_status("qk_norm any_kernel");
   }
-  constexpr int VP = 8;
+  constexpr int VP = 8, WARPS = kWarps<T>;
+  // Lanes of a head: a power of two, or as many as it has vectors where a warp then holds more heads
+  // and the rows fill the SMs (the sum takes a step more).  bf16, 12 heads of 80: 8 x 2048 rows 15.0
+  // us with five lanes, 17.8 with eight; 3 x 1037 rows 6.5 and 6.0; of 160: 3 x 1037 rows 8.7 us
+  // with ten, 10.3 with sixteen, 8 x 2048 32.6 and 34.4.
   int G = 1;
-  while (VP * G < h) G *= 2;
+  const int vectors = (h + VP - 1) / VP;
+  while (G < vectors) G *= 2;
+  if (32 / vectors > 32 / G && (vectors > 8 || (vectors > 4 && p.rows * G > (int64_t)148 * 16 * 32))) G = vectors;
   Params q = p;
-  // Few rows: the heads of a row are spread over several groups of lanes, up to 16 warps an SM
-  // or one head a group.  3 x 1037 rows of 12 heads of 80: 8.3 us with one group a row, 5.7 with
-  // three, 6.9 with four, 7.3 with six (each group looks up its position and table row).
+  // The heads of a row are spread over several groups of lanes.  Few rows: up to 16 warps an SM or
+  // one head a group (3 x 1037 rows of 12 heads of 80: 8.8 us with one group a row, 5.9 with three,
+  // 7.3 with four, 7.6 with six: each group looks up its position and table row); from four on a
+  // power of two, so that a warp's groups are of one row (1024 rows of 40 heads of 128: 6.6 us with
+  // eight, 6.8 with nine, 7.4 with ten).  Many rows: at most 14 heads a group (8 x 1024 rows of 40
+  // heads 41.2 us with one group a row, 33.6 with two, 32.5 with four, 33.8 with eight; of 12 heads
+  // 11.5 with one, 11.7 with two).
   const int ng = 32 / G, most = p.Hq + p.H;
   const int64_t fit = (int64_t)148 * 16 * ng / p.rows;
-  q.slots = (int)(fit < 1 ? 1 : fit < most ? fit : most);
+  int slots = 1;
+  while (slots * 14 < most || (slots * 2 <= fit && slots * 2 <= most)) slots *= 2;
+  if (fit == 3 && slots < 3) slots = 3;
+  q.slots = fit >= most || slots > most ? most : slots;
   warps = (p.rows * q.slots + ng - 1) / ng;
-  SPX_REQUIRE((warps + WARPS - 1) / WARPS <= 0x7fffffff, SPX_ERR_SHAPE, "spx_qk_norm_rope: too many rows");
+  SPX_REQUIRE(warps * 32 <= 0x7fffffff, SPX_ERR_SHAPE, "spx_qk_norm_rope: too many rows");   // 32-bit indexes
   const unsigned grid = (unsigned)((warps + WARPS - 1) / WARPS);
   switch (G) {
     case 1: vec_kernel<T, VP, 1><<<grid, WARPS * 32, 0, st>>>(q); break;
     case 2: vec_kernel<T, VP, 2><<<grid, WARPS * 32, 0, st>>>(q); break;
     case 4: vec_kernel<T, VP, 4><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 5: vec_kernel<T, VP, 5><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 6: vec_kernel<T, VP, 6><<<grid, WARPS * 32, 0, st>>>(q); break;
     case 8: vec_kernel<T, VP, 8><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 9: vec_kernel<T, VP, 9><<<grid, WARPS * 32, 0, st>>>(q); break;
+    case 10: vec_kernel<T, VP, 10><<<grid, WARPS * 32, 0, st>>>(q); break;
     case 16: vec_kernel<T, VP, 16><<<grid, WARPS * 32, 0, st>>>(q); break;
     default: vec_kernel<T, VP, 32><<<grid, WARPS * 32, 0, st>>>(q); break;
   }
