@@ -79,6 +79,10 @@ CASES = [
     (5, 700, 1024, (1400,), [128, 80, 3], [2, 1, 0, -1, 1]),
     (64, 64, 4104, (4136,), [16, 9], [i % 3 - 1 for i in range(64)]),
     (2, 530, 14336, (18000,), [7, 16], [0, 1]),
+    (160, 64, 4104, (4136,), [16, 9], [i % 3 - 1 for i in range(160)]),
+    (50, 120, 6000, (640,), [16, 9], [i % 3 - 1 for i in range(50)]),
+    (100, 128, 2056, (1000,), [16, 9], [i % 3 - 1 for i in range(100)]),
+    (30, 127, 4096, (136, 128, 72), [64, 50], [i % 3 - 1 for i in range(30)]),
 ]
 
 
@@ -148,7 +152,7 @@ def test_blocks_with_and_without_adapters_in_turn(B, T, K, W, parts):
     ranks = [tuple((8 if (s + p) % 3 else 0) for p in range(parts)) for s in range(6)]
     pool, held = _adapters(g, 6, K, widths, ranks, dt)
     ids = [i % 7 - 1 for i in range(B)]
-    assert B * T * (K + W * parts) * 16 >= 1 << 29
+    assert (T / (-(-T // 128) * 128)) ** 3 * B * T * (K + W) * parts * 16 >= 1.5e8     # taken as blocks
     x = torch.randn(B, T, K, generator=g, device="cuda").to(dt)
     y = torch.randn(B, T, W * parts, generator=g, device="cuda").to(dt)
     batch = LoraBatch(ids)

@@ -296,11 +296,14 @@ struct Pool {
     }
     require_device(a.device());
     if (rows == 0) return out_ ? *out_ : at::empty_like(y);
-    // Prompts take the kernels for blocks of adjacent rows, whose start takes longer and whose
-    // time does not grow with the rank.  They meet at about 30M values of x and y at rank 16 and
-    // 32 (4096 -> 6144 columns at rank 16: 2048 rows 24 us against 27, 4096 rows 45 against 42,
-    // 16384 rows 162 against 109) and 8M at rank 64 (4096 -> 4096: 1024 rows 31 against 23).
-    const bool blocks = tokens >= kBlockTokens && rows * (in + out) * args.max_rank >= (int64_t)1 << 29;
+    // Prompts take the kernels for blocks of adjacent rows, whose start takes longer, whose time does
+    // not grow with the rank, and whose blocks of 128 rows end with a sequence.  Over 110 calls (300
+    // to 95000 rows, 24 to 3900 tokens a sequence, rank 16 to 64) this rule takes the faster side
+    // but for 0.7 %; rank 64, 9982 rows of 322 tokens 112 us by rows, 55 by blocks; rank 16, 3267 rows
+    // of 363 tokens 21.8 and 22.2; 5548 rows of 76 tokens 16.5 and 28.0.
+    const double fill = (double)tokens / ((tokens + 127) / 128 * 128);
+    const bool blocks = tokens >= kBlockTokens &&
+                        fill * fill * fill * rows * ((double)in * args.parts + out) * args.max_rank >= 1.5e8;
     const c10::cuda::CUDAGuard guard(a.device());
     Batch::Plan& p = batch.plan(tokens, blocks);
     p.use(at::cuda::getCurrentCUDAStream(a.device().index()));

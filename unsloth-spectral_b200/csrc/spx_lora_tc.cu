@@ -612,20 +612,31 @@ static int rows_map(CUtensorMap* m, const void* ptr, int dtype, int64_t rows, in
 }
 
 int shrink_block_launch(const Params& p, int dtype, int tiles, cudaStream_t st) {
+  // Two CTAs an SM, and all columns in one group up to 256: x is read once (rank 64 in three parts:
+  // 77 us against 109 in two groups).  Few tiles: the CTAs of a cluster split k until they fill the
+  // SMs (clusters of eight do not fill every GPC: two thirds of the places), with at least four
+  // steps each: 77 tiles at K = 12560 95 us with one CTA a tile, 65 with two.  Where the cluster's
+  // sums take too much shared memory for that, a CTA has an SM to itself.
   Cfg c;
-  // The cluster's CTAs split k until the grid fills the SMs, with at least four steps each; then
-  // a CTA has an SM to itself (and clusters of eight do not fill every GPC: 12 of them at most).
-  // Else two an SM, and all columns in one group up to 256: x is read once (rank 64 in three
-  // parts: 77 us against 109 in two groups).
-  c.cs = 1;
-  const int units = tiles * ((p.SR + 127) / 128);
-  while (c.cs < 8 && (int64_t)units * c.cs * 2 <= (c.cs < 4 ? num_sms() : 96) && p.K >= 4 * KB * 2 * c.cs) c.cs *= 2;
-  const int widest = c.cs > 1 ? 128 : 256;
-  c.groups = (p.SR + widest - 1) / widest;
-  c.nb = ((p.SR + c.groups - 1) / c.groups + 15) / 16 * 16;
-  const int sbytes = XBYTES + c.nb * KB * 2, got = c.cs > 1 ? M * (c.nb + 4) * 4 : 0;
-  c.stages = c.cs > 1 ? (220 * 1024 - got) / sbytes : 110 * 1024 / sbytes;   // 2 (256 columns) to 8
-  if (c.stages > MAXSTAGES) c.stages = MAXSTAGES;
+  int sbytes = 0, got = 0;
+  const auto shape = [&](int cs) {   // CTAs an SM
+    const int widest = cs > 1 ? 128 : 256;
+    c.cs = cs;
+    c.groups = (p.SR + widest - 1) / widest;
+    c.nb = ((p.SR + c.groups - 1) / c.groups + 15) / 16 * 16;
+    sbytes = XBYTES + c.nb * KB * 2, got = cs > 1 ? M * (c.nb + 4) * 4 : 0;
+    const bool two = cs == 1 || (110 * 1024 - got) / sbytes >= 3;
+    c.stages = ((two ? 110 : 220) * 1024 - got) / sbytes;   // 2 (256 columns) to 8
+    if (c.stages > MAXSTAGES) c.stages = MAXSTAGES;
+    return two ? 2 : 1;
+  };
+  int cs = 1;
+  while (cs < 8 && p.K >= 4 * KB * 2 * cs) {
+    const int places = shape(2 * cs) * (cs < 4 ? num_sms() : 96);
+    if ((int64_t)tiles * c.groups * 2 * cs > places) break;
+    cs *= 2;
+  }
+  shape(cs);
   c.smem = (size_t)c.stages * sbytes + got + 1024;
   CUtensorMap mx, ma;
   int rc = rows_map(&mx, p.x, dtype, p.rows, p.xs, p.K, KB, M, CU_TENSOR_MAP_SWIZZLE_128B);
