@@ -12,9 +12,9 @@
 // m16n8k16 steps (16-byte loads, whole sectors); the same choice over the output columns
 // gives 16-byte accesses of y and out.
 // These are the kernels for few rows of a slot; prompts take spx_lora_tc.cu's.  Bound by latency
-// and by the weights: one request on q|k|v at rank 16 takes 5.3 us (two launches, the second
+// and by the weights: one request on q|k|v at rank 16 takes 4.8 us (two launches, the second
 // one waiting for the first inside the GPU), 64 requests with 24 adapters of rank 64 and 32 at
-// K = 14336 17.7 us, of which 50 MB of weights need 7.6.
+// K = 14336 17.8 us, of which 50 MB of weights need 7.6.
 // t is kept in float32; for the second product it is split into a high and a low value of
 // the row type (two MMAs), which keeps about 16 (bf16) or 22 (f16) bits of it.
 #include "spx_lora.cuh"
@@ -47,9 +47,10 @@ __device__ __forceinline__ void copy16(uint4* dst, const void* src, bool in) {  
 }
 
 template <typename T, int MT, int NT>
-__global__ void __launch_bounds__(SW * 32) shrink_kernel(const Params p) {
+__global__ void __launch_bounds__(SW * 32, MT * NT > 8 ? 2 : 3) shrink_kernel(const Params p) {
   using Ri = Ring<MT, NT>;
   extern __shared__ uint4 ring[];
+  __shared__ int s_left[NT];   // of each group of eight columns: how many hold a rank in use
   constexpr int N = NT * 8, E = MT * 16 * N;
   float* const sums = reinterpret_cast<float*>(ring);   // [SW][MT * 16][N], after the stream
   float* const got = reinterpret_cast<float*>(ring) + Ri::FLOATS;   // [cs][E / cs]: the cluster's sums of this CTA's share
@@ -68,12 +69,13 @@ __global__ void __launch_bounds__(SW * 32) shrink_kernel(const Params p) {
       const int r = m * 16 + h * 8 + g;
       xr[m][h] = r < tile.z ? static_cast<const T*>(p.x) + (int64_t)p.order[tile.y + r] * p.xs + 8 * c : nullptr;
     }
-  uint32_t act = 0;   // column groups of eight that hold a rank in use
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int col = col0 + n * 8;
-    if (col < p.SR && col % p.R < p.ranks[tile.x * p.parts + col / p.R]) act |= 1u << n;
+  int in_use = 0;   // lane n: group n of eight columns
+  if (lane < NT && col0 + lane * 8 < p.SR) {
+    const int col = col0 + lane * 8, part = col / p.R;
+    in_use = p.ranks[tile.x * p.parts + part] - (col - part * p.R);
   }
+  const uint32_t act = __ballot_sync(0xffffffffu, in_use > 0);   // groups that hold a rank in use
+  if (warp == 0 && lane < NT) s_left[lane] = in_use;
   const T* ar = static_cast<const T*>(p.a) + ((int64_t)tile.x * p.SR + col0 + g) * p.K + 8 * c;
   float acc[MT][NT][4];
 #pragma unroll
@@ -137,23 +139,24 @@ __global__ void __launch_bounds__(SW * 32) shrink_kernel(const Params p) {
   __syncthreads();
   cluster_started();
   const int share = E / cs;   // cs is a power of two up to 8, E a multiple of 256
+  const int used = tile.z * N;
+#pragma unroll 4
   for (int e = threadIdx.x; e < E; e += SW * 32) {
+    if (e >= used) break;
     float v = sums[e];
 #pragma unroll
     for (int w = 1; w < SW; ++w) v += sums[w * E + e];
-    const int owner = e / share;
+    const int owner = e * cs / E;   // e / share
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(in_cta(got + cr * share + e - owner * share, owner)), "f"(v) : "memory");
   }
   cluster_pushed();
   for (int i = threadIdx.x; i < share; i += SW * 32) {
     const int e = cr * share + i, r = e / N, col = col0 + e % N;
+    if (r >= tile.z || col >= p.SR) continue;
     float v = got[i];
     for (int k = 1; k < cs; ++k) v += got[k * share + i];
-    if (r < tile.z && col < p.SR) {
-      // past the rank: exact zeros, also where x holds an infinity
-      if (col % p.R >= p.ranks[tile.x * p.parts + col / p.R]) v = 0.f;
-      p.t[(int64_t)(tile.y + r) * p.SR + col] = v;
-    }
+    // past the rank: exact zeros, also where x holds an infinity
+    p.t[(int64_t)(tile.y + r) * p.SR + col] = e % 8 < s_left[e % N / 8] ? v : 0.f;
   }
 }
 
@@ -281,20 +284,36 @@ __global__ void __launch_bounds__(EW * 32) expand_kernel(const Params p, const i
 }
 
 template <typename T, int MT, int NT>
-int launch_shrink(const Params& p, int tiles, int groups, int cs, cudaStream_t st) {
+int launch_shrink(const Params& p, int tiles, int groups, cudaStream_t st) {
   const size_t smem = Ring<MT, NT>::BYTES;
-  static std::atomic<int> have[64];
+  static std::atomic<int> have[64], places[64][4];   // places: clusters of 1, 2, 4 and 8 CTAs that a device holds
   cudaError_t e = allow_smem(shrink_kernel<T, MT, NT>, (int)smem, have);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(tiles * cs), (unsigned)groups);
   cfg.blockDim = dim3(SW * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)cs, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
+  const auto cluster = [&](int cs) {
+    cfg.gridDim = dim3((unsigned)(tiles * cs), (unsigned)groups);
+    at[0].val.clusterDim.x = (unsigned)cs, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  };
+  // CTAs that share a tile's k: as many as the device holds at once, with at least two steps of 32
+  // for each warp, 8 at most (the portable cluster size).
+  int dev = 0, l = 0;
+  if (e == cudaSuccess) e = cudaGetDevice(&dev);
+  for (; e == cudaSuccess && l < 3 && p.K >= 32 * SW * 2 << l; ++l) {
+    cluster(2 << l);
+    int n = dev < 64 ? places[dev][l + 1].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+      e = cudaOccupancyMaxActiveClusters(&n, shrink_kernel<T, MT, NT>, &cfg);
+      if (e == cudaSuccess && dev < 64) places[dev][l + 1].store(n, std::memory_order_relaxed);
+    }
+    if ((int64_t)tiles * groups > n + n / 16) break;   // a few more than fit, or tiles without an adapter, cost less than half the CTAs
+  }
+  cluster(1 << l);
   if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, shrink_kernel<T, MT, NT>, p);
   if (e != cudaSuccess) {
     set_error("lora shrink_kernel: %s", cudaGetErrorString(e));
@@ -333,20 +352,16 @@ int launch_shrink_rows(const Params& p, int tiles, int tile_rows, cudaStream_t s
   const int cols = (int64_t)tiles * (p.SR / 16) * 8 <= 2 * 148 ? 16 : tile_rows == 16 ? 32 : 64;
   const int groups = (p.SR + cols - 1) / cols;
   const int nt = ((p.SR / 8 + groups - 1) / groups + 1) / 2 * 2;  // 2, 4, 6 or 8
-  // CTAs that share a tile's k: until three CTAs an SM hold the grid, with at least two steps of
-  // 32 for each warp, 8 at most (the portable cluster size).
-  int cs = 1;
-  while (cs < 8 && (int64_t)tiles * groups * cs * 2 <= 3 * 148 && p.K >= 32 * SW * 2 * cs) cs *= 2;
   if (tile_rows == 16) {
-    return nt == 2   ? launch_shrink<T, 1, 2>(p, tiles, groups, cs, st)
-           : nt == 4 ? launch_shrink<T, 1, 4>(p, tiles, groups, cs, st)
-           : nt == 6 ? launch_shrink<T, 1, 6>(p, tiles, groups, cs, st)
-                     : launch_shrink<T, 1, 8>(p, tiles, groups, cs, st);
+    return nt == 2   ? launch_shrink<T, 1, 2>(p, tiles, groups, st)
+           : nt == 4 ? launch_shrink<T, 1, 4>(p, tiles, groups, st)
+           : nt == 6 ? launch_shrink<T, 1, 6>(p, tiles, groups, st)
+                     : launch_shrink<T, 1, 8>(p, tiles, groups, st);
   }
-  return nt == 2   ? launch_shrink<T, 2, 2>(p, tiles, groups, cs, st)
-         : nt == 4 ? launch_shrink<T, 2, 4>(p, tiles, groups, cs, st)
-         : nt == 6 ? launch_shrink<T, 2, 6>(p, tiles, groups, cs, st)
-                   : launch_shrink<T, 2, 8>(p, tiles, groups, cs, st);
+  return nt == 2   ? launch_shrink<T, 2, 2>(p, tiles, groups, st)
+         : nt == 4 ? launch_shrink<T, 2, 4>(p, tiles, groups, st)
+         : nt == 6 ? launch_shrink<T, 2, 6>(p, tiles, groups, st)
+                   : launch_shrink<T, 2, 8>(p, tiles, groups, st);
 }
 
 template <typename T>
