@@ -50,7 +50,8 @@ def _first_max(x):
 
 CASES = [(1, 32768, 16, True), (8, 32768, 3, True), (3, 1000, 2, True), (5, 50021, 40, True), (2, 7, 1, True), (1, 1, 0, False),
          (4, 31, 0, True), (2, 33, 2, False), (300, 513, 1, True), (2, 131077, 300, False), (7, 4104, 0, True),
-         (700, 9001, 2, True), (3, 20000, 9, False), (90, 40003, 3, True)]
+         (700, 9001, 2, True), (3, 20000, 9, False), (90, 40003, 3, True),
+         (2, 131075, 300, True), (20, 70001, 40, False), (25, 65536, 0, True)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])

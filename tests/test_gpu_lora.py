@@ -83,6 +83,8 @@ CASES = [
     (50, 120, 6000, (640,), [16, 9], [i % 3 - 1 for i in range(50)]),
     (100, 128, 2056, (1000,), [16, 9], [i % 3 - 1 for i in range(100)]),
     (30, 127, 4096, (136, 128, 72), [64, 50], [i % 3 - 1 for i in range(30)]),
+    (3, 1, 8200, (264, 16), [24, (16, 0)], [1, 0, -1]),
+    (40, 1, 4608, (1000,), [16], [0] * 40),
 ]
 
 

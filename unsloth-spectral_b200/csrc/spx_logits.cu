@@ -14,6 +14,8 @@
 // memory, so that one launch gives the token and no workspace is shared by calls.  Each
 // operation is rounded in float32 (no contraction), as the float32 expression is.
 
+#include <atomic>
+
 #include "spx_common.cuh"
 
 namespace spx {
@@ -93,7 +95,7 @@ template <typename T, int U_>
 __global__ void __launch_bounds__(NT, 4) rules_kernel(const Params p) {
   using Ti = Tile<T, U_>;
   __shared__ unsigned long long red[WARPS];
-  __shared__ unsigned long long tops[8];   // of the cluster's CTAs, in the first one's shared memory
+  __shared__ unsigned long long tops[16];   // of the cluster's CTAs, in the first one's shared memory
   __shared__ int listed[2];
   extern __shared__ uint16_t list[];
   constexpr int N = Ti::N, U = Ti::U, TOK = Ti::TOKENS, WORDS = Ti::WORDS;
@@ -300,15 +302,46 @@ __global__ void observe_kernel(const int64_t* tokens, int64_t stride, int count,
   }
 }
 
+// Whether the device takes clusters of 16 CTAs of a kernel (more than the portable 8), which has to
+// be asked for once.
+template <typename F>
+bool wide_clusters(F kernel, std::atomic<int> (&known)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return false;
+  int k = known[dev].load(std::memory_order_relaxed);
+  if (k == 0) {
+    int n = 0;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(16), cfg.blockDim = dim3(NT), cfg.dynamicSmemBytes = 2 * SEG;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 16, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    cfg.attrs = at, cfg.numAttrs = 1;
+    const bool ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                    cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0;
+    if (!ok) cudaGetLastError();   // not an error of this call
+    known[dev].store(k = ok ? 2 : 1, std::memory_order_relaxed);
+  }
+  return k == 2;
+}
+
+// CTAs of a row: as many as are resident at once (four an SM), at most the portable 8; or 16 where
+// those leave a third of the places free, which clusters of that size need (one row of 131072 bf16
+// 6.4 us with 16, 7.8 with 8; eight rows 6.9 and 8.4; 30 rows of 50000 7.8 and 6.5).
+inline int row_ctas(int batch) {
+  const int fit = 4 * 148 / batch;
+  return fit >= 24 ? 16 : fit > 8 ? 8 : fit < 1 ? 1 : fit;
+}
+
 template <typename T, int U>
 int launch_tiles(const Params& p, int batch, cudaStream_t st) {
-  // CTAs a row: as many as are resident at once (four an SM), at most one for a round of
-  // tiles of its warps, 8 at most (the portable cluster size).
+  // CTAs of a row: at most one for a round of tiles of its warps.
+  static std::atomic<int> known[64];
   constexpr int ROUND = WARPS * Tile<T, U>::TOKENS;
-  int cs = 4 * 148 / batch;
   const int most = (p.V + Tile<T, U>::N + ROUND - 1) / ROUND;
+  int cs = row_ctas(batch);
   cs = cs > most ? most : cs;
-  cs = cs > 8 ? 8 : cs < 1 ? 1 : cs;
+  if (cs > 8 && !wide_clusters(rules_kernel<T, U>, known)) cs = 8;
   const int64_t mine = (int64_t)((most + cs - 1) / cs) * ROUND;
   const size_t smem = p.touched ? 2 * (size_t)(mine < SEG ? mine : SEG) : 0;
   cudaLaunchConfig_t cfg{};
@@ -333,7 +366,7 @@ template <typename T>
 int launch(const Params& p, int batch, cudaStream_t st) {
   // Loads that a lane has in flight: as many as its CTAs need for the row at once, at most four
   // (128 x 131072 f32: 51 us with one, 31 with four).
-  const int cs = 4 * 148 / batch, row = (cs > 8 ? 8 : cs < 1 ? 1 : cs) * NT * Tile<T, 1>::N;
+  const int row = row_ctas(batch) * NT * Tile<T, 1>::N;
   if (p.V <= row) return launch_tiles<T, 1>(p, batch, st);
   if (p.V <= 2 * row) return launch_tiles<T, 2>(p, batch, st);
   return launch_tiles<T, 4>(p, batch, st);

@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(SW * 32, MT * NT > 8 ? 2 : 3) shrink_kernel(co
     }
   __syncthreads();
   cluster_started();
-  const int share = E / cs;   // cs is a power of two up to 8, E a multiple of 256
+  const int share = E / cs;   // cs is a power of two up to 16, E a multiple of 256
   const int used = tile.z * N;
 #pragma unroll 4
   for (int e = threadIdx.x; e < E; e += SW * 32) {
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(EW * 32) expand_kernel(const Params p, const i
 template <typename T, int MT, int NT>
 int launch_shrink(const Params& p, int tiles, int groups, cudaStream_t st) {
   const size_t smem = Ring<MT, NT>::BYTES;
-  static std::atomic<int> have[64], places[64][4];   // places: clusters of 1, 2, 4 and 8 CTAs that a device holds
+  static std::atomic<int> have[64], places[64][5];   // places: clusters of 1 .. 16 CTAs that a device holds (-1: none)
   cudaError_t e = allow_smem(shrink_kernel<T, MT, NT>, (int)smem, have);
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(SW * 32);
@@ -301,15 +301,18 @@ int launch_shrink(const Params& p, int tiles, int groups, cudaStream_t st) {
     at[0].val.clusterDim.x = (unsigned)cs, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
   };
   // CTAs that share a tile's k: as many as the device holds at once, with at least two steps of 32
-  // for each warp, 8 at most (the portable cluster size).
+  // for each warp, 16 at most (more than the portable 8, so it has to be asked for).
   int dev = 0, l = 0;
   if (e == cudaSuccess) e = cudaGetDevice(&dev);
-  for (; e == cudaSuccess && l < 3 && p.K >= 32 * SW * 2 << l; ++l) {
+  for (; e == cudaSuccess && l < 4 && p.K >= 32 * SW * 2 << l; ++l) {
     cluster(2 << l);
     int n = dev < 64 ? places[dev][l + 1].load(std::memory_order_relaxed) : 0;
     if (n == 0) {
-      e = cudaOccupancyMaxActiveClusters(&n, shrink_kernel<T, MT, NT>, &cfg);
-      if (e == cudaSuccess && dev < 64) places[dev][l + 1].store(n, std::memory_order_relaxed);
+      cudaError_t q = l < 3 ? cudaSuccess : cudaFuncSetAttribute(shrink_kernel<T, MT, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (q == cudaSuccess) q = cudaOccupancyMaxActiveClusters(&n, shrink_kernel<T, MT, NT>, &cfg);
+      if (q != cudaSuccess) cudaGetLastError();   // not an error of this call: a smaller cluster
+      if (q != cudaSuccess || n == 0) n = -1;
+      if (dev < 64) places[dev][l + 1].store(n, std::memory_order_relaxed);
     }
     if ((int64_t)tiles * groups > n + n / 16) break;   // a few more than fit, or tiles without an adapter, cost less than half the CTAs
   }
