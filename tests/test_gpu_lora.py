@@ -83,6 +83,9 @@ CASES = [
     (50, 120, 6000, (640,), [16, 9], [i % 3 - 1 for i in range(50)]),
     (100, 128, 2056, (1000,), [16, 9], [i % 3 - 1 for i in range(100)]),
     (30, 127, 4096, (136, 128, 72), [64, 50], [i % 3 - 1 for i in range(30)]),
+    (2, 128, 8192, (1032,), [64, 30], [0, 1]),
+    (19, 200, 1912, (1520, 128, 136), [64, (5, 0, 64), 9], [i % 4 - 1 for i in range(19)]),
+    (4, 112, 14152, (488, 40, 1000), [24, 9], [1, 0, -1, 0]),
     (3, 1, 8200, (264, 16), [24, (16, 0)], [1, 0, -1]),
     (40, 1, 4608, (1000,), [16], [0] * 40),
 ]

@@ -611,32 +611,68 @@ static int rows_map(CUtensorMap* m, const void* ptr, int dtype, int64_t rows, in
   return SPX_OK;
 }
 
+// Clusters of 16 CTAs (more than the portable 8) of the kernel that the device holds at once, one or
+// two CTAs an SM; asked for once.
+static int wide_clusters(int an_sm) {
+  static std::atomic<int> known[64][2];   // the number + 1
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
+  std::atomic<int>& k = known[dev][an_sm - 1];
+  if (k.load(std::memory_order_relaxed) == 0) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(16), cfg.blockDim = dim3(128), cfg.dynamicSmemBytes = (an_sm == 2 ? 111 : 221) * 1024;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 16, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    cfg.attrs = at, cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(shrink_block_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 221 * 1024) != cudaSuccess ||
+        cudaFuncSetAttribute(shrink_block_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, shrink_block_kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();   // not an error of this call: smaller clusters
+      n = 0;
+    }
+    k.store(n + 1, std::memory_order_relaxed);
+  }
+  return k.load(std::memory_order_relaxed) - 1;
+}
+
 int shrink_block_launch(const Params& p, int dtype, int tiles, cudaStream_t st) {
   // Two CTAs an SM, and all columns in one group up to 256: x is read once (rank 64 in three parts:
   // 77 us against 109 in two groups).  Few tiles: the CTAs of a cluster split k until they fill the
-  // SMs (clusters of eight do not fill every GPC: two thirds of the places), with at least four
-  // steps each: 77 tiles at K = 12560 95 us with one CTA a tile, 65 with two.  Where the cluster's
-  // sums take too much shared memory for that, a CTA has an SM to itself.
+  // SMs (clusters of eight do not fill every GPC: two thirds of the places), with at least four steps
+  // each: 77 tiles at K = 12560 95 us with one CTA a tile, 65 with two; four tiles at K = 14336 25.3
+  // us a call with eight, 21.3 with sixteen.  More columns than 128 are two groups then, or one where
+  // two do not fit (38 tiles of 192 columns 61 us with one CTA each, 50).  Where the CTAs leave an SM
+  // to each, or the cluster's sums take the room, a ring has all of its shared memory.
   Cfg c;
   int sbytes = 0, got = 0;
-  const auto shape = [&](int cs) {   // CTAs an SM
-    const int widest = cs > 1 ? 128 : 256;
+  const auto shape = [&](int cs, int widest, bool alone) {   // CTAs an SM
     c.cs = cs;
     c.groups = (p.SR + widest - 1) / widest;
     c.nb = ((p.SR + c.groups - 1) / c.groups + 15) / 16 * 16;
     sbytes = XBYTES + c.nb * KB * 2, got = cs > 1 ? M * (c.nb + 4) * 4 : 0;
-    const bool two = cs == 1 || (110 * 1024 - got) / sbytes >= 3;
+    const bool two = !alone && (cs == 1 || (110 * 1024 - got) / sbytes >= 3);
     c.stages = ((two ? 110 : 220) * 1024 - got) / sbytes;   // 2 (256 columns) to 8
     if (c.stages > MAXSTAGES) c.stages = MAXSTAGES;
     return two ? 2 : 1;
   };
-  int cs = 1;
-  while (cs < 8 && p.K >= 4 * KB * 2 * cs) {
-    const int places = shape(2 * cs) * (cs < 4 ? num_sms() : 96);
-    if ((int64_t)tiles * c.groups * 2 * cs > places) break;
-    cs *= 2;
+  const auto fits = [&](int cs, int widest) {
+    const int an_sm = shape(cs, widest, false);
+    const int64_t places = cs < 8 ? an_sm * num_sms() : cs == 8 ? an_sm * 96 : 16 * wide_clusters(an_sm);
+    return (int64_t)tiles * c.groups * cs <= places;
+  };
+  int cs = 1, widest = 256;
+  for (; cs < 16 && p.K >= 4 * KB * 2 * cs; cs *= 2) {
+    if (fits(2 * cs, 128)) {
+      widest = 128;
+    } else if (p.SR > 128 && p.SR <= 192 && fits(2 * cs, 192)) {
+      widest = 192;
+    } else {
+      break;
+    }
   }
-  shape(cs);
+  shape(cs, widest, false);
+  if ((int64_t)tiles * c.groups * cs <= (cs < 8 ? num_sms() : cs == 8 ? 96 : 16 * wide_clusters(1))) shape(cs, widest, true);
   c.smem = (size_t)c.stages * sbytes + got + 1024;
   CUtensorMap mx, ma;
   int rc = rows_map(&mx, p.x, dtype, p.rows, p.xs, p.K, KB, M, CU_TENSOR_MAP_SWIZZLE_128B);
