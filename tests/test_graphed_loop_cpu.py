@@ -1,0 +1,57 @@
+"""The graphed decode loop on the host: which stream each of its operations is issued on, with
+fake streams (no GPU)."""
+import contextlib
+from types import SimpleNamespace
+
+import pytest
+import torch
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from unsloth_spectral.llama_loop import SpectralLlama
+
+
+class _Streams(TorchDispatchMode):
+    """Notes every tensor operation with the stream that is current, and every wait."""
+
+    def __init__(self, monkeypatch):
+        super().__init__()
+        self.log, log = [], []
+        self.log = log
+        make = lambda name: SimpleNamespace(  # noqa: E731
+            name=name, wait_stream=lambda other: log.append(("wait", name, other.name)))
+        self.main, self.side = make("main"), make("side")
+        self.current = self.main
+
+        @contextlib.contextmanager
+        def use(stream):
+            before, self.current = self.current, stream
+            yield
+            self.current = before
+
+        monkeypatch.setattr(torch.cuda, "Stream", lambda device=None: self.side)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: self.current)
+        monkeypatch.setattr(torch.cuda, "stream", use)
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.log.append(("op", self.current.name, str(func)))
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("n", [1, 2, 4])
+def test_what_the_side_stream_reads_was_issued_before_it_waits(monkeypatch, n):
+    """The side stream follows the main one from its wait on: what is issued on the main stream
+    after that wait (the copy of the first token) may run beside the first step that reads it."""
+    streams = _Streams(monkeypatch)
+    tiers = SimpleNamespace(num_blocks=0, hot_len=0)
+    caches = [SimpleNamespace(tiers=tiers, block_size=512)]
+    model = SimpleNamespace(decode_step=lambda tok, pos, caches: torch.nn.functional.one_hot(tok + 1, 50).float())
+    tok, pos, out = torch.tensor([3, 7]), torch.zeros(1, 1, dtype=torch.long), torch.zeros(2, n, dtype=torch.long)
+    with streams:
+        SpectralLlama._decode_graphed(model, tok, pos, caches, out, lambda logits: logits.argmax(-1))
+    assert torch.equal(out, torch.tensor([[3], [7]]) + torch.arange(n))
+    assert torch.equal(tok, torch.tensor([3, 7]))          # the caller's token stays
+    log = streams.log
+    start, end = log.index(("wait", "side", "main")), log.index(("wait", "main", "side"))
+    assert start < end
+    assert [e for e in log[start:end] if e[:2] == ("op", "main")] == []
+    assert [e for e in log[:start] + log[end:] if e[:2] == ("op", "side")] == []

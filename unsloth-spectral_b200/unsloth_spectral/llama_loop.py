@@ -272,9 +272,10 @@ class SpectralLlama(torch.nn.Module):
         n = out.shape[1]
         dev = tok.device
         stream = torch.cuda.Stream(device=dev)
-        stream.wait_stream(torch.cuda.current_stream(dev))
         tok, s = tok.clone(), 0
         out[:, 0] = tok
+        # from here on nothing is issued on the caller's stream until it waits for this one
+        stream.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(stream):
             while s + 1 < n:
                 t0 = caches[0].tiers
