@@ -1,0 +1,60 @@
+"""LoraAdapters on the host: which modules a set holds, and what it refuses (no GPU)."""
+import pytest
+import torch
+
+from unsloth_spectral import LoraAdapters
+from unsloth_spectral.adapters import adapted
+from unsloth_spectral.llama_loop import LlamaShape, SpectralLlama
+
+SHAPE = LlamaShape(layers=2, hidden=64, heads=4, kv_heads=2, head_dim=16, ffn=96, vocab=50)
+
+
+def _model(seed=0):
+    return SpectralLlama(SHAPE, device="cpu", dtype=torch.bfloat16, seed=seed)
+
+
+def _held(model):
+    return [getattr(m, "spx_lora", None) for layer in model.model.layers for m in (layer.self_attn, layer.mlp)]
+
+
+@pytest.mark.parametrize("first,second", [
+    (LoraAdapters.ATTENTION + LoraAdapters.MLP, ("q_proj",)), (("q_proj",), ("o_proj",)), (("up_proj",), ("down_proj",)),
+    (LoraAdapters.ATTENTION + LoraAdapters.MLP, LoraAdapters.ATTENTION), (("v_proj", "up_proj"), LoraAdapters.MLP)])
+def test_a_second_set_on_a_module_is_refused_until_the_first_is_detached(first, second):
+    model = _model()
+    a = LoraAdapters(model, max_rank=4, slots=2, targets=first)
+    held = _held(model)
+    with pytest.raises(ValueError, match="detach"):
+        LoraAdapters(model, max_rank=8, slots=3, targets=second)
+    assert all(x is y for x, y in zip(_held(model), held))       # the refused set left nothing behind
+    a.use([0, 1])
+    a.detach()
+    assert _held(model) == [None] * 4 and a.batch is None
+    b = LoraAdapters(model, max_rank=8, slots=3, targets=second)
+    with pytest.raises(RuntimeError, match="detached"):
+        a.use([0, 1])
+    a.use(None)
+    a.detach()                                                   # again: nothing left to take off
+    assert [x[0] for x in _held(model) if x is not None] == [b] * sum(x is not None for x in _held(model))
+
+
+def test_sets_on_different_modules_stand_beside_each_other():
+    model = _model()
+    a = LoraAdapters(model, max_rank=4, slots=2, targets=("q_proj", "o_proj"))
+    b = LoraAdapters(model, max_rank=4, slots=2, targets=("down_proj",))
+    assert [x[0] for x in _held(model)] == [a, b, a, b]
+    b.detach()
+    assert [x and x[0] for x in _held(model)] == [a, None, a, None]
+    y = torch.zeros(2, 1, 64, dtype=torch.bfloat16)
+    a.use([0, 1])
+    assert adapted(model.model.layers[0].mlp, "down_proj", y, y) is y
+    with pytest.raises(RuntimeError):                            # reaches the pool (on a CPU tensor)
+        adapted(model.model.layers[0].self_attn, "o_proj", y, y)
+
+
+def test_a_refused_set_leaves_the_model_as_it_was():
+    model = _model()
+    model.model.layers[1].mlp = torch.nn.Identity()
+    with pytest.raises(ValueError, match="layer 1"):
+        LoraAdapters(model, max_rank=4, slots=2)
+    assert _held(model) == [None] * 4

@@ -149,7 +149,8 @@ class LoraAdapters:
         model.generate(ids, 64, adapters=adapters, adapter_slots=[0, -1, 3, 0])
 
     ``use(slots)`` names the slot of each sequence for the forwards that follow, ``use(None)``
-    switches the adapters off."""
+    switches the adapters off.  An attention module or an MLP takes the adapters of one set at a
+    time; ``detach()`` takes a set off its model."""
 
     ATTENTION = ("q_proj", "k_proj", "v_proj", "o_proj")
     MLP = ("gate_proj", "up_proj", "down_proj")
@@ -163,10 +164,15 @@ class LoraAdapters:
         self._pools: Dict[Tuple[int, str], Tuple[LoraPool, int]] = {}
         make = lambda w, out: LoraPool(w.shape[1], out, max_rank, slots, w.dtype, w.device)  # noqa: E731
         layers = model.model.layers
+        covered = []           # (module, its pools), attached when all of them are there
         for i, layer in enumerate(layers):
             attn, mlp = layer.self_attn, getattr(layer, "mlp", None)
             if set(targets) & set(self.MLP) and not hasattr(mlp, "spx_lora"):
                 raise ValueError(f"layer {i}: {type(mlp).__name__} takes no adapters; leave {self.MLP} out of targets")
+            for module, names in ((attn, self.ATTENTION), (mlp, self.MLP)):
+                if set(targets) & set(names) and getattr(module, "spx_lora", None) is not None:
+                    raise ValueError(f"layer {i}: {type(module).__name__} has the adapters of another LoraAdapters; "
+                                     f"detach() that first")
             held = {}
             qkv = [n for n in self.ATTENTION[:3] if n in targets]
             if qkv and getattr(attn, "spx_qkv_weight", None) is not None:
@@ -181,15 +187,26 @@ class LoraAdapters:
             if "o_proj" in targets:
                 held["o_proj"] = make(attn.o_proj.weight, attn.o_proj.weight.shape[0])
                 self._pools[i, "o_proj"] = held["o_proj"], 0
-            attn.spx_lora = (self, held)
+            covered.append((attn, held))
             held = {}
             for n in self.MLP:
                 if n in targets:
                     held[n] = make(getattr(mlp, n).weight, getattr(mlp, n).weight.shape[0])
                     self._pools[i, n] = held[n], 0
-            if held:
-                mlp.spx_lora = (self, held)
+            covered.append((mlp, held))
         self.device = layers[0].self_attn.o_proj.weight.device
+        self._modules = [module for module, held in covered if held]
+        for module, held in covered:
+            if held:
+                module.spx_lora = (self, held)
+
+    def detach(self):
+        """Take the set off its model, whose modules run their shared weights alone again and can
+        take another set."""
+        self.batch = None
+        for module in self._modules or ():
+            module.spx_lora = None
+        self._modules = None
 
     def load(self, slot: int, weights: Dict[Tuple[int, str], Tuple[torch.Tensor, torch.Tensor]], scale: float = 1.0):
         """Put an adapter into a slot, in place of what it held: ``{(layer, projection): (A, B)}``
@@ -216,6 +233,8 @@ class LoraAdapters:
         if slots is None:
             self.batch = None
             return
+        if self._modules is None:
+            raise RuntimeError("these adapters are detached from their model")
         batch = LoraBatch(slots, self.device)
         if batch.highest >= self.slots:
             raise IndexError(f"slot {batch.highest} of {self.slots}")
