@@ -58,3 +58,21 @@ def test_a_refused_set_leaves_the_model_as_it_was():
     with pytest.raises(ValueError, match="layer 1"):
         LoraAdapters(model, max_rank=4, slots=2)
     assert _held(model) == [None] * 4
+
+
+def test_generate_refuses_a_set_that_is_not_this_models():
+    model, other = _model(), _model(1)
+    ids = torch.zeros(2, 3, dtype=torch.long)
+    foreign = LoraAdapters(other, max_rank=4, slots=2)
+    gone = LoraAdapters(model, max_rank=4, slots=2)
+    gone.detach()
+    mine = LoraAdapters(model, max_rank=4, slots=2, targets=("q_proj", "down_proj"))
+    for bad in (foreign, gone):
+        with pytest.raises(ValueError, match="not .* of this model"):
+            model.generate(ids, 1, adapters=bad, adapter_slots=[0, 1])
+        assert bad.batch is None
+    with pytest.raises(RuntimeError):                            # accepted, then refused for the device
+        model.generate(ids, 1, adapters=mine, adapter_slots=[0, 1])
+    model.model.layers[1] = other.model.layers[1]                # half of the set is no longer in the model
+    with pytest.raises(ValueError, match="not .* of this model"):
+        model.generate(ids, 1, adapters=mine, adapter_slots=[0, 1])

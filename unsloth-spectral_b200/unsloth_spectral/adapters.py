@@ -208,6 +208,12 @@ class LoraAdapters:
             module.spx_lora = None
         self._modules = None
 
+    def covers(self, model) -> bool:
+        """Whether ``model`` is the one that this set is on: each of its modules, and no set since
+        detached."""
+        there = {id(m) for layer in model.model.layers for m in (layer.self_attn, getattr(layer, "mlp", None))}
+        return self._modules is not None and all(id(m) in there and m.spx_lora[0] is self for m in self._modules)
+
     def load(self, slot: int, weights: Dict[Tuple[int, str], Tuple[torch.Tensor, torch.Tensor]], scale: float = 1.0):
         """Put an adapter into a slot, in place of what it held: ``{(layer, projection): (A, B)}``
         with ``A [rank, in]``, ``B [out, rank]``; projections left out keep the shared weight alone."""

@@ -225,6 +225,8 @@ class SpectralLlama(torch.nn.Module):
         if adapters is not None:
             if len(adapter_slots) != B:
                 raise ValueError(f"{B} sequences, {len(adapter_slots)} adapter slots")
+            if not adapters.covers(self):
+                raise ValueError("these adapters are not on the modules of this model")
             before = adapters.batch
             adapters.use(adapter_slots)
             adapters.batch.prepare(T).prepare(1)
