@@ -76,3 +76,13 @@ def test_generate_refuses_a_set_that_is_not_this_models():
     model.model.layers[1] = other.model.layers[1]                # half of the set is no longer in the model
     with pytest.raises(ValueError, match="not .* of this model"):
         model.generate(ids, 1, adapters=mine, adapter_slots=[0, 1])
+
+
+def test_a_generation_that_fails_to_start_leaves_the_adapters_as_they_were():
+    model = _model()
+    ad = LoraAdapters(model, max_rank=4, slots=2)
+    ad.use([1])
+    before = ad.batch
+    with pytest.raises(RuntimeError):                            # the rows cannot be grouped on the CPU
+        model.generate(torch.zeros(2, 3, dtype=torch.long), 1, adapters=ad, adapter_slots=[0, 1])
+    assert ad.batch is before

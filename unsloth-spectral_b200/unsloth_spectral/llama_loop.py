@@ -228,9 +228,9 @@ class SpectralLlama(torch.nn.Module):
             if not adapters.covers(self):
                 raise ValueError("these adapters are not on the modules of this model")
             before = adapters.batch
-            adapters.use(adapter_slots)
-            adapters.batch.prepare(T).prepare(1)
             try:
+                adapters.use(adapter_slots)
+                adapters.batch.prepare(T).prepare(1)
                 return self.generate(input_ids, max_new_tokens, timer, cuda_graphs, rules=rules, allow=allow)
             finally:
                 adapters.batch = before
