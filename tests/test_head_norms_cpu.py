@@ -1,0 +1,117 @@
+"""Which q_norm / k_norm modules the patched forwards hand to the fused kernel, and how they run
+the others (no GPU)."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from unsloth_spectral import integration as I
+from unsloth_spectral.llama_loop import RMSNorm
+
+D = 16
+
+
+class Norm(torch.nn.Module):
+    """A norm of head vectors that names its epsilon as the usual one does."""
+
+    def __init__(self, dtype=torch.float32, dim=D, eps=1e-6, fill=None):
+        super().__init__()
+        w = torch.linspace(0.5, 1.5, dim) if fill is None else torch.full((dim,), fill)
+        self.weight = torch.nn.Parameter(w.to(dtype))
+        self.variance_epsilon = eps
+
+    def scaled(self, y):
+        return y.to(self.weight.dtype) * self.weight
+
+    def forward(self, x):
+        y = x.float()
+        return self.scaled(y * torch.rsqrt(y.square().mean(-1, keepdim=True) + self.variance_epsilon))
+
+
+class RoundedOnce(Norm):
+    def scaled(self, y):
+        return (y * self.weight.float()).to(self.weight.dtype)
+
+
+class Centered(Norm):          # a layer norm
+    def forward(self, x):
+        y = x.float()
+        y = y - y.mean(-1, keepdim=True)
+        return self.scaled(y * torch.rsqrt(y.square().mean(-1, keepdim=True) + self.variance_epsilon))
+
+
+class Plus(Norm):
+    def scaled(self, y):
+        return (y * (1 + self.weight.float())).to(self.weight.dtype)
+
+
+class Biased(Norm):
+    def __init__(self, *a, **kw):
+        super().__init__(*a, **kw)
+        self.bias = torch.nn.Parameter(torch.zeros_like(self.weight))
+
+    def scaled(self, y):
+        return super().scaled(y) + self.bias
+
+
+class NoEpsilon(Norm):
+    def forward(self, x):
+        y = x.float()
+        return self.scaled(y * torch.rsqrt(y.square().mean(-1, keepdim=True)))
+
+
+class Outside(Norm):           # epsilon beside the root
+    def forward(self, x):
+        y = x.float()
+        return self.scaled(y / (y.square().mean(-1, keepdim=True).sqrt() + self.variance_epsilon))
+
+
+class L2(Norm):                # of the length, not of the mean
+    def forward(self, x):
+        y = x.float()
+        return self.scaled(y * torch.rsqrt(y.square().sum(-1, keepdim=True) + self.variance_epsilon))
+
+
+class Refuses(Norm):
+    def forward(self, x):
+        raise RuntimeError("not with these shapes")
+
+
+def _of(q, k, dtype=torch.float32):
+    return I._head_norms(SimpleNamespace(q_norm=q, k_norm=k), D, torch.zeros(1, 1, 2 * D, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("eps", [1e-6, 1e-5, 1e-12])
+@pytest.mark.parametrize("kind", [Norm, RoundedOnce])
+def test_the_usual_norm_is_recognised(dtype, eps, kind):
+    q, k = kind(dtype, eps=eps), kind(dtype, eps=eps, fill=0.25)
+    for _ in range(2):
+        got = _of(q, k, dtype)
+        assert got[0] is q.weight and got[1] is k.weight and got[2] == eps
+    q, k = (RMSNorm(D, eps, "cpu", dtype) for _ in range(2))
+    assert _of(q, k, dtype) == (q.weight, k.weight, eps)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("fill", [None, 0.0, 1.0])
+@pytest.mark.parametrize("kind", [Centered, Plus, Biased, NoEpsilon, Outside, L2, Refuses])
+def test_other_norms_run_their_own_code(dtype, fill, kind):
+    if fill == 0.0 and kind is not Plus and kind is not Biased and kind is not Refuses:
+        pytest.skip("every value is zero, as with the usual norm")
+    usual, other = Norm(dtype), kind(dtype, fill=fill)
+    for _ in range(2):
+        assert _of(usual, other, dtype) is None and _of(other, usual, dtype) is None
+
+
+def test_a_changed_norm_is_asked_again():
+    q, k = Norm(), Norm()
+    assert _of(q, k) is not None
+    q.variance_epsilon = k.variance_epsilon = 1e-5
+    assert _of(q, k)[2] == 1e-5
+    k.__class__ = Centered
+    assert _of(q, k) is None
+    k.__class__ = Norm
+    assert _of(q, k) is not None
+    k.forward = Centered.forward.__get__(k)      # a forward of the instance's own
+    assert _of(q, k) is None

@@ -113,17 +113,57 @@ def _qkv(self, hidden_states):
     return qkv[..., :nq], qkv[..., nq:nq + nk], qkv[..., nq + nk:]
 
 
+def _is_plain_rms(norm, weight: torch.Tensor, eps: float) -> bool:
+    """Whether ``norm(x)`` is ``x * rsqrt(mean(x^2) + eps) * weight`` for head vectors: this package's
+    ``RMSNorm``, or a module without a bias that gives the formula's values for three vectors (one
+    whose mean is not zero, one of both signs, one as small as the epsilon), each rounded to the
+    dtype once or, before the weight, twice.  A module is asked once for its class, dtype and
+    epsilon; inside a CUDA graph's capture, where the answer cannot be read, not at all (False)."""
+    from .llama_loop import RMSNorm
+    if type(norm) is RMSNorm:
+        return True
+    if getattr(norm, "bias", None) is not None:
+        return False
+    key = (type(norm), weight.dtype, eps)
+    known = norm.__dict__.get("_spx_plain_rms")
+    if known is not None and known[0] == key:
+        return known[1]
+    if weight.is_cuda and torch.cuda.is_current_stream_capturing():
+        return False
+    D, info = weight.numel(), torch.finfo(weight.dtype)
+    ramp = torch.linspace(0.25, 2.0, D, dtype=torch.float64)
+    sign = 1.0 - 2.0 * (torch.arange(D) % 3 == 1).double()
+    x = torch.stack([ramp, ramp.flip(0) * sign, ramp * max(math.sqrt(eps), 64 * info.tiny)])
+    x = x.to(device=weight.device, dtype=weight.dtype).view(1, 1, 3, D)
+    try:
+        with torch.no_grad():
+            got = norm(x).double()
+        xd = x.double()
+        want = xd * torch.rsqrt(xd.square().mean(-1, keepdim=True) + eps) * weight.detach().double()
+        # two roundings of half a step, and float32 sums
+        tol = (info.eps + 1e-5) * want.abs() + 4 * info.tiny * info.eps
+        plain = got.shape == want.shape and bool(((got - want).abs() <= tol).all())
+    except Exception:
+        plain = False
+    norm.__dict__["_spx_plain_rms"] = (key, plain)
+    return plain
+
+
 def _head_norms(self, head_dim: int, like: torch.Tensor):
     """``(q weight, k weight, eps)`` when module ``self`` normalises its query and key heads
     the way ``qk_norm_rope`` does -- ``q_norm`` / ``k_norm`` of ``head_dim`` weights in the dtype of
-    ``like`` with the usual RMS norm (this package's, or one that names its epsilon
-    ``variance_epsilon``) -- else None."""
+    ``like`` that compute the usual RMS norm (this package's, or one that names its epsilon
+    ``variance_epsilon`` and gives the formula's values) -- else None."""
     from .llama_loop import RMSNorm
     found = []
     for norm in (self.q_norm, self.k_norm):
         w = getattr(norm, "weight", None)
         eps = norm.eps if isinstance(norm, RMSNorm) else getattr(norm, "variance_epsilon", None)
         if w is None or eps is None or w.shape != (head_dim,) or w.dtype != like.dtype or w.device != like.device:
+            return None
+        if "forward" in norm.__dict__:
+            return None
+        if not _is_plain_rms(norm, w, float(eps)):
             return None
         found.append((w, float(eps)))
     (qw, eps), (kw, keps) = found
