@@ -115,3 +115,12 @@ def test_a_changed_norm_is_asked_again():
     assert _of(q, k) is not None
     k.forward = Centered.forward.__get__(k)      # a forward of the instance's own
     assert _of(q, k) is None
+
+
+def test_hooks_on_a_norm_are_called():
+    for register in ("register_forward_hook", "register_forward_pre_hook"):
+        q, k = Norm(), Norm()
+        handle = getattr(k, register)(lambda *a: None)
+        assert _of(q, k) is None
+        handle.remove()
+        assert _of(q, k) is not None

@@ -153,13 +153,15 @@ def _head_norms(self, head_dim: int, like: torch.Tensor):
     """``(q weight, k weight, eps)`` when module ``self`` normalises its query and key heads
     the way ``qk_norm_rope`` does -- ``q_norm`` / ``k_norm`` of ``head_dim`` weights in the dtype of
     ``like`` that compute the usual RMS norm (this package's, or one that names its epsilon
-    ``variance_epsilon`` and gives the formula's values) -- else None."""
+    ``variance_epsilon`` and gives the formula's values), without forward hooks -- else None."""
     from .llama_loop import RMSNorm
     found = []
     for norm in (self.q_norm, self.k_norm):
         w = getattr(norm, "weight", None)
         eps = norm.eps if isinstance(norm, RMSNorm) else getattr(norm, "variance_epsilon", None)
         if w is None or eps is None or w.shape != (head_dim,) or w.dtype != like.dtype or w.device != like.device:
+            return None
+        if getattr(norm, "_forward_hooks", None) or getattr(norm, "_forward_pre_hooks", None):
             return None
         if "forward" in norm.__dict__:
             return None
