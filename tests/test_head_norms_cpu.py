@@ -124,3 +124,37 @@ def test_hooks_on_a_norm_are_called():
         assert _of(q, k) is None
         handle.remove()
         assert _of(q, k) is not None
+
+
+class _HeadsOwn(torch.nn.Module):
+    """A norm of each head with weights of each head's own, [heads, head_dim]."""
+
+    def __init__(self, heads):
+        super().__init__()
+        self.weight = torch.nn.Parameter(torch.linspace(0.5, 2.0, heads * D).view(heads, D))
+
+    def forward(self, x):
+        return torch.nn.functional.layer_norm(x, (D,)) * self.weight
+
+
+class _Rows(torch.nn.Module):
+    """A norm of whole projection rows."""
+
+    def __init__(self, n):
+        super().__init__()
+        self.weight = torch.nn.Parameter(torch.linspace(0.5, 2.0, n))
+
+    def forward(self, x):
+        assert x.shape[-1] == len(self.weight)
+        return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6) * self.weight
+
+
+@pytest.mark.parametrize("heads", [1, 3])
+def test_own_norms_of_heads_and_of_rows(heads):
+    x = torch.randn(2, 5, heads * D, generator=torch.Generator().manual_seed(heads))
+    split = lambda y: y.view(2, 5, heads, D).transpose(1, 2)  # noqa: E731
+    for norm, want in ((_HeadsOwn(heads), lambda n: split(n(x.view(2, 5, heads, D)))), (_Rows(heads * D), lambda n: split(n(x))),
+                       (Norm(), lambda n: split(n(x.view(2, 5, heads, D)))),
+                       (torch.nn.LayerNorm((heads, D)), lambda n: split(n(x.view(2, 5, heads, D))))):
+        got = I._own_norm(norm, x, heads, D)
+        assert got.shape == (2, heads, 5, D) and torch.equal(got, want(norm))

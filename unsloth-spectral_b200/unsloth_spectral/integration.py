@@ -173,11 +173,13 @@ def _head_norms(self, head_dim: int, like: torch.Tensor):
 
 
 def _own_norm(norm, x: torch.Tensor, heads: int, head_dim: int) -> torch.Tensor:
-    """A module's own norm on projection rows ``[B, T, heads * head_dim]``: of each head, or of
-    whole rows when its weight is that wide; ``[B, heads, T, head_dim]``."""
+    """A module's own norm on projection rows ``[B, T, heads * head_dim]``: of whole rows when its
+    weight is one row of that width, else of each head (whose weights may be each head's own,
+    ``[heads, head_dim]``); ``[B, heads, T, head_dim]``."""
     B, T, n = x.shape
     w = getattr(norm, "weight", None)
-    y = norm(x) if w is not None and w.numel() == n and n != head_dim else norm(x.reshape(B, T, heads, head_dim))
+    rows = w is not None and w.shape == (n,) and n != head_dim
+    y = norm(x) if rows else norm(x.reshape(B, T, heads, head_dim))
     return y.reshape(B, T, heads, head_dim).transpose(1, 2)
 
 
