@@ -158,3 +158,36 @@ def test_own_norms_of_heads_and_of_rows(heads):
                        (torch.nn.LayerNorm((heads, D)), lambda n: split(n(x.view(2, 5, heads, D))))):
         got = I._own_norm(norm, x, heads, D)
         assert got.shape == (2, heads, 5, D) and torch.equal(got, want(norm))
+
+
+class _Cuda(torch.Tensor):
+    """A CPU tensor that says it is on the GPU: for the choice of a path, not for a launch."""
+
+    is_cuda = property(lambda self: True)
+
+
+def _choice(monkeypatch, positions, prepare=lambda q, k: (q, k), norms=None):
+    """What ``_normed_qk`` does with a query and a key of two heads each: the arguments that it hands
+    to the fused kernel (None: the modules' own norms), and its results."""
+    seen = []
+    monkeypatch.setattr(I, "qk_norm_rope", lambda *a, **kw: seen.append((a, kw)) or ("q", "k"))
+    g = torch.Generator().manual_seed(0)
+    q, k = prepare(torch.randn(2, 3, 2 * D, generator=g), torch.randn(2, 3, 2 * D, generator=g))
+    mod = SimpleNamespace(q_norm=(norms or [Norm()])[0], k_norm=(norms or [Norm()])[-1])
+    tab = torch.linspace(0, 1, 20 * D).view(20, D)
+    out = I._normed_qk(mod, q.as_subclass(_Cuda), k.as_subclass(_Cuda), 2, 2, D, tab.cos(), tab.sin(), positions)
+    return (seen[0] if seen else None), out
+
+
+def test_gradients_take_the_modules_own_norms(monkeypatch):
+    pos = torch.arange(3)[None]
+    frozen = [Norm().requires_grad_(False) for _ in range(2)]
+    with torch.no_grad():
+        for q, k in ((False, False), (True, True)):
+            assert _choice(monkeypatch, pos, lambda x, y: (x.requires_grad_(q), y.requires_grad_(k)))[0] is not None
+    assert _choice(monkeypatch, pos, norms=frozen)[0] is not None
+    for q, k in ((True, False), (False, True)):
+        used, (qo, ko) = _choice(monkeypatch, pos, lambda x, y: (x.requires_grad_(q), y.requires_grad_(k)), frozen)
+        assert used is None and qo.requires_grad == q and ko.requires_grad == k
+    used, (qo, ko) = _choice(monkeypatch, pos)             # of the norms' weights alone
+    assert used is None and qo.requires_grad and ko.requires_grad

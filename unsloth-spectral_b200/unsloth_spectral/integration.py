@@ -186,8 +186,13 @@ def _own_norm(norm, x: torch.Tensor, heads: int, head_dim: int) -> torch.Tensor:
 def _normed_qk(self, qp, kp, nh: int, nkv: int, hd: int, cos, sin, positions):
     """Queries and keys of an attention with ``q_norm`` / ``k_norm``: the queries normalised and
     rotated, the keys normalised (the cache holds them before the rotation), head-major.
-    ``positions``: int64 ``[1 or B, T]``, or the first one as an int."""
+    ``positions``: int64 ``[1 or B, T]``, or the first one as an int.  The fused kernel has no
+    gradients: where some are wanted, of the projections or of the norms' weights, the modules'
+    own norms run."""
     norms = _head_norms(self, hd, qp) if qp.is_cuda else None
+    if norms is not None and torch.is_grad_enabled() and any(
+            t.requires_grad for t in (qp, kp, norms[0], norms[1])):
+        norms = None
     if norms is not None:
         return qk_norm_rope(qp, kp, norms[0], norms[1], cos, sin, positions, eps=norms[2])
     q, k = _own_norm(self.q_norm, qp, nh, hd), _own_norm(self.k_norm, kp, nkv, hd)
