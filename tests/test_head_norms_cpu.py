@@ -191,3 +191,17 @@ def test_gradients_take_the_modules_own_norms(monkeypatch):
         assert used is None and qo.requires_grad == q and ko.requires_grad == k
     used, (qo, ko) = _choice(monkeypatch, pos)             # of the norms' weights alone
     assert used is None and qo.requires_grad and ko.requires_grad
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int16, torch.int64])
+@pytest.mark.parametrize("rows", [1, 2])
+def test_positions_of_any_whole_type_are_taken(monkeypatch, dtype, rows):
+    pos = torch.arange(4, 4 + 3 * rows).view(rows, 3)
+    with torch.no_grad():
+        (args, _), _ = _choice(monkeypatch, pos.to(dtype))
+        assert args[6].dtype == torch.int64 and torch.equal(args[6], pos)
+        want = _choice(monkeypatch, pos, norms=[Centered(), Centered()])[1]
+        got = _choice(monkeypatch, pos.to(dtype), norms=[Centered(), Centered()])[1]
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        (args, _), _ = _choice(monkeypatch, 4)
+        assert args[6] == 4

@@ -186,9 +186,11 @@ def _own_norm(norm, x: torch.Tensor, heads: int, head_dim: int) -> torch.Tensor:
 def _normed_qk(self, qp, kp, nh: int, nkv: int, hd: int, cos, sin, positions):
     """Queries and keys of an attention with ``q_norm`` / ``k_norm``: the queries normalised and
     rotated, the keys normalised (the cache holds them before the rotation), head-major.
-    ``positions``: int64 ``[1 or B, T]``, or the first one as an int.  The fused kernel has no
-    gradients: where some are wanted, of the projections or of the norms' weights, the modules'
-    own norms run."""
+    ``positions``: ``[1 or B, T]`` of a whole type, or the first one as an int.  The fused kernel
+    has no gradients: where some are wanted, of the projections or of the norms' weights, the
+    modules' own norms run."""
+    if isinstance(positions, torch.Tensor):
+        positions = positions.to(qp.device, torch.int64)
     norms = _head_norms(self, hd, qp) if qp.is_cuda else None
     if norms is not None and torch.is_grad_enabled() and any(
             t.requires_grad for t in (qp, kp, norms[0], norms[1])):
@@ -322,7 +324,7 @@ def create_spectral_forward_inference(block_size: int = 512, k_rank_keys: int = 
         if position_ids is not None:
             pid = position_ids.reshape(-1, position_ids.shape[-1])[:, -1:].to(hidden_states.device)
         if normed:
-            q, k_pre = _normed_qk(self, qp, kp, nh, nkv, hd, cos, sin, qpos if pid is None else pid.long())
+            q, k_pre = _normed_qk(self, qp, kp, nh, nkv, hd, cos, sin, qpos if pid is None else pid)
         elif (hidden_states.is_cuda and cos.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous()
                 and qp.stride(-1) == 1 and (pid is None or pid.shape[0] in (1, bsz))):
             # one launch (spx_rope_rows), the same float32 arithmetic as apply_rope below
