@@ -205,3 +205,16 @@ def test_positions_of_any_whole_type_are_taken(monkeypatch, dtype, rows):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         (args, _), _ = _choice(monkeypatch, 4)
         assert args[6] == 4
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float64, D), (torch.float32, 1026)])
+def test_what_the_fused_kernel_does_not_take_runs_the_modules_norms(monkeypatch, dtype, dim):
+    monkeypatch.setattr(I, "qk_norm_rope", lambda *a, **kw: pytest.fail("handed to the kernel"))
+    norm, x = Norm(dtype, dim), torch.linspace(-1, 1, 2 * 2 * dim, dtype=dtype).view(1, 2, 2 * dim)
+    tab = torch.zeros(4, dim)
+    with torch.no_grad():
+        q, k = I._normed_qk(SimpleNamespace(q_norm=norm, k_norm=norm), x.as_subclass(_Cuda), x.as_subclass(_Cuda), 2, 2, dim,
+                            tab.cos(), tab.sin(), 0)
+        want = norm(x.view(1, 2, 2, dim)).transpose(1, 2)
+    assert k.dtype == dtype and torch.equal(k.as_subclass(torch.Tensor), want)
+    assert torch.equal(q.as_subclass(torch.Tensor), want.float().to(dtype))      # cos 1, sin 0; rotated in float32

@@ -155,6 +155,8 @@ def _head_norms(self, head_dim: int, like: torch.Tensor):
     ``like`` that compute the usual RMS norm (this package's, or one that names its epsilon
     ``variance_epsilon`` and gives the formula's values), without forward hooks -- else None."""
     from .llama_loop import RMSNorm
+    if like.dtype not in (torch.float32, torch.float16, torch.bfloat16) or head_dim > 1024:
+        return None      # not of the kernel's types and sizes
     found = []
     for norm in (self.q_norm, self.k_norm):
         w = getattr(norm, "weight", None)
