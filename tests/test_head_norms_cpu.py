@@ -218,3 +218,21 @@ def test_what_the_fused_kernel_does_not_take_runs_the_modules_norms(monkeypatch,
         want = norm(x.view(1, 2, 2, dim)).transpose(1, 2)
     assert k.dtype == dtype and torch.equal(k.as_subclass(torch.Tensor), want)
     assert torch.equal(q.as_subclass(torch.Tensor), want.float().to(dtype))      # cos 1, sin 0; rotated in float32
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+@pytest.mark.parametrize("positions", [7, torch.tensor([[4, 0, 9]]), torch.tensor([[4, 5, 6], [19, 2, 40]])])
+def test_only_the_rows_in_use_of_tables_in_another_type_are_converted(monkeypatch, dtype, positions):
+    """A rotary module's tables in the model's type: thousands of rows, of which a step needs a few."""
+    seen = []
+    monkeypatch.setattr(I, "qk_norm_rope", lambda *a, **kw: seen.append(a))
+    x = torch.zeros(2, 3, 2 * D).as_subclass(_Cuda)
+    ang = torch.outer(torch.arange(20.0), torch.linspace(0.1, 1, D))
+    cos, sin = ang.cos().to(dtype), ang.sin().to(dtype)
+    with torch.no_grad():
+        I._normed_qk(SimpleNamespace(q_norm=Norm(), k_norm=Norm()), x, x, 2, 2, D, cos, sin, positions)
+    c, s, at = (v.as_subclass(torch.Tensor) for v in seen[0][4:7])
+    idx = torch.arange(7, 10)[None] if isinstance(positions, int) else positions.clamp(max=19)     # clamped to the tables
+    assert c.dtype == s.dtype == torch.float32 and len(c) == len(s) == idx.numel() and at.dtype == torch.int64
+    assert c.is_contiguous() and s.is_contiguous() and at.shape == idx.shape
+    assert torch.equal(c[at], cos[idx].float()) and torch.equal(s[at], sin[idx].float())

@@ -198,6 +198,13 @@ def _normed_qk(self, qp, kp, nh: int, nkv: int, hd: int, cos, sin, positions):
             t.requires_grad for t in (qp, kp, norms[0], norms[1])):
         norms = None
     if norms is not None:
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            # tables in the model's type: the rows in use become float32, not the whole tables
+            if not isinstance(positions, torch.Tensor):
+                positions = torch.arange(positions, positions + qp.shape[1], device=cos.device)[None]
+            rows = positions.reshape(-1).clamp(0, cos.shape[0] - 1)
+            cos, sin = cos[rows].float(), sin[rows].float()
+            positions = torch.arange(rows.numel(), device=rows.device).view(positions.shape)
         return qk_norm_rope(qp, kp, norms[0], norms[1], cos, sin, positions, eps=norms[2])
     q, k = _own_norm(self.q_norm, qp, nh, hd), _own_norm(self.k_norm, kp, nkv, hd)
     if not isinstance(positions, torch.Tensor):
