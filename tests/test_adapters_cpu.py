@@ -86,3 +86,56 @@ def test_a_generation_that_fails_to_start_leaves_the_adapters_as_they_were():
     with pytest.raises(RuntimeError):                            # the rows cannot be grouped on the CPU
         model.generate(torch.zeros(2, 3, dtype=torch.long), 1, adapters=ad, adapter_slots=[0, 1])
     assert ad.batch is before
+
+
+class _Packed(torch.nn.Module):
+    """A projection whose weight is packed: its sizes and type do not show in it."""
+
+    def __init__(self, linear, compute_dtype=None, **sizes):
+        super().__init__()
+        n = linear.weight.numel()
+        self.weight = torch.nn.Parameter(torch.zeros(n // 2, 1, dtype=torch.uint8), requires_grad=False)
+        self.in_features, self.out_features = linear.weight.shape[1], linear.weight.shape[0]
+        if compute_dtype is not None:
+            self.compute_dtype = compute_dtype
+
+
+def _pack(model, dtype):
+    for layer in model.model.layers:
+        layer.self_attn.spx_qkv_weight = None
+        for m, names in ((layer.self_attn, LoraAdapters.ATTENTION), (layer.mlp, LoraAdapters.MLP)):
+            for n in names:
+                setattr(m, n, _Packed(getattr(m, n), dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_packed_projections_take_adapters(dtype):
+    model = _model()
+    want = {n: tuple(getattr(m, n).weight.shape) for m, names in
+            ((model.model.layers[0].self_attn, LoraAdapters.ATTENTION), (model.model.layers[0].mlp, LoraAdapters.MLP))
+            for n in names}
+    _pack(model, dtype)
+    ad = LoraAdapters(model, max_rank=4, slots=2)
+    assert len(ad._pools) == 2 * len(want)
+    for (i, n), (pool, part) in ad._pools.items():
+        assert (pool.out_features, pool.in_features) == want[n] and pool.dtype == dtype and part == 0
+    ad.load(1, {(1, "down_proj"): (torch.ones(2, 96), torch.ones(64, 2))})
+    assert ad._pools[1, "down_proj"][0].ranks[1, 0] == 2
+
+
+def test_the_type_of_packed_projections():
+    """The model's own type comes before the one that a projection computes in: outputs come in the
+    type of the inputs."""
+    model = _model()
+    _pack(model, torch.float16)
+    model.dtype = torch.bfloat16
+    assert LoraAdapters(model, max_rank=4, slots=2)._pools[0, "q_proj"][0].dtype == torch.bfloat16
+    for dtype in (None, torch.float32):
+        model = _model()
+        _pack(model, dtype)
+        with pytest.raises(TypeError, match="layer 0: q_proj"):
+            LoraAdapters(model, max_rank=4, slots=2)
+        assert _held(model) == [None] * 4
+    model = SpectralLlama(SHAPE, device="cpu", dtype=torch.float32)
+    with pytest.raises(TypeError, match="layer 0: q_proj"):
+        LoraAdapters(model, max_rank=4, slots=2)

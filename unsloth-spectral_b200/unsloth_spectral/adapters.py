@@ -139,6 +139,25 @@ def adapted(module, name: str, y: torch.Tensor, x: torch.Tensor) -> torch.Tensor
     return pool.add(y, x, owner.batch, out=y)
 
 
+def _projection(where: str, module, model_dtype):
+    """``(in, out, dtype, device)`` of a projection.  A packed weight (4 bits a value, say) shows
+    neither its sizes nor the type of the products: the module's ``in_features`` and
+    ``out_features`` do, and the model's ``dtype`` or else the module's ``compute_dtype``."""
+    w = module.weight
+    if w.dim() == 2 and w.dtype.is_floating_point:
+        n_out, n_in = w.shape
+    else:
+        n_in, n_out = getattr(module, "in_features", None), getattr(module, "out_features", None)
+    types = (torch.float16, torch.bfloat16)
+    held = (w.dtype,) if w.dtype.is_floating_point and w.dtype.itemsize > 1 else (
+        model_dtype, getattr(module, "compute_dtype", None))
+    dtype = next((t for t in held if t in types), None)
+    if dtype is None or n_in is None or n_out is None:
+        raise TypeError(f"{where} takes no adapters: its weight is {w.dtype} {tuple(w.shape)}, and float16 or bfloat16 "
+                        f"products of known sizes are expected")
+    return n_in, n_out, dtype, w.device
+
+
 class LoraAdapters:
     """The adapters of a model: a ``LoraPool`` for every projection of its layers named in
     ``targets``.  ``model`` is a ``SpectralLlama`` or any model that ``patch_unsloth_attention``
@@ -162,7 +181,7 @@ class LoraAdapters:
         self.batch: Optional[LoraBatch] = None
         self.slots, self.targets = slots, tuple(targets)
         self._pools: Dict[Tuple[int, str], Tuple[LoraPool, int]] = {}
-        make = lambda w, out: LoraPool(w.shape[1], out, max_rank, slots, w.dtype, w.device)  # noqa: E731
+        model_dtype = getattr(model, "dtype", None)
         layers = model.model.layers
         covered = []           # (module, its pools), attached when all of them are there
         for i, layer in enumerate(layers):
@@ -173,25 +192,31 @@ class LoraAdapters:
                 if set(targets) & set(names) and getattr(module, "spx_lora", None) is not None:
                     raise ValueError(f"layer {i}: {type(module).__name__} has the adapters of another LoraAdapters; "
                                      f"detach() that first")
+            shape = {n: _projection(f"layer {i}: {n}", getattr(module, n), model_dtype)
+                     for module, names in ((attn, self.ATTENTION), (mlp, self.MLP)) for n in names if n in targets}
+
+            def make(name, out=None):
+                n_in, n_out, dtype, device = shape[name]
+                return LoraPool(n_in, n_out if out is None else out, max_rank, slots, dtype, device)
+
             held = {}
             qkv = [n for n in self.ATTENTION[:3] if n in targets]
             if qkv and getattr(attn, "spx_qkv_weight", None) is not None:
-                widths = [getattr(attn, n).weight.shape[0] for n in self.ATTENTION[:3]]
-                held["qkv"] = make(attn.spx_qkv_weight, widths)
+                held["qkv"] = make(qkv[0], [getattr(attn, n).weight.shape[0] for n in self.ATTENTION[:3]])
                 for n in qkv:
                     self._pools[i, n] = held["qkv"], self.ATTENTION.index(n)
             else:
                 for n in qkv:
-                    held[n] = make(getattr(attn, n).weight, getattr(attn, n).weight.shape[0])
+                    held[n] = make(n)
                     self._pools[i, n] = held[n], 0
             if "o_proj" in targets:
-                held["o_proj"] = make(attn.o_proj.weight, attn.o_proj.weight.shape[0])
+                held["o_proj"] = make("o_proj")
                 self._pools[i, "o_proj"] = held["o_proj"], 0
             covered.append((attn, held))
             held = {}
             for n in self.MLP:
                 if n in targets:
-                    held[n] = make(getattr(mlp, n).weight, getattr(mlp, n).weight.shape[0])
+                    held[n] = make(n)
                     self._pools[i, n] = held[n], 0
             covered.append((mlp, held))
         self.device = layers[0].self_attn.o_proj.weight.device
