@@ -1,4 +1,6 @@
 """LoraAdapters on the host: which modules a set holds, and what it refuses (no GPU)."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -139,3 +141,22 @@ def test_the_type_of_packed_projections():
     model = SpectralLlama(SHAPE, device="cpu", dtype=torch.float32)
     with pytest.raises(TypeError, match="layer 0: q_proj"):
         LoraAdapters(model, max_rank=4, slots=2)
+
+
+def test_a_model_on_two_devices_has_a_batch_on_each():
+    """The second layer's pool on another device (here one that takes the call down): it gets the
+    batch there, kept with the one that is in use."""
+    model, far, calls = _model(), torch.device("meta"), []
+    ad = LoraAdapters(model, max_rank=4, slots=2, targets=("o_proj",))
+    pool = SimpleNamespace(device=far, add=lambda y, x, batch, out: calls.append(batch) or out)
+    model.model.layers[1].self_attn.spx_lora[1]["o_proj"] = pool
+    ad._pools[1, "o_proj"] = (pool, 0)
+    ad.use([1, -1])
+    assert ad.batch.device == ad.device == torch.device("cpu") and ad.batch.slots == (1, -1)
+    x = torch.zeros(2, 1, 64, dtype=torch.bfloat16)
+    for _ in range(2):
+        assert adapted(model.model.layers[1].self_attn, "o_proj", x, x) is x
+    assert calls[0] is calls[1] and calls[0].device == far and calls[0].slots == (1, -1)
+    assert ad.batch.on(torch.device("cpu")) is ad.batch and ad.batch.on(far) is calls[0]
+    with pytest.raises(RuntimeError):                            # the first layer's: reaches the pool on the CPU
+        adapted(model.model.layers[0].self_attn, "o_proj", x, x)

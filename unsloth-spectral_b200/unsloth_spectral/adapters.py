@@ -39,6 +39,15 @@ class LoraBatch:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self._front = N.front().Batch(self.slots, self.device)
         self.highest = self._front.highest
+        self._elsewhere: Dict[torch.device, "LoraBatch"] = {}
+
+    def on(self, device: torch.device) -> "LoraBatch":
+        """This batch on ``device``: itself, or one with the same slots that is kept with it."""
+        if device == self.device:
+            return self
+        if device not in self._elsewhere:
+            self._elsewhere[device] = LoraBatch(self.slots, device)
+        return self._elsewhere[device]
 
     def __len__(self) -> int:
         return len(self.slots)
@@ -47,6 +56,8 @@ class LoraBatch:
         """Group the rows of ``tokens`` tokens per sequence now, and wait until the grouping is on
         the device."""
         self._front.prepare(tokens)
+        for other in self._elsewhere.values():
+            other.prepare(tokens)
         return self
 
     @staticmethod
@@ -136,7 +147,7 @@ def adapted(module, name: str, y: torch.Tensor, x: torch.Tensor) -> torch.Tensor
         return y
     if y.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("the adapters' products have no gradients: run the forward under torch.no_grad()")
-    return pool.add(y, x, owner.batch, out=y)
+    return pool.add(y, x, owner.batch.on(pool.device), out=y)
 
 
 def _projection(where: str, module, model_dtype):
@@ -269,4 +280,6 @@ class LoraAdapters:
         batch = LoraBatch(slots, self.device)
         if batch.highest >= self.slots:
             raise IndexError(f"slot {batch.highest} of {self.slots}")
+        for pool, _ in self._pools.values():
+            batch.on(pool.device)      # of a model that lies on several devices
         self.batch = batch
