@@ -83,12 +83,17 @@ def build(jobs: int = 0, force: bool = False, verbose: bool = False, ptxas_verbo
 
 
 def build_front(force: bool = False) -> str:
-    src = os.path.join(CSRC, "spx_front.cpp")
-    if not force and not _stale(FRONT, [src, os.path.join(INCLUDE, "spx.h"), os.path.abspath(__file__)]):
-        return FRONT
     import sysconfig
 
     import torch
+    src = os.path.join(CSRC, "spx_front.cpp")
+    # what it was built against, kept beside the objects: another torch or Python cannot load it
+    record = os.path.join(BUILD, "front.txt")
+    against = (f"torch {torch.__version__}, C++11 ABI {int(torch.compiled_with_cxx11_abi())}, "
+               f"python {sysconfig.get_config_var('SOABI')}")
+    if not force and not _stale(FRONT, [src, os.path.join(INCLUDE, "spx.h"), os.path.abspath(__file__)]):
+        if os.path.exists(record) and open(record).read() == against:
+            return FRONT
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     inc = [INCLUDE, os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
@@ -102,6 +107,9 @@ def build_front(force: bool = False) -> str:
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError("g++ failed for spx_front.cpp")
+    os.makedirs(BUILD, exist_ok=True)
+    with open(record, "w") as f:
+        f.write(against)
     return FRONT
 
 
