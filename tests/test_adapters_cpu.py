@@ -4,7 +4,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from unsloth_spectral import LoraAdapters
+from unsloth_spectral import LoraAdapters, LoraPool
 from unsloth_spectral.adapters import adapted
 from unsloth_spectral.llama_loop import LlamaShape, SpectralLlama
 
@@ -160,3 +160,16 @@ def test_a_model_on_two_devices_has_a_batch_on_each():
     assert ad.batch.on(torch.device("cpu")) is ad.batch and ad.batch.on(far) is calls[0]
     with pytest.raises(RuntimeError):                            # the first layer's: reaches the pool on the CPU
         adapted(model.model.layers[0].self_attn, "o_proj", x, x)
+
+
+def test_an_adapter_made_from_a_slots_own_storage():
+    """A slot's own rows and columns, scaled or cut to a smaller rank, put back into it."""
+    pool = LoraPool(16, (24, 8), max_rank=4, slots=2, device="cpu")
+    A, B = torch.randn(4, 16), torch.randn(24, 4)
+    pool.load(1, A, B, 2.0)
+    a, b = pool.a.clone(), pool.b.clone()
+    pool.load(1, pool.a[1, 0, :4], pool.b[1, :24, :4], 1.0)
+    assert torch.equal(pool.a, a) and torch.equal(pool.b, b) and pool.scales[1, 0] == 1.0
+    pool.load(1, pool.a[1, 0, 1:4], pool.b[1, :24, 1:4], 0.5)    # rows that overlap their new places
+    assert torch.equal(pool.a[1, 0, :3], a[1, 0, 1:4]) and torch.equal(pool.b[1, :24, :3], b[1, :24, 1:4])
+    assert not pool.a[1, 0, 3:].any() and not pool.b[1, :24, 3:].any() and pool.ranks[1, 0] == 3

@@ -115,6 +115,9 @@ class LoraPool:
             raise ValueError(f"scale must be finite, got {scale}")
         at = sum(self.widths[:part])
         with torch.no_grad():
+            # what lies in the pool itself is read before its place is cleared
+            A, B = (t.clone() if t.untyped_storage().data_ptr() == held.untyped_storage().data_ptr() else t
+                    for t, held in ((A, self.a), (B, self.b)))
             self.a[slot, part].zero_()
             self.a[slot, part, :r].copy_(A)
             self.b[slot, at:at + w].zero_()
