@@ -227,3 +227,19 @@ def test_out_over_another_place_of_the_input_is_refused():
                                (rules.apply, room[:, :10], {}, room[:, 10:20]), (rules.apply, room[:, :10], {}, room[:, :10])):
         with pytest.raises(N.SpxUnavailable):
             call(y, **more, out=out)
+
+
+def test_settings_past_float32_are_refused():
+    """The kernels hold them in float32: 1e39 is an infinity there, 1e-46 zero."""
+    for bad in (dict(repetition_penalty=1e39), dict(repetition_penalty=1e-46), dict(frequency_penalty=[0.0, 1e39]),
+                dict(presence_penalty=-1e39), dict(logit_bias={3: 1e39})):
+        with pytest.raises(ValueError):
+            LogitsRules(**{**dict(batch=2, vocab=50, device="cpu"), **bad})
+    r = LogitsRules(2, 50, device="cpu", repetition_penalty=1e-38, presence_penalty=3e38,
+                    logit_bias={3: -1e39, 4: 3e38, 5: float("-inf")})
+    assert r._bias[2].tolist()[:3] == [float("-inf"), pytest.approx(3e38), float("-inf")]
+    pool = LoraPool(16, 24, max_rank=4, slots=2, device="cpu")
+    for scale in (1e39, -1e39):
+        with pytest.raises(ValueError):
+            pool.load(0, torch.ones(2, 16), torch.ones(24, 2), scale)
+    assert not pool.ranks.any()

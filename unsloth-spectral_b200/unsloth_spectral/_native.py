@@ -244,6 +244,11 @@ def front():
     return _spx_front
 
 
+def f32(v) -> float:
+    """A number as the kernels hold it: rounded to float32, an infinity past its range."""
+    return C.c_float(float(v)).value
+
+
 def on_device(device: torch.device, fn, *args):
     """``fn(*args)`` with ``device`` current."""
     if device.index is None or device.index == torch.cuda.current_device():

@@ -111,7 +111,7 @@ class LoraPool:
         if A.shape != (r, self.in_features) or B.shape != (w, r) or not 1 <= r <= self.max_rank:
             raise ValueError(f"A must be [rank, {self.in_features}] and B [{w}, rank] with rank 1..{self.max_rank}, "
                              f"got {tuple(A.shape)} and {tuple(B.shape)}")
-        if not math.isfinite(scale):
+        if not math.isfinite(N.f32(scale)):
             raise ValueError(f"scale must be finite, got {scale}")
         at = sum(self.widths[:part])
         with torch.no_grad():

@@ -50,7 +50,7 @@ class LogitsRules:
         words = allow_words(vocab)
         rep = _setting("repetition_penalty", repetition_penalty, batch)
         if any(v <= 0 for v in rep):
-            raise ValueError("repetition_penalty must be positive")
+            raise ValueError("repetition_penalty must be positive, in float32 too")
         freq = _setting("frequency_penalty", frequency_penalty, batch)
         pres = _setting("presence_penalty", presence_penalty, batch)
         rows, toks, vals = _biases(logit_bias, batch, vocab)
@@ -119,7 +119,7 @@ class LogitsRules:
 
 
 def _setting(name: str, v: Setting, batch: int):
-    vals = [float(v)] * batch if isinstance(v, (int, float)) else [float(x) for x in v]
+    vals = [N.f32(v)] * batch if isinstance(v, (int, float)) else [N.f32(x) for x in v]
     if len(vals) != batch or not all(math.isfinite(x) for x in vals):
         raise ValueError(f"{name} must be one finite number or {batch} of them, got {v!r}")
     return vals
@@ -133,7 +133,7 @@ def _biases(bias, batch: int, vocab: int):
     rows, toks, vals = [], [], []
     for b, d in enumerate(each):
         for t in sorted(d or {}):
-            v = float(d[t])
+            v = N.f32(d[t])
             if not isinstance(t, int) or not 0 <= t < vocab or math.isnan(v) or v == math.inf:
                 raise ValueError(f"logit_bias {{{t!r}: {d[t]!r}}}: a token 0..{vocab - 1} and a number (or -inf) expected")
             rows.append(b)
