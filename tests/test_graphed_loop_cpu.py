@@ -55,3 +55,24 @@ def test_what_the_side_stream_reads_was_issued_before_it_waits(monkeypatch, n):
     assert start < end
     assert [e for e in log[start:end] if e[:2] == ("op", "main")] == []
     assert [e for e in log[:start] + log[end:] if e[:2] == ("op", "side")] == []
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("n", [0, 1, 3])
+def test_as_many_tokens_are_recorded_as_are_returned(n, graphs, monkeypatch):
+    _Streams(monkeypatch)
+    picked = []
+
+    def pick(logits, allow, record):
+        assert record
+        picked.append(logits.argmax(-1))
+        return picked[-1]
+
+    rules = SimpleNamespace(reset=picked.clear, observe_prompt=lambda ids: None, pick=pick)
+    caches = [SimpleNamespace(tiers=SimpleNamespace(num_blocks=0, hot_len=0), block_size=512)]
+    step = lambda tok: torch.nn.functional.one_hot(tok + 1, 50).float()  # noqa: E731
+    model = SimpleNamespace(prefill=lambda ids: (step(ids[:, -1]), caches), decode_step=lambda tok, pos, caches: step(tok))
+    model._decode_graphed = lambda *a: SpectralLlama._decode_graphed(model, *a)
+    out = SpectralLlama.generate(model, torch.tensor([[1, 4], [2, 9]]), n, cuda_graphs=graphs, rules=rules)
+    assert out.shape == (2, n) and len(picked) == n
+    assert torch.equal(out, torch.stack(picked, 1) if n else out)

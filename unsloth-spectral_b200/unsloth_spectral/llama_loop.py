@@ -244,18 +244,19 @@ class SpectralLlama(torch.nn.Module):
         if timer is not None:
             timer("prefill")
         out = torch.empty(B, max_new_tokens, dtype=torch.long, device=input_ids.device)
-        tok = choose(logits)
-        pos = torch.full((1, 1), T, dtype=torch.long, device=input_ids.device)
-        if cuda_graphs:
-            self._decode_graphed(tok, pos, caches, out, choose)
-        else:
-            for s in range(max_new_tokens):
-                out[:, s] = tok
-                if s + 1 == max_new_tokens:
-                    break
-                logits = self.decode_step(tok, pos, caches)
-                tok = choose(logits)
-                pos += 1
+        if max_new_tokens > 0:     # a token that is not returned is not chosen (nor recorded) either
+            tok = choose(logits)
+            pos = torch.full((1, 1), T, dtype=torch.long, device=input_ids.device)
+            if cuda_graphs:
+                self._decode_graphed(tok, pos, caches, out, choose)
+            else:
+                for s in range(max_new_tokens):
+                    out[:, s] = tok
+                    if s + 1 == max_new_tokens:
+                        break
+                    logits = self.decode_step(tok, pos, caches)
+                    tok = choose(logits)
+                    pos += 1
         if timer is not None:
             timer("decode")
         self._caches = caches
