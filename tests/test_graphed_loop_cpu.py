@@ -76,3 +76,17 @@ def test_as_many_tokens_are_recorded_as_are_returned(n, graphs, monkeypatch):
     out = SpectralLlama.generate(model, torch.tensor([[1, 4], [2, 9]]), n, cuda_graphs=graphs, rules=rules)
     assert out.shape == (2, n) and len(picked) == n
     assert torch.equal(out, torch.stack(picked, 1) if n else out)
+
+
+def test_layers_patched_for_dense_attention_decode_eagerly(monkeypatch):
+    """Dense attention takes the context's length from the host at every step: no step is captured."""
+    from unsloth_spectral.llama_loop import LlamaShape
+    _Streams(monkeypatch)
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda: pytest.fail("a step was captured"))
+    real = SpectralLlama(LlamaShape(layers=1, hidden=64, heads=4, kv_heads=2, head_dim=16, ffn=96, vocab=50), device="cpu")
+    real.patch(block_size=512, use_spectral_attention=False)
+    caches = [SimpleNamespace(tiers=SimpleNamespace(num_blocks=1, hot_len=0), block_size=512)]
+    real.decode_step = lambda tok, pos, caches: torch.nn.functional.one_hot(tok + 1, 50).float()
+    out = torch.zeros(1, 8, dtype=torch.long)
+    real._decode_graphed(torch.tensor([3]), torch.zeros(1, 1, dtype=torch.long), caches, out, lambda logits: logits.argmax(-1))
+    assert out.tolist() == [list(range(3, 11))]

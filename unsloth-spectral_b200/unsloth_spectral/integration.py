@@ -371,6 +371,7 @@ def patch_unsloth_attention(model, block_size: int = 512, k_rank_keys: int = 16,
                                           hot_buffer_size, use_spectral_attention, debug_logging,
                                           use_attention_weighted_svd, landmark_count)
             layer.self_attn.forward = fwd.__get__(layer.self_attn, type(layer.self_attn))
+            layer.self_attn._spx_dense = not use_spectral_attention
             layer.self_attn._spx_inference = create_spectral_forward_inference(
                 block_size, k_rank_keys, k_rank_values, hot_buffer_size, use_spectral_attention, debug_logging,
                 use_triton_kernel, use_attention_weighted_svd, landmark_count).__get__(

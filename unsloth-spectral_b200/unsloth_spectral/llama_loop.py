@@ -283,9 +283,10 @@ class SpectralLlama(torch.nn.Module):
             while s + 1 < n:
                 t0 = caches[0].tiers
                 room = caches[0].block_size - 1 - t0.hot_len   # appends before one fills a block
-                # before the first full block a step runs the dense attention, whose length is a
-                # host argument: eager steps too
-                if t0.num_blocks == 0 or room < 3 or n - 1 - s < 3:
+                # before the first full block, and in layers that are patched to keep it, a step runs
+                # the dense attention, whose length is a host argument: eager steps too
+                if t0.num_blocks == 0 or room < 3 or n - 1 - s < 3 or any(
+                        layer.self_attn._spx_dense for layer in self.model.layers):
                     logits = self.decode_step(tok, pos, caches)
                     tok.copy_(choose(logits))
                     pos.add_(1)
