@@ -244,6 +244,8 @@ struct Batch {
     for (const bool blocks : {false, true})
       if (!blocks || tokens >= kBlockTokens) {
         Plan& p = plan(tokens, blocks);
+        if (p.there) continue;
+        const c10::cuda::CUDAStreamCaptureModeGuard allowed(cudaStreamCaptureModeRelaxed);   // of an earlier, uncaptured copy
         p.copied.synchronize();
         p.there = true;
       }
