@@ -38,3 +38,21 @@ def test_a_batch_is_prepared_again_inside_a_capture(T, waited):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def test_one_row_of_wider_rows_off_16_bytes():
+    """One row has no distance to another: views of rows whose width is no multiple of 8."""
+    from unsloth_spectral import LoraBatch
+    g = torch.Generator(device="cuda").manual_seed(3)
+    pool = _pool(g)
+    x, y = (torch.randn(1, 1, n, generator=g, device="cuda").bfloat16() for n in (256, 136))
+    want = pool.add(y, x, LoraBatch([1]))
+    for shape in ((1, 1, 303), (1, 303)):
+        n = len(shape)
+        xw, yw, ow = (torch.full(shape, 2.0, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+        xv, yv, ov = xw[..., :256], yw[..., 8:144], ow[..., 16:152]
+        xv.copy_(x.view(xv.shape)), yv.copy_(y.view(yv.shape))
+        got = pool.add(yv, xv, LoraBatch([1]), out=ov)
+        assert got.dim() == n and torch.equal(got.flatten(), want.flatten())
+        assert (ow[..., :16] == 2).all() and (ow[..., 152:] == 2).all()
+        assert torch.equal(pool.add(yv, xv, LoraBatch([1])).flatten(), want.flatten())

@@ -252,10 +252,11 @@ struct Batch {
   }
 };
 
-// The distance between the rows of t [.., n], which must be even.
+// The distance between the rows of t [.., n], which must be even (one row: any, so its length).
 int64_t row_stride(const Tensor& t) {
   TORCH_CHECK_VALUE(t.stride(-1) == 1, "the last dimension must be contiguous, got strides ", t.strides());
-  if (t.dim() == 2 || t.size(1) == 1) return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(-1));
+  if (t.numel() == t.size(-1)) return t.size(-1);
+  if (t.dim() == 2 || t.size(1) == 1) return t.stride(0);
   TORCH_CHECK_VALUE(t.size(0) == 1 || t.stride(0) == t.size(1) * t.stride(1), "rows must be evenly spaced, got strides ",
                     t.strides(), " of ", t.sizes());
   return t.stride(1);
