@@ -354,13 +354,8 @@ int launch_shrink_rows(const Params& p, int tiles, int tile_rows, cudaStream_t s
   // against 6.8 with 48), else as many as leave the rows enough warps: each group reads x again.
   const int cols = (int64_t)tiles * (p.SR / 16) * 8 <= 2 * 148 ? 16 : tile_rows == 16 ? 32 : 64;
   const int groups = (p.SR + cols - 1) / cols;
-  const int nt = ((p.SR / 8 + groups - 1) / groups + 1) / 2 * 2;  // 2, 4, 6 or 8
-  if (tile_rows == 16) {
-    return nt == 2   ? launch_shrink<T, 1, 2>(p, tiles, groups, st)
-           : nt == 4 ? launch_shrink<T, 1, 4>(p, tiles, groups, st)
-           : nt == 6 ? launch_shrink<T, 1, 6>(p, tiles, groups, st)
-                     : launch_shrink<T, 1, 8>(p, tiles, groups, st);
-  }
+  const int nt = ((p.SR / 8 + groups - 1) / groups + 1) / 2 * 2;  // 2, 4, 6 or 8; 2 or 4 of up to 32 columns
+  if (tile_rows == 16) return nt == 2 ? launch_shrink<T, 1, 2>(p, tiles, groups, st) : launch_shrink<T, 1, 4>(p, tiles, groups, st);
   return nt == 2   ? launch_shrink<T, 2, 2>(p, tiles, groups, st)
          : nt == 4 ? launch_shrink<T, 2, 4>(p, tiles, groups, st)
          : nt == 6 ? launch_shrink<T, 2, 6>(p, tiles, groups, st)
