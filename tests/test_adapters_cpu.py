@@ -173,3 +173,22 @@ def test_an_adapter_made_from_a_slots_own_storage():
     pool.load(1, pool.a[1, 0, 1:4], pool.b[1, :24, 1:4], 0.5)    # rows that overlap their new places
     assert torch.equal(pool.a[1, 0, :3], a[1, 0, 1:4]) and torch.equal(pool.b[1, :24, :3], b[1, :24, 1:4])
     assert not pool.a[1, 0, 3:].any() and not pool.b[1, :24, 3:].any() and pool.ranks[1, 0] == 3
+
+
+@pytest.mark.parametrize("bad", [(torch.ones(2, 64), torch.ones(63, 2)), (torch.ones(9, 64), torch.ones(64, 9)),
+                                 (torch.ones(2, 63), torch.ones(64, 2)), (torch.ones(64), torch.ones(64, 2))])
+def test_a_refused_adapter_leaves_the_one_in_the_slot(bad):
+    model = _model()
+    ad = LoraAdapters(model, max_rank=4, slots=2)
+    good = {(i, "q_proj"): (torch.full((3, 64), i + 1.0), torch.ones(64, 3)) for i in range(2)}
+    ad.load(1, good, scale=2.0)
+    pools = [ad._pools[i, "q_proj"][0] for i in range(2)]
+    before = [(p.a.clone(), p.b.clone(), p.ranks.clone(), p.scales.clone()) for p in pools]
+    for weights, scale in (({(0, "q_proj"): good[0, "q_proj"], (1, "o_proj"): bad}, 1.0), (good, float("nan"))):
+        with pytest.raises(ValueError):
+            ad.load(1, weights, scale)
+        for p, held in zip(pools, before):
+            assert all(torch.equal(u, v) for u, v in zip((p.a, p.b, p.ranks, p.scales), held))
+    for slot in (-1, 2):
+        with pytest.raises(IndexError):
+            ad.load(slot, good)

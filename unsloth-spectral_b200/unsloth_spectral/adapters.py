@@ -101,18 +101,22 @@ class LoraPool:
         if not 0 <= slot < self.slots or not 0 <= part < len(self.widths):
             raise IndexError(f"slot {slot}, part {part} of a pool of {self.slots} slots, {len(self.widths)} parts")
 
-    def load(self, slot: int, A: torch.Tensor, B: torch.Tensor, scale: float = 1.0, part: int = 0):
-        """Put an adapter's ``A [rank, in_features]``, ``B [width, rank]`` and scale
-        (alpha / rank) into a slot; its other parts keep what they hold (nothing at first:
-        the shared projection alone)."""
+    def _fits(self, slot: int, A: torch.Tensor, B: torch.Tensor, scale: float, part: int) -> Tuple[int, int]:
+        """The width of a part and the rank of an adapter that is to go there; raises when it cannot."""
         self._slot(slot, part)
-        w = self.widths[part]
-        r = A.shape[0]
+        w, r = self.widths[part], A.shape[0] if A.dim() == 2 else 0
         if A.shape != (r, self.in_features) or B.shape != (w, r) or not 1 <= r <= self.max_rank:
             raise ValueError(f"A must be [rank, {self.in_features}] and B [{w}, rank] with rank 1..{self.max_rank}, "
                              f"got {tuple(A.shape)} and {tuple(B.shape)}")
         if not math.isfinite(N.f32(scale)):
             raise ValueError(f"scale must be finite, got {scale}")
+        return w, r
+
+    def load(self, slot: int, A: torch.Tensor, B: torch.Tensor, scale: float = 1.0, part: int = 0):
+        """Put an adapter's ``A [rank, in_features]``, ``B [width, rank]`` and scale
+        (alpha / rank) into a slot; its other parts keep what they hold (nothing at first:
+        the shared projection alone)."""
+        w, r = self._fits(slot, A, B, scale, part)
         at = sum(self.widths[:part])
         with torch.no_grad():
             # what lies in the pool itself is read before its place is cleared
@@ -259,6 +263,9 @@ class LoraAdapters:
         for key in weights:
             if key not in self._pools:
                 raise KeyError(f"no adapted projection {key}; targets are {self.targets}")
+        for (layer, name), (A, B) in weights.items():     # all of it fits, or the slot keeps what it holds
+            pool, part = self._pools[layer, name]
+            pool._fits(slot, A, B, scale, part)
         self.unload(slot)
         try:
             for key, (A, B) in weights.items():
