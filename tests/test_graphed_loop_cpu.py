@@ -90,3 +90,23 @@ def test_layers_patched_for_dense_attention_decode_eagerly(monkeypatch):
     out = torch.zeros(1, 8, dtype=torch.long)
     real._decode_graphed(torch.tensor([3]), torch.zeros(1, 1, dtype=torch.long), caches, out, lambda logits: logits.argmax(-1))
     assert out.tolist() == [list(range(3, 11))]
+
+
+def test_layers_without_the_patchs_mark_are_taken_for_spectral_ones(monkeypatch):
+    """A single-token forward put on the layers by hand: the loop asks only whether dense attention was
+    asked for."""
+    _Streams(monkeypatch)
+    captured = []
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda: captured.append(1) or pytest.skip("reached the capture"))
+    import unsloth_spectral.llama_loop as L
+    monkeypatch.setattr(L, "rope_tables_for", lambda *a: None)
+    tiers = SimpleNamespace(num_blocks=1, hot_len=0, hot_bound=None, ensure_hot=lambda n: None, hot_len_device=lambda: None)
+    caches = [SimpleNamespace(tiers=tiers, block_size=512, total_tokens=512)]
+    model = SimpleNamespace(model=SimpleNamespace(layers=[SimpleNamespace(self_attn=SimpleNamespace())]),
+                            decode_step=lambda tok, pos, caches: torch.nn.functional.one_hot(tok + 1, 50).float())
+    try:
+        SpectralLlama._decode_graphed(model, torch.tensor([3]), torch.zeros(1, 1, dtype=torch.long), caches,
+                                      torch.zeros(1, 8, dtype=torch.long), lambda logits: logits.argmax(-1))
+    except pytest.skip.Exception:
+        pass
+    assert captured == [1]

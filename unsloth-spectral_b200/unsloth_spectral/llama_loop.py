@@ -286,7 +286,7 @@ class SpectralLlama(torch.nn.Module):
                 # before the first full block, and in layers that are patched to keep it, a step runs
                 # the dense attention, whose length is a host argument: eager steps too
                 if t0.num_blocks == 0 or room < 3 or n - 1 - s < 3 or any(
-                        layer.self_attn._spx_dense for layer in self.model.layers):
+                        getattr(layer.self_attn, "_spx_dense", False) for layer in self.model.layers):
                     logits = self.decode_step(tok, pos, caches)
                     tok.copy_(choose(logits))
                     pos.add_(1)
