@@ -434,7 +434,8 @@ typedef struct spx_lora_args {
   const int32_t* order;        /* [num_rows]: row of x, y and out; not read with tile_rows 128 */
   float* workspace;            /* >= spx_lora_workspace_size(args) bytes: the inner products,
                                   f32 [num_rows][parts*max_rank], then an int32 that is set to 1
-                                  when a kernel's wait expired (rows of out are NaN then) */
+                                  when a kernel's wait expired after 2 s (rows of out are NaN
+                                  then); the call does not clear it: who reads it does, before */
   size_t workspace_bytes;
 } spx_lora_args;
 

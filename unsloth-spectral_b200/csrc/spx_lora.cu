@@ -4,17 +4,19 @@
 //   shrink  t = A x      (K = in_features is long, the result has `rank` columns: the warps
 //                         and the CTAs of a cluster split K, the partial sums meet in
 //                         shared and distributed shared memory in a fixed order)
-//   expand  out = y + scale * B t   (each warp owns 64 output columns and keeps their B
-//                         fragments in registers over the tile's rows)
-// Both are streams with little arithmetic (2 * rank flops a value of x and of y), so the
-// operands go from global memory straight into mma fragments.  The sum over k may take its
+//   expand  out = y + scale * B t   (each warp owns 64 output columns, or 32 at ranks above 64 and
+//                         where there are few columns, and keeps their B fragments in
+//                         registers over the tile's rows)
+// Both are streams with little arithmetic (2 * rank flops a value of x and of y), so each lane
+// fetches the values of its own mma fragments: of x and A through a ring of its own, of y and
+// B into registers.  The sum over k may take its
 // terms in any order, so lane c of a quad takes k = 8c..8c+7 of 32 as the k of two
 // m16n8k16 steps (16-byte loads, whole sectors); the same choice over the output columns
 // gives 16-byte accesses of y and out.
 // These are the kernels for few rows of a slot; prompts take spx_lora_tc.cu's.  Bound by latency
-// and by the weights: one request on q|k|v at rank 16 takes 4.8 us (two launches, the second
+// and by the weights: one request on q|k|v at rank 16 takes 4.6 us (two launches, the second
 // one waiting for the first inside the GPU), 64 requests with 24 adapters of rank 64 and 32 at
-// K = 14336 17.8 us, of which 50 MB of weights need 7.6.
+// K = 14336 18.0 us, of which 50 MB of weights need 7.6.
 // t is kept in float32; for the second product it is split into a high and a low value of
 // the row type (two MMAs), which keeps about 16 (bf16) or 22 (f16) bits of it.
 #include "spx_lora.cuh"

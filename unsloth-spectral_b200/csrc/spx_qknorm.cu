@@ -6,9 +6,10 @@
 // rotation).  Bound by memory: each value is read once and written once; the tables' rows
 // come from L2 and are held in registers over the heads of a token.
 // What it takes is warps: 8 x 4096 tokens of 32/8 heads of 128 bf16 take 115 us (floor 103)
-// with 32 warps an SM and the next vector fetched ahead; 155 with four vectors at once and 16
-// warps, 126 without fetching ahead; narrower lanes (four values of a half) 150; more warps
-// than the registers allow without spills 150 to 230.
+// with 32 warps an SM and the next vector fetched ahead, at 64 registers a thread, of which most
+// variants spill a few (8 to 60 bytes; eight lanes of bf16 28); 155 with four vectors at once and
+// 16 warps, 126 without fetching ahead; narrower lanes (four values of a half) 150; more warps
+// still 150 to 230.
 #include <type_traits>
 
 #include "spx_common.cuh"
@@ -166,8 +167,10 @@ __global__ void __launch_bounds__(kWarps<T> * 32, (sizeof(T) == 4 ? 24 : 32) / k
                         p.rotk != 0, first, p.H, step, on, h, p.eps, xa, xb, g >= p.Hq);
 }
 
-// Any even head dim, any alignment: one warp per head vector, read twice (the second time
-// from L1).
+// Any even head dim, any alignment: one warp per head vector, value by value, read twice (the
+// second time from L1).  bf16, 64 rows of 40 heads of 128 off 16 bytes 3.4 us on the device (as
+// the vector kernel on aligned ones), 8 x 4096 rows 530 us (120 aligned); heads of 72: 3 x 1037 rows
+// of 12 heads 17 us, 8 x 4096 of 40 heads 539 (58 us of bytes).
 template <typename T>
 __global__ void __launch_bounds__(ANY_WARPS * 32) any_kernel(const Params p) {
   const int lane = threadIdx.x & 31, h = p.D / 2, n = p.Hq + p.H;
@@ -224,9 +227,12 @@ int launch(const Params& p, bool vec, cudaStream_t st) {
   // one head a group (3 x 1037 rows of 12 heads of 80: 8.8 us with one group a row, 5.9 with three,
   // 7.3 with four, 7.6 with six: each group looks up its position and table row); from four on a
   // power of two, so that a warp's groups are of one row (1024 rows of 40 heads of 128: 6.6 us with
-  // eight, 6.8 with nine, 7.4 with ten).  Many rows: at most 14 heads a group (8 x 1024 rows of 40
-  // heads 41.2 us with one group a row, 33.6 with two, 32.5 with four, 33.8 with eight; of 12 heads
-  // 11.5 with one, 11.7 with two).
+  // eight, 6.8 with nine, 7.4 with ten).  Three where the SMs hold three but not four: over 80 shapes
+  // of 1315 to 6110 rows, heads of 64 to 256, against two groups, bf16 rows of 12 heads 5.7 and 6.8
+  // us, of 26 heads 9.2 and 10.2, of 20 and 40 heads level, of 8 heads 5.6 and 5.1 (float32: 12 heads
+  // 7 to 11 % less, 26 heads up to 8 % less, 8 heads 1 to 7 % more).  Many rows: at most 14 heads a
+  // group (8 x 1024 rows of 40 heads 41.2 us with one group a row, 33.6 with two, 32.5 with four, 33.8
+  // with eight; of 12 heads 11.5 with one, 11.7 with two).
   const int ng = 32 / G, most = p.Hq + p.H;
   const int64_t fit = (int64_t)148 * 16 * ng / p.rows;
   int slots = 1;

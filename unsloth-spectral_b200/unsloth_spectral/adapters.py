@@ -138,7 +138,8 @@ class LoraPool:
         """``y + scale * B (A x)`` of each sequence's slot.  ``x [B, T, in]`` (or ``[B, in]``:
         one token each) and ``y [B, T, out]`` in the pool's dtype, rows on 16 bytes and evenly
         spaced; ``out`` may be ``y`` itself (in place) or lie beside it, without it a new tensor is
-        returned."""
+        returned.  The call does not wait for the GPU: should a copy inside a kernel fail to arrive
+        within 2 s, the rows that it was for come out as NaN."""
         return self._add(y, x, batch._front, out)
 
 
