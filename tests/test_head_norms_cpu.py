@@ -236,3 +236,18 @@ def test_only_the_rows_in_use_of_tables_in_another_type_are_converted(monkeypatc
     assert c.dtype == s.dtype == torch.float32 and len(c) == len(s) == idx.numel() and at.dtype == torch.int64
     assert c.is_contiguous() and s.is_contiguous() and at.shape == idx.shape
     assert torch.equal(c[at], cos[idx].float()) and torch.equal(s[at], sin[idx].float())
+
+
+@pytest.mark.parametrize("before", [0.0, float("nan")])
+def test_weights_that_say_nothing_are_not_an_answer(before):
+    """Asked before its weights are there, a norm runs its own code, and is asked again."""
+    q, k = Centered(fill=before), Centered(fill=before)
+    assert _of(q, k) is None
+    for norm in (q, k):
+        norm.weight.data.fill_(1.0)
+    assert _of(q, k) is None
+    q, k = Norm(fill=before), Norm(fill=before)
+    assert _of(q, k) is None
+    for norm in (q, k):
+        norm.weight.data.fill_(1.0)
+    assert _of(q, k) is not None

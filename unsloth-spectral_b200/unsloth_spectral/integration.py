@@ -130,6 +130,8 @@ def _is_plain_rms(norm, weight: torch.Tensor, eps: float) -> bool:
         return known[1]
     if weight.is_cuda and torch.cuda.is_current_stream_capturing():
         return False
+    if not bool(torch.isfinite(weight).all() & weight.any()):
+        return False       # weights that are not there yet say nothing: it is asked again
     D, info = weight.numel(), torch.finfo(weight.dtype)
     ramp = torch.linspace(0.25, 2.0, D, dtype=torch.float64)
     sign = 1.0 - 2.0 * (torch.arange(D) % 3 == 1).double()
