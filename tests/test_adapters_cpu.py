@@ -192,3 +192,16 @@ def test_a_refused_adapter_leaves_the_one_in_the_slot(bad):
     for slot in (-1, 2):
         with pytest.raises(IndexError):
             ad.load(slot, good)
+
+
+def test_a_module_whose_adapters_were_taken_off_by_hand_is_not_covered():
+    model = _model()
+    ad = LoraAdapters(model, max_rank=4, slots=2, targets=("q_proj",))
+    assert ad.covers(model) and not ad.covers(_model(1))
+    model.model.layers[1].self_attn.spx_lora = None
+    assert not ad.covers(model)
+    other = LoraAdapters(_model(2), max_rank=4, slots=2, targets=("q_proj",))
+    model.model.layers[1].self_attn.spx_lora = (other, {})
+    ad.detach()
+    assert model.model.layers[0].self_attn.spx_lora is None
+    assert model.model.layers[1].self_attn.spx_lora[0] is other      # what another set holds stays

@@ -249,14 +249,18 @@ class LoraAdapters:
         take another set."""
         self.batch = None
         for module in self._modules or ():
-            module.spx_lora = None
+            if self._holds(module):
+                module.spx_lora = None
         self._modules = None
 
     def covers(self, model) -> bool:
         """Whether ``model`` is the one that this set is on: each of its modules, and no set since
         detached."""
         there = {id(m) for layer in model.model.layers for m in (layer.self_attn, getattr(layer, "mlp", None))}
-        return self._modules is not None and all(id(m) in there and m.spx_lora[0] is self for m in self._modules)
+        return self._modules is not None and all(id(m) in there and self._holds(m) for m in self._modules)
+
+    def _holds(self, module) -> bool:
+        return module.spx_lora is not None and module.spx_lora[0] is self
 
     def load(self, slot: int, weights: Dict[Tuple[int, str], Tuple[torch.Tensor, torch.Tensor]], scale: float = 1.0):
         """Put an adapter into a slot, in place of what it held: ``{(layer, projection): (A, B)}``
